@@ -20,7 +20,8 @@ from .parallel.program import Program, ProgramError, list_algorithms, cached_pro
 __all__ = ["Program", "ProgramError", "list_algorithms", "cached_program", "Communicator", "CollectiveError",
            "all_reduce", "reduce_scatter", "all_gather", "all_to_all", "gather",
            "allgather_radix_batch", "reduce_scatter_radix_batch", "all_reduce_radix_batch",
-           "all_reduce_host", "HostAllReduce", "TwoLevel", "DeviceLevel", "LibraryLevel", "GlooLevel", "split_world"]
+           "all_reduce_host", "HostAllReduce", "TwoLevel", "DeviceLevel", "LibraryLevel", "GlooLevel", "split_world",
+           "linear_cross_entropy", "check_operators", "OperatorError"]
 
 _LAZY = {
     "Communicator": ("parallel.comm", "Communicator"),
@@ -39,6 +40,9 @@ _LAZY = {
     "DeviceLevel": ("parallel.hierarchy", "DeviceLevel"),
     "LibraryLevel": ("parallel.hierarchy", "LibraryLevel"),
     "GlooLevel": ("parallel.hierarchy", "GlooLevel"),
+    "linear_cross_entropy": ("ops.decoder", "linear_cross_entropy"),
+    "check_operators": ("ops.decoder", "check_operators"),
+    "OperatorError": ("ops.decoder", "OperatorError"),
     "split_world": ("parallel.hierarchy", "split_world"),
 }
 

@@ -1,0 +1,72 @@
+// Host side of the matrix kernels: tensor maps, and the status word that an expired wait leaves.
+#include "tc.cuh"
+
+#include <mutex>
+
+#include "../api/chb.h"
+
+namespace chb {
+namespace tc {
+
+namespace {
+__device__ unsigned int g_status = 0;
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode() {
+  // (looked up in the loaded driver: the library itself is not linked against it and loads on machines without one)
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  return fn;
+}
+}  // namespace
+
+bool make_map(CUtensorMap* m, int dtype, const void* base, int ndims, const unsigned long long* dims,
+              const unsigned long long* strides, unsigned rows) {
+  if (!encode() || ndims < 2 || ndims > 3 || rows > 256) return false;
+  cuuint64_t d[3], s[2];
+  cuuint32_t box[3] = {64, rows, 1}, one[3] = {1, 1, 1};
+  for (int i = 0; i < ndims; ++i) d[i] = dims[i] ? dims[i] : 1;
+  for (int i = 0; i + 1 < ndims; ++i) {
+    s[i] = strides[i] * 2;
+    if (d[i + 1] == 1) s[i] = 16;      // (never taken, but it has to be a legal one)
+    if (s[i] % 16 || !s[i]) return false;
+  }
+  const CUtensorMapDataType t = dtype == CHB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode()(m, t, (cuuint32_t)ndims, const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+unsigned* status_word() {
+  constexpr int kDevices = 64;
+  static std::mutex mu;
+  static unsigned* known[kDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return nullptr;
+  std::lock_guard<std::mutex> g(mu);
+  if (!known[dev]) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_status) != cudaSuccess) return nullptr;
+    known[dev] = static_cast<unsigned*>(p);
+  }
+  return known[dev];
+}
+
+}  // namespace tc
+}  // namespace chb
+
+// Status of the matrix kernels on the current device (synchronises the stream): 0, or 1 after a wait ran out; cleared.
+extern "C" int chb_matrix_status(unsigned* out, cudaStream_t stream) {
+  unsigned* p = chb::tc::status_word();
+  if (!p || !out) return CHB_ERR_ARG;
+  if (cudaMemcpyAsync(out, p, sizeof(unsigned), cudaMemcpyDeviceToHost, stream) != cudaSuccess ||
+      cudaMemsetAsync(p, 0, sizeof(unsigned), stream) != cudaSuccess || cudaStreamSynchronize(stream) != cudaSuccess)
+    return CHB_ERR_CUDA;
+  return CHB_SUCCESS;
+}
