@@ -1,5 +1,6 @@
-"""Operators of a decoder's training step as hand-written kernels, with their gradients: softmax cross entropy of a linear
-output layer without its logits (``csrc/kernels/linear_ce.cu``).
+"""Operators of a decoder's training step as hand-written kernels, with their gradients: norm of the query and key heads
+with the position rotation in the same pass (``csrc/kernels/head_rope.cu``), and softmax cross entropy of a linear output
+layer without its logits (``csrc/kernels/linear_ce.cu``).
 
 They take CUDA tensors, run on the current stream of the tensors' device, and get their workspaces from torch's allocator,
 so they can be captured into CUDA graphs.  The reference stops at the collectives
@@ -9,6 +10,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import struct
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -21,6 +24,9 @@ N.optional("chb_matrix_status", i32, [C.POINTER(C.c_uint), vp])
 N.optional("chb_linear_ce_bytes", i32, [i64, i32, i32, C.POINTER(i64), C.POINTER(i64), C.POINTER(i64)])
 N.optional("chb_linear_ce_forward", i32, [i32, vp, i64, vp, vp, i64, i32, i32, i64, i32, vp, vp, vp, vp])
 N.optional("chb_linear_ce_backward", i32, [i32, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp])
+
+N.optional("chb_head_rope_ctas", i32, [C.POINTER(i32)])
+N.optional("chb_head_rope", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, vp, i32, f32, C.c_double, i32, vp, vp, vp])
 
 _HALF = (torch.bfloat16, torch.float16)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -71,6 +77,115 @@ def check_operators(device=None):
         _check(N.lib().chb_matrix_status(C.byref(word), _stream(device)), "chb_matrix_status")
     if word.value:
         raise OperatorError("a wait inside a matrix kernel ran out")
+
+
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """[T, H, D] whose heads are contiguous and start on 16-byte boundaries (copied if they do not)."""
+    size = t.element_size()
+    if t.stride(2) == 1 and all(t.stride(i) * size % 16 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0:
+        return t
+    return _aligned(t)
+
+
+def _table(*tensors) -> bytes:
+    """Device pointers as a C array (packed bytes: a tenth of the time of a ctypes array)."""
+    return _pack_table[len(tensors)](*[0 if t is None else t.data_ptr() for t in tensors])
+
+
+_pack_table = {k: struct.Struct(f"{k}Q").pack for k in (2,)}
+_pack_strides = struct.Struct("8q").pack
+
+
+# ---------------------------------------------------------------------------------------- head norm and position rotation
+
+def _head_rope(x, dy, y, heads, w, pos, eps, base, interleaved, part=None, dw=None):
+    q, k = y
+    sx, sd = (((t.stride(0), t.stride(1)) if t is not None else (0, 0) for t in ts) for ts in (x, dy or (None, None)))
+    (a, b), (c, d) = sx
+    (e, f), (g, h) = sd
+    dev = q.device
+    with _on(dev):
+        rc = N.lib().chb_head_rope(DTYPES[q.dtype], _table(*x), _table(*dy) if dy else None, _table(q, k), _pack_strides(a, b, c, d, e, f, g, h),
+                                   q.shape[0], heads[0], heads[1], q.shape[2], _table(*w) if w else None,
+                                   DTYPES[w[0].dtype] if w else 0, pos.data_ptr() if pos is not None else None,
+                                   int(pos is not None and pos.dtype == torch.int64), eps, base, interleaved,
+                                   part.data_ptr() if part is not None else None, _table(*dw) if dw else None, _stream(dev))
+    _check(rc, "head_norm_rope")
+
+
+class _HeadNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pos, eps, base, interleaved):
+        heads = q.shape[1], k.shape[1]
+        x = _heads(q), _heads(k)
+        y = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        w = None if wq is None else (_aligned(wq), _aligned(wk))
+        if len(q):
+            _head_rope(x, None, y, heads, w, pos, eps, base, interleaved)
+        ctx.normed = w is not None
+        ctx.save_for_backward(*((q, k, wq, wk) if w else ()), *((pos,) if pos is not None else ()))
+        ctx.args = eps, base, interleaved, pos is not None
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        eps, base, interleaved, has_pos = ctx.args
+        saved = ctx.saved_tensors
+        pos = saved[-1] if has_pos else None
+        dy = _heads(gq), _heads(gk)
+        heads = gq.shape[1], gk.shape[1]
+        dx = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device), torch.empty(gk.shape, dtype=gk.dtype, device=gk.device)
+        x, w, part, dw = (None, None), None, None, None
+        if ctx.normed:
+            x, w = (_heads(saved[0]), _heads(saved[1])), (_aligned(saved[2]), _aligned(saved[3]))
+            if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+                dw = torch.empty_like(w[0]), torch.empty_like(w[1])
+                part = torch.empty(_rope_ctas(gq.device) * 2 * gq.shape[2], dtype=torch.float32, device=gq.device)
+        if len(gq):
+            _head_rope(x, dy, dx, heads, w, pos, eps, base, interleaved, part, dw)
+        elif dw:
+            dw = torch.zeros_like(w[0]), torch.zeros_like(w[1])
+        return (*dx, *(dw or (None, None)), None, None, None, None)
+
+
+@lru_cache(maxsize=None)
+def _rope_ctas(device: torch.device) -> int:
+    n = i32(0)
+    with _on(device):
+        _check(N.lib().chb_head_rope_ctas(C.byref(n)), "chb_head_rope_ctas")
+    return n.value
+
+
+def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                   positions: torch.Tensor | None = None, *, eps: float = 1e-5, base: float = 10000.0,
+                   interleaved: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of ``q`` [T, H, D] and ``k`` [T, Hk, D], then the rotation of its pairs by
+    ``positions`` [T] * ``base`` ** (-2i / D), in one pass; differentiable in ``q``, ``k`` and the weights.
+
+    bf16, fp16 or fp32; D a multiple of 8, at most 256; any strides (views of one projection's output are read in place
+    where their heads start on 16-byte boundaries).  ``q_weight``, ``k_weight`` [D]: fp32 or the type of ``q``, both or
+    neither (no norm then).  ``positions``: int32 or int64, any value; None: 0, 1, 2, ...  ``interleaved``: pair i is
+    elements 2i and 2i + 1, else i and i + D / 2.  Returns contiguous tensors of the types of ``q`` and ``k``."""
+    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and q.shape[1] > 0 and k.shape[1] > 0,
+          "head_norm_rope: q [T, H, D] and k [T, Hk, D] expected")
+    _need(q.dtype in (*_HALF, torch.float32) and k.dtype == q.dtype, "head_norm_rope: q and k have to be bf16, fp16 or fp32, and alike")
+    d = q.shape[2]
+    _need(d % 8 == 0 and 0 < d <= 256 and q.shape[0] < 1 << 31, "head_norm_rope: D has to be a multiple of 8, at most 256")
+    _need((q_weight is None) == (k_weight is None), "head_norm_rope: weights for both or for neither")
+    tensors = [q, k]
+    if q_weight is not None:
+        tensors += [q_weight, k_weight]
+        _need(all(w.shape == (d,) and w.dtype in (q.dtype, torch.float32) for w in tensors[2:]) and q_weight.dtype == k_weight.dtype,
+              "head_norm_rope: weights [D] of fp32 or the type of q expected")
+    if positions is not None:
+        tensors.append(positions)
+        _need(positions.shape == (q.shape[0],) and positions.dtype in (torch.int32, torch.int64),
+              "head_norm_rope: int32 or int64 positions [T] expected")
+    _need(base > 0 and eps >= 0, "head_norm_rope: base has to be positive, eps not negative")
+    _need(q.is_cuda and all(t.device == q.device for t in tensors), "head_norm_rope: tensors of one CUDA device expected")
+    return _HeadNormRope.apply(q, k, q_weight, k_weight, None if positions is None else positions.contiguous(), float(eps),
+                               float(base), bool(interleaved))
 
 
 # ---------------------------------------------------------------------------------------------- output layer and loss

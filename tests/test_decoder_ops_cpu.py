@@ -25,3 +25,28 @@ def zeros(*s, dtype=BF):
 def test_linear_cross_entropy_refuses(x, w, t, kw, what):
     with pytest.raises(ValueError, match=what):
         chb.linear_cross_entropy(x, w, t, **kw)
+
+
+Q, K, W = zeros(4, 2, 16), zeros(4, 1, 16), zeros(16)
+
+
+@pytest.mark.parametrize("q,k,args,kw,what", [
+    (Q, K, (), {}, "CUDA device"),
+    (Q, zeros(5, 1, 16), (), {}, "expected"),
+    (Q, zeros(4, 0, 16), (), {}, "expected"),
+    (Q, zeros(4, 1, 16, dtype=torch.float16), (), {}, "alike"),
+    (Q.double(), K.double(), (), {}, "alike"),
+    (zeros(4, 2, 12), zeros(4, 1, 12), (), {}, "multiple of 8"),
+    (zeros(4, 2, 264), zeros(4, 1, 264), (), {}, "at most 256"),
+    (Q, K, (W,), {}, "both or for neither"),
+    (Q, K, (W, zeros(8)), {}, "weights"),
+    (Q, K, (W, W.float()), {}, "weights"),
+    (Q, K, (W.half(), W.half()), {}, "weights"),
+    (Q, K, (None, None, torch.zeros(3, dtype=torch.int32)), {}, "positions"),
+    (Q, K, (None, None, torch.zeros(4)), {}, "positions"),
+    (Q, K, (), {"base": 0.0}, "base"),
+    (Q, K, (W, W), {"eps": -1.0}, "eps"),
+])
+def test_head_norm_rope_refuses(q, k, args, kw, what):
+    with pytest.raises(ValueError, match=what):
+        chb.head_norm_rope(q, k, *args, **kw)
