@@ -21,7 +21,7 @@ __all__ = ["Program", "ProgramError", "list_algorithms", "cached_program", "Comm
            "all_reduce", "reduce_scatter", "all_gather", "all_to_all", "gather",
            "allgather_radix_batch", "reduce_scatter_radix_batch", "all_reduce_radix_batch",
            "all_reduce_host", "HostAllReduce", "TwoLevel", "DeviceLevel", "LibraryLevel", "GlooLevel", "split_world",
-           "head_norm_rope", "linear_cross_entropy", "check_operators", "OperatorError"]
+           "causal_attention", "head_norm_rope", "linear_cross_entropy", "check_operators", "OperatorError"]
 
 _LAZY = {
     "Communicator": ("parallel.comm", "Communicator"),
@@ -40,6 +40,7 @@ _LAZY = {
     "DeviceLevel": ("parallel.hierarchy", "DeviceLevel"),
     "LibraryLevel": ("parallel.hierarchy", "LibraryLevel"),
     "GlooLevel": ("parallel.hierarchy", "GlooLevel"),
+    "causal_attention": ("ops.decoder", "causal_attention"),
     "head_norm_rope": ("ops.decoder", "head_norm_rope"),
     "linear_cross_entropy": ("ops.decoder", "linear_cross_entropy"),
     "check_operators": ("ops.decoder", "check_operators"),

@@ -1,0 +1,872 @@
+// Causal attention over packed sequences with grouped heads, and its gradients, on the tensor cores.
+//
+//   S = Q K^T;  P_ij = exp(scale S_ij - lse_i) for j <= i of the same sequence, else 0;  O = P V
+//   D_i = dO_i . O_i;  dS = P (dO V^T - D);  dQ = scale dS K;  dK = scale dS^T Q;  dV = P^T dO
+//
+// A tile is 128 rows of 128 keys (or of 128 queries); a thread owns a row, so maxima and sums need no exchange.  Scores are
+// accumulators in tensor memory; P and dS go back there in 16 bits as the left operand of the second product, over the
+// scores that they came from, and never to shared or global memory.  Every operand tile is loaded once and serves as K-major
+// operand of a score product and as MN-major operand of an output product.  Three kernels:
+//
+//   forward  a CTA has two tiles of queries (neighbouring in (tile, head of the group) order, so that two heads share the
+//            keys and values where there are groups): the products of one run while the other's exponentials are taken.
+//            One pass with a running maximum; the sums are rescaled only when a maximum grows by more than 2^8.
+//   dq       a CTA has a tile of queries and walks its keys; also writes D.
+//   dkv      a CTA has a tile of keys of one key head and walks the queries of all heads of the group that see it, so
+//            gradients of shared heads are summed in the accumulators, in one order: no atomics anywhere.
+//
+// Sequences: the rows [cu[s], cu[s+1]); a CTA finds its own from the bounds, so lengths stay on the device.  Rows outside all
+// sequences get zeros.  A tile that reaches past its sequence holds the next one's rows: those are overwritten with zeros
+// where they would be summed over (a product 0 * infinity would carry them across).
+//
+// P and dS are rounded to the operands' type (as the tensor cores need them); maxima, sums, lse and D are fp32.
+#include "../api/chb.h"
+#include "common.cuh"
+#include "tc.cuh"
+
+namespace chb {
+namespace {
+
+using namespace tc;
+
+constexpr int TILE = 128;
+constexpr int kAtom = TILE * 128;        // bytes of a tile's 64 elements: 128 rows of 128 bytes
+
+struct AttnArgs {
+  const int* cu;          // null: one sequence
+  int seqs, T, heads, kv_heads, group, D;
+  float scale, scale_log2;
+  char* o;                // [T, heads, D] (written by forward, read by dq)
+  float* lse;             // [heads, T], in units of log2
+  float* delta;           // [heads, T]
+  const char* dout;       // strides in elements
+  long long dout_t, dout_h;
+  char *dq, *dk, *dv;     // contiguous
+  unsigned* status;
+};
+
+struct Work { int start, len, unit, nothing; };      // nothing: rows outside all sequences
+
+// The sequence of unit number `unit`, by one warp: prefix sums over the sequences' numbers of units (tiles, or pairs of
+// (tile, head) where `group` is not 0).
+__device__ __forceinline__ void find_work(const AttnArgs& p, int unit, int group, Work* out) {
+  const int lane = threadIdx.x & 31;
+  const int n = p.cu ? p.seqs + 2 : 1;
+  int before = 0;
+  for (int base = 0; base < n; base += 32) {
+    const int s = base + lane;
+    int a = 0, b = 0;
+    if (s < n) {
+      if (p.cu) {
+        a = s == 0 ? 0 : min(max(p.cu[s - 1], 0), p.T);
+        b = s == n - 1 ? p.T : min(max(p.cu[s], 0), p.T);
+      } else {
+        b = p.T;
+      }
+    }
+    const int len = max(b - a, 0), tiles = (len + TILE - 1) / TILE;
+    const int units = group ? (tiles * group + 1) / 2 : tiles;
+    int inc = units;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, unit < before + inc);
+    if (hit) {
+      if (lane == __ffs(hit) - 1) {
+        out->start = a;
+        out->len = len;
+        out->unit = unit - before - (inc - units);
+        out->nothing = p.cu && (s == 0 || s == n - 1);
+      }
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) out->len = 0;
+}
+
+// rows [from, 128) of a tile of `atoms` x 64 elements become zero (by one warp)
+__device__ __forceinline__ void zero_rows(char* tile, int atoms, int from) {
+  const int lane = threadIdx.x & 31;
+  for (int a = 0; a < atoms; ++a)
+    for (int i = from * 8 + lane; i < TILE * 8; i += 32) reinterpret_cast<uint4*>(tile + a * kAtom)[i] = make_uint4(0u, 0u, 0u, 0u);
+  fence_async_proxy();
+  __syncwarp();
+}
+
+// A K-major tile as operand of the k-th 16 summed elements; and an MN-major one
+__device__ __forceinline__ uint64_t along(uint64_t tile, int k) { return tile + (uint64_t)((k >> 2) * (kAtom >> 4) + (k & 3) * 2); }
+__device__ __forceinline__ uint64_t across(uint64_t tile, int k) { return tile + (uint64_t)(k * 128); }
+
+// 32 columns of an accumulator row, times a factor, to 32 elements of a row of D (those below D)
+template <typename T>
+__device__ __forceinline__ void store_cols(char* row, int col, int D, const uint32_t* r, float f) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (col + 8 * q < D) {
+      uint4 o;
+      o.x = pack2<T>(__uint_as_float(r[8 * q]) * f, __uint_as_float(r[8 * q + 1]) * f);
+      o.y = pack2<T>(__uint_as_float(r[8 * q + 2]) * f, __uint_as_float(r[8 * q + 3]) * f);
+      o.z = pack2<T>(__uint_as_float(r[8 * q + 4]) * f, __uint_as_float(r[8 * q + 5]) * f);
+      o.w = pack2<T>(__uint_as_float(r[8 * q + 6]) * f, __uint_as_float(r[8 * q + 7]) * f);
+      *reinterpret_cast<uint4*>(row + (col + 8 * q) * 2) = o;
+    }
+  }
+}
+
+__device__ __forceinline__ void zero_out(char* base, long long first, int rows, int heads, int head, int D) {
+  const int words = D / 8;
+  for (int i = threadIdx.x; i < rows * words; i += blockDim.x)
+    *reinterpret_cast<uint4*>(base + (((first + i / words) * heads + head) * D + i % words * 8) * 2) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// ------------------------------------------------------------------ forward
+constexpr int kFwdThreads = 320;      // warps 0-3 and 4-7: rows of the two tiles; 8: loads; 9: products
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+             const AttnArgs p) {
+  constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
+  extern __shared__ char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[14];
+  __shared__ uint32_t tmem_;
+  __shared__ Fault fault;
+  __shared__ Work work;
+  char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
+  const uint32_t qfull = bar0, kfull = bar0 + 16, kempty = bar0 + 32, vfull = bar0 + 48, vempty = bar0 + 64, sfull = bar0 + 80,
+                 pfull = bar0 + 96;      // (two of each; the outputs' barrier is the scores' last phase)
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  dependent_launch();
+  if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, p.group, &work);
+  __syncthreads();
+  const Work w = work;
+  if (w.len == 0) return;
+  const int kvh = blockIdx.x % p.kv_heads, nt = (w.len + TILE - 1) / TILE, total = nt * p.group;
+  // long tiles first; tile 1 is the same one of the next head, or the one before
+  int tile[2], head[2], n[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int x = 2 * w.unit + u;
+    tile[u] = x < total ? nt - 1 - x / p.group : -1;
+    head[u] = kvh * p.group + x % p.group;
+    n[u] = tile[u] + 1;
+  }
+  if (w.nothing) {
+    for (int u = 0; u < 2; ++u)
+      if (n[u]) zero_out(p.o, w.start + tile[u] * TILE, min(TILE, w.len - tile[u] * TILE), p.heads, head[u], p.D);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    fault.raised = 0;
+    fault.status = p.status;
+    for (int i = 0; i < 12; ++i) bar_init(bar0 + 8 * i, 1);
+    bar_init(pfull, 128);
+    bar_init(pfull + 8, 128);
+    bar_init_done();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_;
+  const uint32_t sq = smem, sk = smem + 2 * TB, sv = smem + 4 * TB;
+  const int ksteps = (p.D + 15) / 16;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+#pragma unroll
+        for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
+      };
+      bool ok = true;
+      for (int i = 0; i < n[0] && ok; ++i) {
+        const int s = i & 1;
+        const unsigned ph = ((i >> 1) & 1) ^ 1u;
+        if (i == 0) {
+          bar_expect(qfull, TB);
+          load_tile(sq, &mq, w.start + tile[0] * TILE, head[0], qfull);
+        }
+        if (!(ok = bar_wait(kempty + 8 * s, ph, &fault))) break;
+        bar_expect(kfull + 8 * s, TB);
+        load_tile(sk + s * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s);
+        if (i == 0 && n[1]) {
+          bar_expect(qfull + 8, TB);
+          load_tile(sq + TB, &mq, w.start + tile[1] * TILE, head[1], qfull + 8);
+        }
+        if (!(ok = bar_wait(vempty + 8 * s, ph, &fault))) break;
+        bar_expect(vfull + 8 * s, TB);
+        load_tile(sv + s * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s);
+      }
+    }
+  } else if (warp == 9) {
+    const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
+    const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
+    const auto scores = [&](int u, int i) {
+      if (lane == 0) {
+        const uint64_t a = operand(sq + u * TB), b = operand(sk + (i & 1) * TB);
+        for (int k = 0; k < ksteps; ++k) mma_ss(tmem + u * TILE, along(a, k), along(b, k), dscore, k > 0);
+        commit(sfull + 8 * u);
+      }
+      __syncwarp();
+    };
+    bool ok = bar_wait_warp(kfull, 0, &fault);
+    for (int u = 0; u < 2 && ok; ++u)
+      if (n[u]) {
+        if (!(ok = bar_wait_warp(qfull + 8 * u, 0, &fault))) break;
+        fence_after();
+        scores(u, 0);
+      }
+    if (ok && lane == 0) commit(kempty);
+    for (int i = 0; i < n[0] && ok; ++i) {
+      const int s = i & 1;
+      for (int u = 0; u < 2 && ok; ++u) {
+        if (i >= n[u]) continue;
+        if (u == 0) {
+          if (!(ok = bar_wait_warp(vfull + 8 * s, (i >> 1) & 1, &fault))) break;
+          if ((i + 1) * TILE > w.len) zero_rows(smem_p + 4 * TB + s * TB, ATOMS, w.len - i * TILE);
+          if (i + 1 < n[0] && !(ok = bar_wait_warp(kfull + 8 * (s ^ 1), ((i + 1) >> 1) & 1, &fault))) break;
+        }
+        if (!(ok = bar_wait_warp(pfull + 8 * u, i & 1, &fault))) break;
+        fence_after();
+        if (lane == 0) {
+          const uint64_t b = operand(sv + s * TB, kAtom);
+#pragma unroll
+          for (int k = 0; k < TILE / 16; ++k)
+            mma_ts(tmem + 2 * TILE + u * DP, tmem + u * TILE + 8 * k, across(b, k), dout, i > 0 || k > 0);
+        }
+        // the next scores go over P, behind the products that read it (a last commit stands for the output)
+        if (i + 1 < n[u]) scores(u, i + 1);
+        else if (lane == 0) commit(sfull + 8 * u);
+        __syncwarp();
+      }
+      if (ok && lane == 0) {
+        commit(vempty + 8 * s);
+        if (i + 1 < n[0]) commit(kempty + 8 * (s ^ 1));
+      }
+      __syncwarp();
+    }
+  } else {
+    const int u = warp >> 2, nu = n[u];
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + u * TILE + lanes, to = tmem + 2 * TILE + u * DP + lanes;
+    const int row = tile[u] * TILE + (warp & 3) * 32 + lane;
+    const float sl = p.scale_log2;
+    float ref = -INFINITY, sum = 0.f;      // (ref: the maximum that the sums are relative to, times scale log2 e)
+    bool ok = nu > 0;
+    for (int i = 0; i < nu; ++i) {
+      if (!(ok = bar_wait_warp(sfull + 8 * u, i & 1, &fault))) break;
+      fence_after();
+      uint32_t r[TILE];
+#pragma unroll
+      for (int c = 0; c < TILE; c += 32) ld32(ts + c, r + c);
+      wait_ld();
+      if (i == nu - 1) {
+#pragma unroll
+        for (int c = 0; c < TILE; ++c)
+          if (i * TILE + c > row) r[c] = __float_as_uint(-INFINITY);
+      }
+      float m4[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) m4[c] = __uint_as_float(r[c]);
+#pragma unroll
+      for (int c = 4; c < TILE; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(r[c]));
+      const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
+      if (i == 0) {
+        ref = top == -INFINITY ? 0.f : top;
+      } else if (__any_sync(0xffffffffu, top > ref + 8.f)) {
+        // (the commit that signalled these scores came behind the products of the tile before: the output rests)
+        const float next = fmaxf(ref, top), f = ex2(ref - next);
+        ref = next;
+        sum *= f;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          ld32(to + c, o);
+          wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+          st32(to + c, o);
+        }
+        wait_st();
+      }
+      float a4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float x = ex2(fmaf(__uint_as_float(r[64 * h + 2 * c]), sl, -ref)), y = ex2(fmaf(__uint_as_float(r[64 * h + 2 * c + 1]), sl, -ref));
+          a4[(2 * c) & 3] += x;
+          a4[(2 * c + 1) & 3] += y;
+          pk[c] = pack2<T>(x, y);
+        }
+        st32(ts + 32 * h, pk);
+      }
+      sum += (a4[0] + a4[1]) + (a4[2] + a4[3]);
+      wait_st();
+      fence_before();
+      bar_arrive(pfull + 8 * u);
+    }
+    if (ok && bar_wait_warp(sfull + 8 * u, nu & 1, &fault)) {
+      fence_after();
+      const bool in = row < w.len;
+      const float f = 1.f / sum;
+      if (in) p.lse[(long long)head[u] * p.T + w.start + row] = ref + log2f(sum);
+      char* out = p.o + ((long long)(w.start + row) * p.heads + head[u]) * p.D * 2;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t r[32];
+        __syncwarp();
+        ld32(to + c, r);
+        wait_ld();
+        if (in) store_cols<T>(out, c, p.D, r, f);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (fault.raised) drain_after_abort();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+// The kernel below fills the shared memory of an SM to the last kilobyte: what aligning the tiles leaves is checked.
+__device__ __forceinline__ bool fits(const char* end, const char* dynamic) {
+  unsigned size;
+  asm("mov.u32 %0, %dynamic_smem_size;" : "=r"(size));
+  return end <= dynamic + size;
+}
+
+// ------------------------------------------------------------------ backward
+// Both kernels: warps 0-7 hold the tile's rows twice, each half of the 128 columns (P and dS of a half go over the first half
+// of its scores' columns, so no thread writes where another reads); warp 8 loads, warp 9 issues the products.  Shared memory:
+// the CTA's own two tiles, three slots of the operand that is used by two products and two of the other.
+constexpr int kBwdThreads = 320;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+        const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
+  constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
+  extern __shared__ char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ float part[2][TILE];
+  __shared__ uint32_t tmem_;
+  __shared__ Fault fault;
+  __shared__ Work work;
+  char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
+  const uint32_t qfull = bar0, kfull = bar0 + 8, kempty = bar0 + 32, vfull = bar0 + 56, vempty = bar0 + 72, sfull = bar0 + 88,
+                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  dependent_launch();
+  if (warp == 0) find_work(p, blockIdx.x / p.heads, 0, &work);
+  __syncthreads();
+  const Work w = work;
+  if (w.len == 0) return;
+  const int head = blockIdx.x % p.heads, kvh = head / p.group, nt = (w.len + TILE - 1) / TILE;
+  const int tile = nt - 1 - w.unit, n = tile + 1;
+  if (w.nothing) {
+    zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    fault.raised = 0;
+    fault.status = p.status;
+    for (int i = 0; i < 16; ++i) bar_init(bar0 + 8 * i, bar0 + 8 * i == dsfull ? 256 : 1);
+    bar_init_done();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_;
+  const uint32_t sq = smem, sdo = smem + TB, sk = smem + 2 * TB, sv = smem + 5 * TB;
+  const uint32_t tdp = tmem + 2 * TILE, tdq = tmem + 3 * TILE;
+  const int ksteps = (p.D + 15) / 16;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+#pragma unroll
+        for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
+      };
+      bar_expect(qfull, 2 * TB);
+      load_tile(sq, &mq, w.start + tile * TILE, head, qfull);
+      load_tile(sdo, &mdo, w.start + tile * TILE, head, qfull);
+      for (int i = 0; i < n; ++i) {
+        const int s3 = i % 3, s2 = i & 1;
+        if (!bar_wait(kempty + 8 * s3, ((i / 3) & 1) ^ 1u, &fault)) break;
+        bar_expect(kfull + 8 * s3, TB);
+        load_tile(sk + s3 * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s3);
+        if (!bar_wait(vempty + 8 * s2, ((i >> 1) & 1) ^ 1u, &fault)) break;
+        bar_expect(vfull + 8 * s2, TB);
+        load_tile(sv + s2 * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s2);
+      }
+    }
+  } else if (warp == 9) {
+    const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
+    const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
+    // scores of tile i, over the dS of tile i - 2
+    const auto scores = [&](int i) {
+      if (!bar_wait_warp(kfull + 8 * (i % 3), (i / 3) & 1, &fault)) return false;
+      if ((i + 1) * TILE > w.len) zero_rows(smem_p + 2 * TB + (i % 3) * TB, ATOMS, w.len - i * TILE);
+      fence_after();
+      if (lane == 0) {
+        const uint64_t a = operand(sq), b = operand(sk + (i % 3) * TB);
+        for (int k = 0; k < ksteps; ++k) mma_ss(tmem + (i & 1) * TILE, along(a, k), along(b, k), dscore, k > 0);
+        commit(sfull + 8 * (i & 1));
+      }
+      __syncwarp();
+      return true;
+    };
+    const auto dprobs = [&](int i) {
+      if (!bar_wait_warp(vfull + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if ((i + 1) * TILE > w.len) zero_rows(smem_p + 5 * TB + (i & 1) * TB, ATOMS, w.len - i * TILE);
+      fence_after();
+      if (lane == 0) {
+        const uint64_t a = operand(sdo), b = operand(sv + (i & 1) * TB);
+        for (int k = 0; k < ksteps; ++k) mma_ss(tdp, along(a, k), along(b, k), dscore, k > 0);
+        commit(dpfull);
+        commit(vempty + 8 * (i & 1));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = bar_wait_warp(qfull, 0, &fault) && scores(0) && dprobs(0) && (n < 2 || scores(1));
+    for (int i = 0; i < n && ok; ++i) {
+      if (!(ok = bar_wait_warp(dsfull, i & 1, &fault))) break;
+      fence_after();
+      if (i + 1 < n && !(ok = dprobs(i + 1))) break;
+      if (lane == 0) {
+        const uint64_t b = operand(sk + (i % 3) * TB, kAtom);
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k)
+          mma_ts(tdq, tmem + (i & 1) * TILE + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, i > 0 || k > 0);
+        commit(i + 1 < n ? kempty + 8 * (i % 3) : done);
+      }
+      __syncwarp();
+      if (i + 2 < n) ok = scores(i + 2);
+    }
+  } else {
+    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane, row = tile * TILE + r0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const bool in = row < w.len;
+    const long long at = (long long)head * p.T + w.start + row;
+    float d = 0.f;
+    if (in) {
+      const uint4* o = reinterpret_cast<const uint4*>(p.o + ((long long)(w.start + row) * p.heads + head) * p.D * 2);
+      const uint4* g = reinterpret_cast<const uint4*>(p.dout + ((w.start + row) * p.dout_t + head * p.dout_h) * 2);
+#pragma unroll 4
+      for (int c = half * (DP / 16); c < (half + 1) * (DP / 16); ++c) {
+        if (c * 8 >= p.D) break;
+        const uint4 a = __ldcg(o + c), b = __ldcg(g + c);
+        const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = unpack2<T>(av[j]), y = unpack2<T>(bv[j]);
+          d = fmaf(x.x, y.x, fmaf(x.y, y.y, d));
+        }
+      }
+    }
+    part[half][r0] = d;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = part[0][r0] + part[1][r0];
+    const float lse = in ? __ldcg(p.lse + at) : 0.f;
+    if (in && half == 0) p.delta[at] = delta;
+    const float sl = p.scale_log2;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      if (!(ok = bar_wait_warp(sfull + 8 * (i & 1), (i >> 1) & 1, &fault))) break;
+      fence_after();
+      const uint32_t ts = tmem + (i & 1) * TILE + half * 64 + lanes;
+      uint32_t r[64];
+      ld32(ts, r);
+      ld32(ts + 32, r + 32);
+      wait_ld();
+#pragma unroll
+      for (int c = 0; c < 64; ++c) r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl, -lse)));
+      if (!(ok = bar_wait_warp(dpfull, i & 1, &fault))) break;
+      fence_after();
+      const int first = i == n - 1 ? row - i * TILE - half * 64 : 64;      // last column that the row sees
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t g[32], o[16];
+        ld32(tdp + half * 64 + 32 * q + lanes, g);
+        wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) g[c] = __float_as_uint(__uint_as_float(r[32 * q + c]) * (__uint_as_float(g[c]) - delta));
+        if (i == n - 1) {      // (selected: above the diagonal anything may stand)
+          const int last = row == 0 ? -1 : first;      // (a row that sees one key has a probability of 1, whatever its score)
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (32 * q + c > last) g[c] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
+        st16(ts + 16 * q, o);
+      }
+      wait_st();
+      fence_before();
+      bar_arrive(dsfull);
+    }
+    if (ok && bar_wait_warp(done, 0, &fault)) {
+      fence_after();
+      char* out = p.dq + ((long long)(w.start + row) * p.heads + head) * p.D * 2;
+#pragma unroll 1
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+        uint32_t r[32];
+        __syncwarp();
+        ld32(tdq + c + lanes, r);
+        wait_ld();
+        if (in) store_cols<T>(out, c, p.D, r, p.scale);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (fault.raised) drain_after_abort();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+         const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
+  constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
+  extern __shared__ char smem_raw[];
+  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ float2 rows[2][TILE];      // of the walked queries: lse, D
+  __shared__ uint32_t tmem_;
+  __shared__ Fault fault;
+  __shared__ Work work;
+  char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
+  const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
+                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  dependent_launch();
+  if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, 0, &work);
+  __syncthreads();
+  const Work w = work;
+  if (w.len == 0) return;
+  const int kvh = blockIdx.x % p.kv_heads, nt = (w.len + TILE - 1) / TILE;
+  const int tile = w.unit, per_head = nt - tile, n = per_head * p.group;
+  if (w.nothing) {
+    const int rows_here = min(TILE, w.len - tile * TILE);
+    zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
+    zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    fault.raised = 0;
+    fault.status = p.status;
+    if (!fits(smem_p + 7 * TB, smem_raw)) {
+      fault.raised = 1;
+      atomicExch(p.status, 1u);
+    }
+    for (int i = 0; i < 16; ++i) bar_init(bar0 + 8 * i, bar0 + 8 * i == dsfull || bar0 + 8 * i == pfull ? 256 : 1);
+    bar_init_done();
+  }
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_;
+  if (fault.raised) {
+    __syncthreads();
+    if (warp == 9) tmem_free(tmem, 512);
+    return;
+  }
+  const uint32_t sk = smem, sv = smem + TB, sq = smem + 2 * TB, sg = smem + 5 * TB;
+  const uint32_t tdp = tmem + TILE, tdv = tmem + 2 * TILE, tdk = tmem + 3 * TILE;
+  const int ksteps = (p.D + 15) / 16;
+
+  if (warp == 8) {
+    const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+#pragma unroll
+      for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
+    };
+    if (lane == 0) {
+      bar_expect(own, 2 * TB);
+      load_tile(sk, &mk, w.start + tile * TILE, kvh, own);
+      load_tile(sv, &mv, w.start + tile * TILE, kvh, own);
+    }
+    for (int i = 0; i < n; ++i) {
+      const int s3 = i % 3, s2 = i & 1, head = kvh * p.group + i / per_head, q0 = (tile + i % per_head) * TILE;
+      if (!bar_wait_warp(qempty + 8 * s3, ((i / 3) & 1) ^ 1u, &fault)) break;
+      if (lane == 0) {
+        bar_expect(qfull + 8 * s3, TB);
+        load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
+      }
+      if (!bar_wait_warp(gempty + 8 * s2, ((i >> 1) & 1) ^ 1u, &fault)) break;
+      // lse and D of the queries; behind the sequence's end P becomes 0
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = lane + 32 * j;
+        const long long at = (long long)head * p.T + w.start + q0 + r;
+        const bool in = q0 + r < w.len;
+        rows[s2][r] = make_float2(in ? __ldcg(p.lse + at) : INFINITY, in ? __ldcg(p.delta + at) : 0.f);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        bar_expect(gfull + 8 * s2, TB);
+        load_tile(sg + s2 * TB, &mdo, w.start + q0, head, gfull + 8 * s2);
+      }
+    }
+  } else if (warp == 9) {
+    const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
+    const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
+    const auto past = [&](int i) { return (tile + i % per_head + 1) * TILE - w.len; };      // rows behind the sequence's end
+    const auto scores = [&](int i) {
+      if (!bar_wait_warp(qfull + 8 * (i % 3), (i / 3) & 1, &fault)) return false;
+      if (past(i) > 0) zero_rows(smem_p + 2 * TB + (i % 3) * TB, ATOMS, TILE - past(i));
+      fence_after();
+      if (lane == 0) {
+        const uint64_t a = operand(sk), b = operand(sq + (i % 3) * TB);
+        for (int k = 0; k < ksteps; ++k) mma_ss(tmem, along(a, k), along(b, k), dscore, k > 0);
+        commit(sfull);
+      }
+      __syncwarp();
+      return true;
+    };
+    const auto dprobs = [&](int i) {
+      if (!bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (past(i) > 0) zero_rows(smem_p + 5 * TB + (i & 1) * TB, ATOMS, TILE - past(i));
+      fence_after();
+      if (lane == 0) {
+        const uint64_t a = operand(sv), b = operand(sg + (i & 1) * TB);
+        for (int k = 0; k < ksteps; ++k) mma_ss(tdp, along(a, k), along(b, k), dscore, k > 0);
+        commit(dpfull);
+      }
+      __syncwarp();
+      return true;
+    };
+    const auto outputs = [&](uint32_t acc, uint32_t a, uint32_t tile_addr, bool add) {
+      const uint64_t b = operand(tile_addr, kAtom);
+#pragma unroll
+      for (int k = 0; k < TILE / 16; ++k) mma_ts(acc, a + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, add || k > 0);
+    };
+    bool ok = bar_wait_warp(own, 0, &fault) && scores(0) && dprobs(0);
+    for (int i = 0; i < n && ok; ++i) {
+      if (!(ok = bar_wait_warp(pfull, i & 1, &fault))) break;
+      fence_after();
+      if (lane == 0) outputs(tdv, tmem, sg + (i & 1) * TB, i > 0);
+      __syncwarp();
+      if (i + 1 < n && !(ok = scores(i + 1))) break;
+      if (!(ok = bar_wait_warp(dsfull, i & 1, &fault))) break;
+      fence_after();
+      if (lane == 0) {
+        commit(gempty + 8 * (i & 1));      // dO, lse and D of tile i are no longer read
+        outputs(tdk, tdp, sq + (i % 3) * TB, i > 0);
+        commit(i + 1 < n ? qempty + 8 * (i % 3) : done);
+      }
+      __syncwarp();
+      if (i + 1 < n) ok = dprobs(i + 1);
+    }
+  } else {
+    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane, row = tile * TILE + r0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + half * 64 + lanes, tp = tdp + half * 64 + lanes;
+    const float sl = p.scale_log2;
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const float2* rw = rows[i & 1] + half * 64;
+      if (!(ok = bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault) && bar_wait_warp(sfull, i & 1, &fault))) break;
+      fence_after();
+      const bool diagonal = i % per_head == 0;
+      const int first = r0 - half * 64;      // first column (query) of this half that sees the row (key)
+      uint32_t r[64];
+      ld32(ts, r);
+      ld32(ts + 32, r + 32);
+      wait_ld();
+#pragma unroll
+      for (int c = 0; c < 64; ++c) r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl, -rw[c].x)));
+      if (diagonal) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < first) r[c] = 0u;
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t o[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(r[32 * q + 2 * c]), __uint_as_float(r[32 * q + 2 * c + 1]));
+        st16(ts + 16 * q, o);
+      }
+      wait_st();
+      fence_before();
+      bar_arrive(pfull);
+      if (!(ok = bar_wait_warp(dpfull, i & 1, &fault))) break;
+      fence_after();
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t g[32], o[16];
+        ld32(tp + 32 * q, g);
+        wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) g[c] = __float_as_uint(__uint_as_float(r[32 * q + c]) * (__uint_as_float(g[c]) - rw[32 * q + c].y));
+        if (diagonal) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (32 * q + c < first) g[c] = 0u;
+          if (tile == 0 && half == 0 && q == 0) g[0] = 0u;      // (the first query sees one key: its probability is 1)
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
+        st16(tp + 16 * q, o);
+      }
+      wait_st();
+      fence_before();
+      bar_arrive(dsfull);
+    }
+    if (ok && bar_wait_warp(done, 0, &fault)) {
+      fence_after();
+      const bool in = row < w.len;
+      const long long at = ((long long)(w.start + row) * p.kv_heads + kvh) * p.D * 2;
+#pragma unroll 1
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+        uint32_t r[32];
+        __syncwarp();
+        ld32(tdv + c + lanes, r);
+        wait_ld();
+        if (in) store_cols<T>(p.dv + at, c, p.D, r, 1.f);
+        __syncwarp();
+        ld32(tdk + c + lanes, r);
+        wait_ld();
+        if (in) store_cols<T>(p.dk + at, c, p.D, r, p.scale);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (fault.raised) drain_after_abort();
+  if (warp == 9) tmem_free(tmem, 512);
+}
+
+// ------------------------------------------------------------------ host side
+bool map3(CUtensorMap* m, int dtype, const void* base, long long T, int heads, int D, long long st, long long sh) {
+  const unsigned long long d[3] = {(unsigned long long)D, (unsigned long long)T, (unsigned long long)heads};
+  const unsigned long long s[2] = {(unsigned long long)st, (unsigned long long)sh};
+  return make_map(m, dtype, base, 3, d, s, TILE);
+}
+
+template <typename K, typename... A>
+cudaError_t launch(K kernel, int smem, dim3 grid, int threads, cudaStream_t stream, A... args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Units (tiles, or pairs of (tile, head)) that T rows in so many sequences can make at most; each sequence has a tile more than
+// its rows fill, and there may be rows before the first and behind the last.
+long long most_units(long long T, int seqs, bool bounds, int group) {
+  long long s = bounds ? seqs + 2ll : 1;
+  if (s > T) s = T;
+  const long long tiles = T / TILE + s;
+  return group ? (tiles * group + s) / 2 : tiles;
+}
+
+bool args_ok(int dtype, long long T, int heads, int kv_heads, int D, int seqs, float scale) {
+  return (dtype == CHB_BF16 || dtype == CHB_F16) && T >= 1 && T < (1ll << 31) - 2 * TILE && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 &&
+         heads <= 65535 && D >= 8 && D % 8 == 0 && D <= 128 && seqs >= 0 && scale > 0.f && scale < INFINITY;
+}
+
+AttnArgs common_args(long long T, int heads, int kv_heads, int D, const int* cu, int seqs, float scale) {
+  AttnArgs p{};
+  p.cu = cu;
+  p.seqs = seqs;
+  p.T = (int)T;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = heads / kv_heads;
+  p.D = D;
+  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.status = status_word();
+  return p;
+}
+
+template <typename T, int DP>
+int run_forward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaStream_t s) {
+  return launch(attn_forward<T, DP>, 6 * DP / 64 * kAtom + 1024, dim3((unsigned)(p.kv_heads * units)), kFwdThreads, s, m[0], m[1], m[2], p) ==
+                 cudaSuccess ? CHB_SUCCESS : CHB_ERR_CUDA;
+}
+template <typename T, int DP>
+int run_backward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaStream_t s) {
+  constexpr int kMost = 227 * 1024;      // of a CTA, static and dynamic
+  const int smem = 7 * DP / 64 * kAtom + 1024;
+  cudaFuncAttributes f{};
+  if (cudaFuncGetAttributes(&f, attn_dkv<T, DP>) != cudaSuccess) return CHB_ERR_CUDA;
+  const int left = kMost - (int)f.sharedSizeBytes;
+  if (launch(attn_dq<T, DP>, smem, dim3((unsigned)(p.heads * units)), kBwdThreads, s, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
+      launch(attn_dkv<T, DP>, smem < left ? smem : left, dim3((unsigned)(p.kv_heads * units)), kBwdThreads, s, m[0], m[1], m[2], m[3], p) != cudaSuccess)
+    return CHB_ERR_CUDA;
+  return CHB_SUCCESS;
+}
+
+}  // namespace
+}  // namespace chb
+
+using namespace chb;
+
+extern "C" {
+
+// q [T, heads, D], k and v [T, kv_heads, D] with strides[6] (token and head of each, in elements, multiples of 8; 16-byte aligned);
+// cu: seqs + 1 bounds on the device, or null: one sequence.  o [T, heads, D] contiguous, lse [heads, T].
+int chb_attention_forward(int dtype, const void* q, const void* k, const void* v, const long long* strides, long long T, int heads,
+                          int kv_heads, int D, const int* cu, int seqs, float scale, void* o, float* lse, cudaStream_t stream) {
+  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !strides || !o || !lse) return CHB_ERR_ARG;
+  const long long units = most_units(T, seqs, cu != nullptr, heads / kv_heads);
+  if (units * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;      // (CTAs of a launch)
+  AttnArgs p = common_args(T, heads, kv_heads, D, cu, seqs, scale);
+  p.o = static_cast<char*>(o);
+  p.lse = lse;
+  CUtensorMap m[3];
+  if (!p.status || !map3(&m[0], dtype, q, T, heads, D, strides[0], strides[1]) || !map3(&m[1], dtype, k, T, kv_heads, D, strides[2], strides[3]) ||
+      !map3(&m[2], dtype, v, T, kv_heads, D, strides[4], strides[5])) return CHB_ERR_CUDA;
+  if (dtype == CHB_F16) return D <= 64 ? run_forward<__half, 64>(m, p, units, stream) : run_forward<__half, 128>(m, p, units, stream);
+  return D <= 64 ? run_forward<__nv_bfloat16, 64>(m, p, units, stream) : run_forward<__nv_bfloat16, 128>(m, p, units, stream);
+}
+
+// strides[8]: also of dout.  delta: heads * T floats of workspace; dq, dk, dv contiguous.
+int chb_attention_backward(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout, const long long* strides,
+                           const float* lse, long long T, int heads, int kv_heads, int D, const int* cu, int seqs, float scale, float* delta,
+                           void* dq, void* dk, void* dv, cudaStream_t stream) {
+  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !o || !dout || !strides || !lse || !delta || !dq || !dk || !dv) return CHB_ERR_ARG;
+  const long long units = most_units(T, seqs, cu != nullptr, 0);
+  if (units * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;      // (CTAs of a launch)
+  AttnArgs p = common_args(T, heads, kv_heads, D, cu, seqs, scale);
+  p.o = static_cast<char*>(const_cast<void*>(o));
+  p.lse = const_cast<float*>(lse);
+  p.delta = delta;
+  p.dout = static_cast<const char*>(dout);
+  p.dout_t = strides[6];
+  p.dout_h = strides[7];
+  p.dq = static_cast<char*>(dq);
+  p.dk = static_cast<char*>(dk);
+  p.dv = static_cast<char*>(dv);
+  CUtensorMap m[4];
+  if (!p.status || !map3(&m[0], dtype, q, T, heads, D, strides[0], strides[1]) || !map3(&m[1], dtype, k, T, kv_heads, D, strides[2], strides[3]) ||
+      !map3(&m[2], dtype, v, T, kv_heads, D, strides[4], strides[5]) || !map3(&m[3], dtype, dout, T, heads, D, strides[6], strides[7])) return CHB_ERR_CUDA;
+  if (dtype == CHB_F16) return D <= 64 ? run_backward<__half, 64>(m, p, units, stream) : run_backward<__half, 128>(m, p, units, stream);
+  return D <= 64 ? run_backward<__nv_bfloat16, 64>(m, p, units, stream) : run_backward<__nv_bfloat16, 128>(m, p, units, stream);
+}
+
+}  // extern "C"

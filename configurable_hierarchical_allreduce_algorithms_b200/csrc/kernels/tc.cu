@@ -38,9 +38,18 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int ndims, const unsi
     if (s[i] % 16 || !s[i]) return false;
   }
   const CUtensorMapDataType t = dtype == CHB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return encode()(m, t, (cuuint32_t)ndims, const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const auto make = [&] {
+    return encode()(m, t, (cuuint32_t)ndims, const_cast<void*>(base), d, s, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = make();
+  if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+    // (the calling thread has no context yet: a backward pass may be the first thing that autograd's thread does)
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
+    r = make();
+  }
+  return r == CUDA_SUCCESS;
 }
 
 unsigned* status_word() {

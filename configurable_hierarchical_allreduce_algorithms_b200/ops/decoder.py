@@ -1,6 +1,7 @@
 """Operators of a decoder's training step as hand-written kernels, with their gradients: norm of the query and key heads
-with the position rotation in the same pass (``csrc/kernels/head_rope.cu``), and softmax cross entropy of a linear output
-layer without its logits (``csrc/kernels/linear_ce.cu``).
+with the position rotation in the same pass (``csrc/kernels/head_rope.cu``), causal attention over packed sequences with
+grouped heads (``csrc/kernels/attention.cu``), and softmax cross entropy of a linear output layer without its logits
+(``csrc/kernels/linear_ce.cu``).
 
 They take CUDA tensors, run on the current stream of the tensors' device, and get their workspaces from torch's allocator,
 so they can be captured into CUDA graphs.  The reference stops at the collectives
@@ -27,6 +28,8 @@ N.optional("chb_linear_ce_backward", i32, [i32, vp, vp, i64, i32, i32, i32, vp, 
 
 N.optional("chb_head_rope_ctas", i32, [C.POINTER(i32)])
 N.optional("chb_head_rope", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, vp, i32, f32, C.c_double, i32, vp, vp, vp])
+N.optional("chb_attention_forward", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp])
+N.optional("chb_attention_backward", i32, [i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp, vp, vp])
 
 _HALF = (torch.bfloat16, torch.float16)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
@@ -186,6 +189,75 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     _need(q.is_cuda and all(t.device == q.device for t in tensors), "head_norm_rope: tensors of one CUDA device expected")
     return _HeadNormRope.apply(q, k, q_weight, k_weight, None if positions is None else positions.contiguous(), float(eps),
                                float(base), bool(interleaved))
+
+
+# ------------------------------------------------------------------------------------------------------ causal attention
+
+def _strides(*tensors) -> bytes:
+    s = [x for t in tensors for x in (t.stride(0), t.stride(1))]
+    return _pack_strides(*s, *(0,) * (8 - len(s)))
+
+
+class _CausalAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, scale):
+        T, h, d = q.shape
+        o = torch.empty(T, h, d, dtype=q.dtype, device=q.device)
+        lse = torch.empty(h, T, dtype=torch.float32, device=q.device)
+        if T:
+            qs, ks, vs = _heads(q), _heads(k), _heads(v)
+            with _on(q.device):
+                rc = N.lib().chb_attention_forward(DTYPES[q.dtype], qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), _strides(qs, ks, vs), T, h,
+                                                   k.shape[1], d, cu.data_ptr() if cu is not None else None,
+                                                   cu.numel() - 1 if cu is not None else 0, scale, o.data_ptr(), lse.data_ptr(),
+                                                   _stream(q.device))
+            _check(rc, "causal_attention")
+        ctx.save_for_backward(q, k, v, o, lse, *(() if cu is None else (cu,)))
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, o, lse, *rest = ctx.saved_tensors
+        cu = rest[0] if rest else None
+        T, h, d = q.shape
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if T:
+            qs, ks, vs, g = _heads(q), _heads(k), _heads(v), _heads(grad)
+            delta = torch.empty(h, T, dtype=torch.float32, device=q.device)
+            with _on(q.device):
+                rc = N.lib().chb_attention_backward(DTYPES[q.dtype], qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), o.data_ptr(), g.data_ptr(),
+                                                    _strides(qs, ks, vs, g), lse.data_ptr(), T, h, k.shape[1], d,
+                                                    cu.data_ptr() if cu is not None else None, cu.numel() - 1 if cu is not None else 0,
+                                                    ctx.scale, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                                    _stream(q.device))
+            _check(rc, "causal_attention backward")
+        return dq, dk, dv, None, None
+
+
+def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor | None = None, *,
+                     scale: float | None = None) -> torch.Tensor:
+    """Causal softmax attention of ``q`` [T, H, D] over ``k`` and ``v`` [T, Hk, D], differentiable in all three.
+
+    bf16 or fp16; H a multiple of Hk (head h reads key head h // (H / Hk)); D a multiple of 8, at most 128; any strides
+    (views of one projection's output are read in place where their heads start on 16-byte boundaries).  ``cu_seqlens``
+    [B + 1], int32 on the same device: sequence s is the rows cu_seqlens[s] to cu_seqlens[s + 1], ascending from 0 to T at
+    most (not checked; bounds are clamped to 0 and T); lengths of zero are fine, rows outside all sequences get zeros and no
+    gradient, and no sequence is reached by what another holds, infinities and NaN included.  None: one sequence.
+    ``scale`` (default D ** -0.5) has to be positive.  Returns [T, H, D], contiguous."""
+    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
+          "causal_attention: q [T, H, D], k and v [T, Hk, D] expected")
+    _need(q.dtype in _HALF and k.dtype == q.dtype and v.dtype == q.dtype, "causal_attention: q, k and v have to be bf16 or fp16, and alike")
+    h, hk, d = q.shape[1], k.shape[1], q.shape[2]
+    _need(hk > 0 and h > 0 and h % hk == 0, "causal_attention: the number of heads has to be a multiple of the key heads'")
+    _need(d % 8 == 0 and 0 < d <= 128, "causal_attention: D has to be a multiple of 8, at most 128")
+    if cu_seqlens is not None:
+        _need(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.dtype == torch.int32, "causal_attention: int32 cu_seqlens [B + 1] expected")
+    scale = d ** -0.5 if scale is None else float(scale)
+    _need(0.0 < scale < float("inf"), "causal_attention: scale has to be positive")
+    _need(q.is_cuda and all(t.device == q.device for t in (k, v, cu_seqlens) if t is not None), "causal_attention: tensors of one CUDA device expected")
+    return _CausalAttention.apply(q, k, v, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
 
 
 # ---------------------------------------------------------------------------------------------- output layer and loss

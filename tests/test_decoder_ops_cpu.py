@@ -50,3 +50,22 @@ Q, K, W = zeros(4, 2, 16), zeros(4, 1, 16), zeros(16)
 def test_head_norm_rope_refuses(q, k, args, kw, what):
     with pytest.raises(ValueError, match=what):
         chb.head_norm_rope(q, k, *args, **kw)
+
+
+@pytest.mark.parametrize("q,k,v,cu,kw,what", [
+    (Q, K, K, None, {}, "CUDA device"),
+    (Q, K, zeros(4, 2, 16), None, {}, "expected"),
+    (Q, zeros(5, 1, 16), zeros(5, 1, 16), None, {}, "expected"),
+    (Q.float(), K.float(), K.float(), None, {}, "bf16 or fp16"),
+    (Q, K.half(), K, None, {}, "alike"),
+    (zeros(4, 3, 16), zeros(4, 2, 16), zeros(4, 2, 16), None, {}, "multiple of the key"),
+    (zeros(4, 2, 12), zeros(4, 1, 12), zeros(4, 1, 12), None, {}, "multiple of 8"),
+    (zeros(4, 2, 136), zeros(4, 1, 136), zeros(4, 1, 136), None, {}, "at most 128"),
+    (Q, K, K, torch.zeros(2, dtype=torch.int64), {}, "cu_seqlens"),
+    (Q, K, K, torch.zeros(0, dtype=torch.int32), {}, "cu_seqlens"),
+    (Q, K, K, None, {"scale": 0.0}, "scale"),
+    (Q, K, K, None, {"scale": float("nan")}, "scale"),
+])
+def test_causal_attention_refuses(q, k, v, cu, kw, what):
+    with pytest.raises(ValueError, match=what):
+        chb.causal_attention(q, k, v, cu, **kw)
