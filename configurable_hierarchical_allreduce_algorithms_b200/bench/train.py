@@ -8,6 +8,7 @@
         Llama style 1.3B decoder (24 layers, d_model 2048, 16 heads, SwiGLU 5504, seq 2048, bf16): gradient
         reduce-scatter fused with the sharded AdamW update, parameter allgather with the radix-batch kernels.
 
+``--native`` takes attention, rotation and loss from this library's kernels instead of torch's.
 ``--impl nccl`` runs the same step with torch.distributed collectives for comparison.
 Random-init weights, random token ids.  Rank 0 prints one JSON line.
 """
@@ -35,6 +36,7 @@ def main(argv=None):
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--micro-batch", type=int, default=0)
     ap.add_argument("--tiny", action="store_true", help="small model for smoke tests")
+    ap.add_argument("--native", action="store_true", help="attention, rotation and loss on this library's kernels")
     ap.add_argument("--algo", default="auto")
     ap.add_argument("--k", type=int, default=2)
     ap.add_argument("--b", type=int, default=1)
@@ -56,6 +58,7 @@ def main(argv=None):
     else:
         cfg = GPTConfig.tiny("llama") if args.tiny else GPTConfig.llama_1p3b()
         mb = args.micro_batch or (2 if args.tiny else 4)
+    cfg.native = args.native
     model = GPT(cfg).cuda().to(torch.bfloat16)
     nparam = model.num_params()
     ours = args.impl == "ours"
@@ -132,7 +135,7 @@ def main(argv=None):
     if rank == 0:
         out = {
             "metric": "tokens_per_s", "value": world * mb * T / (ms * 1e-3), "unit": "tokens/s", "n_gpus": world,
-            "mode": args.mode, "impl": args.impl, "ms_per_step": ms, "steps": args.steps, "warmup": args.warmup,
+            "mode": args.mode, "impl": args.impl, "native": args.native, "ms_per_step": ms, "steps": args.steps, "warmup": args.warmup,
             "loss": float(loss_host.item()), "params": nparam, "micro_batch": mb, "seq_len": T, "dtype": "bf16",
             "exposed_comm_ms": exposed[-1] if exposed else None,
             "collective_launches": (comm.launches - l0) if comm else None,

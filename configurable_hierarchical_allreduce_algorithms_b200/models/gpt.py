@@ -1,8 +1,10 @@
 """Decoder-only transformers used by the data-parallel and sharded-optimizer
 paths: a GPT-2 style block (LayerNorm, GELU MLP, learned positions) and a
-Llama style block (RMSNorm, SwiGLU, rotary positions).  GEMMs and attention go
-to the vendor libraries through PyTorch; this library's kernels are the
-collectives and the fused optimizer / gradient steps around them."""
+Llama style block (RMSNorm, SwiGLU, rotary positions).  GEMMs go to the vendor
+libraries through PyTorch; this library's kernels are the collectives and the
+fused optimizer / gradient steps around them and, with ``native=True`` (bf16 or
+fp16 parameters on a GPU), causal attention, the head norm with the rotation, and
+the loss of the output layer (``ops/decoder.py``)."""
 from __future__ import annotations
 
 from dataclasses import dataclass
@@ -10,6 +12,8 @@ from dataclasses import dataclass
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops import decoder
 
 
 @dataclass
@@ -21,6 +25,9 @@ class GPTConfig:
     seq_len: int = 1024
     ffn: int = 0            # 0: 4 * d_model (GPT-2); Llama style uses an explicit SwiGLU width
     style: str = "gpt2"     # "gpt2" | "llama"
+    n_kv_head: int = 0      # key / value heads, each shared by n_head / n_kv_head query heads; 0: n_head
+    qk_norm: bool = False   # RMS norm of every query and key head before the rotation (llama style)
+    native: bool = False    # attention, rotation and loss on this library's kernels
 
     @staticmethod
     def gpt2_medium():
@@ -45,11 +52,14 @@ class RMSNorm(nn.Module):
         return F.rms_norm(x, (x.shape[-1],), self.weight, self.eps)
 
 
-def _rope(q, k, base=10000.0):
-    # q, k: [B, H, T, D]
+def _rope(q, k, base=10000.0, pos=None):
+    # q, k: [B, H, T, D]; pos: [B, T], or None: 0, 1, 2, ...
     T, D = q.shape[-2], q.shape[-1]
     inv = 1.0 / (base ** (torch.arange(0, D, 2, device=q.device, dtype=torch.float32) / D))
-    ang = torch.outer(torch.arange(T, device=q.device, dtype=torch.float32), inv)
+    if pos is None:
+        ang = torch.outer(torch.arange(T, device=q.device, dtype=torch.float32), inv)
+    else:
+        ang = pos.to(torch.float32)[:, None, :, None] * inv
     cos, sin = ang.cos().to(q.dtype), ang.sin().to(q.dtype)
 
     def rot(x):
@@ -67,7 +77,9 @@ class Block(nn.Module):
         llama = cfg.style == "llama"
         self.ln1 = RMSNorm(d) if llama else nn.LayerNorm(d)
         self.ln2 = RMSNorm(d) if llama else nn.LayerNorm(d)
-        self.qkv = nn.Linear(d, 3 * d, bias=not llama)
+        self.hd, self.kv = d // cfg.n_head, cfg.n_kv_head or cfg.n_head
+        self.qkv = nn.Linear(d, d + 2 * self.kv * self.hd, bias=not llama)
+        self.q_norm, self.k_norm = (RMSNorm(self.hd), RMSNorm(self.hd)) if cfg.qk_norm and llama else (None, None)
         self.proj = nn.Linear(d, d, bias=not llama)
         if llama:
             self.gate_up = nn.Linear(d, 2 * cfg.ffn, bias=False)
@@ -76,14 +88,34 @@ class Block(nn.Module):
             self.fc = nn.Linear(d, 4 * d)
             self.down = nn.Linear(4 * d, d)
 
-    def forward(self, x):
+    def _attend(self, x, pos, cu, mask):
         B, T, d = x.shape
-        H = self.cfg.n_head
-        q, k, v = self.qkv(self.ln1(x)).view(B, T, 3, H, d // H).permute(2, 0, 3, 1, 4)
-        if self.cfg.style == "llama":
-            q, k = _rope(q, k)
-        a = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        x = x + self.proj(a.transpose(1, 2).reshape(B, T, d))
+        H, kv, hd = self.cfg.n_head, self.kv, self.hd
+        llama = self.cfg.style == "llama"
+        qkv = self.qkv(self.ln1(x))
+        if self.cfg.native:
+            q, k, v = (t.view(B * T, -1, hd) for t in qkv.view(B * T, -1).split([d, kv * hd, kv * hd], dim=1))
+            if llama:
+                norms = (None, None) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
+                q, k = decoder.head_norm_rope(q, k, *norms, pos, eps=self.q_norm.eps if self.q_norm is not None else 1e-5)
+            return decoder.causal_attention(q, k, v, cu).view(B, T, d)
+        if kv == H:
+            q, k, v = qkv.view(B, T, 3, H, hd).permute(2, 0, 3, 1, 4)
+        else:
+            q, k, v = (t.view(B, T, -1, hd).transpose(1, 2) for t in qkv.split([d, kv * hd, kv * hd], dim=2))
+        if self.q_norm is not None:
+            q, k = self.q_norm(q), self.k_norm(k)
+        if llama:
+            q, k = _rope(q, k, pos=None if pos is None else pos.view(B, T))
+        if mask is not None:             # packed sequences: the batch is one row of tokens
+            q, k, v = (t.transpose(0, 1).reshape(1, -1, B * T, hd) for t in (q, k, v))
+        a = F.scaled_dot_product_attention(q, k, v, attn_mask=mask, is_causal=mask is None, enable_gqa=kv != H)
+        if mask is not None:
+            a = a.view(H, B, T, hd).transpose(0, 1)
+        return a.transpose(1, 2).reshape(B, T, d)
+
+    def forward(self, x, pos=None, cu=None, mask=None):
+        x = x + self.proj(self._attend(x, pos, cu, mask))
         h = self.ln2(x)
         if self.cfg.style == "llama":
             g, u = self.gate_up(h).chunk(2, dim=-1)
@@ -110,14 +142,30 @@ class GPT(nn.Module):
             if getattr(m, "bias", None) is not None:
                 nn.init.zeros_(m.bias)
 
-    def forward(self, idx, targets=None):
+    def forward(self, idx, targets=None, cu_seqlens=None):
+        """``idx``, ``targets`` [B, T].  ``cu_seqlens`` (int32 [S + 1], from 0 to B * T): documents packed into the B * T
+        tokens, each with positions from 0 (learned positions: the last one stands for all beyond) and attention of its own;
+        None: every row of the batch is one."""
         B, T = idx.shape
+        native, cu, pos, mask = self.cfg.native, cu_seqlens, None, None
+        rows = torch.arange(B * T, device=idx.device) if native or cu is not None else None
+        if cu is not None:
+            seq = (torch.searchsorted(cu, rows, right=True) - 1).clamp(min=0)
+            pos = rows - cu[seq]
+            if not native:
+                mask = (seq[:, None] == seq[None]) & (rows[:, None] >= rows[None])
+        elif native:
+            pos = rows % T
+            cu = torch.arange(0, B * T + 1, T, device=idx.device, dtype=torch.int32)
         x = self.wte(idx)
         if self.wpe is not None:
-            x = x + self.wpe(torch.arange(T, device=idx.device))
+            x = x + (self.wpe(torch.arange(T, device=idx.device)) if cu_seqlens is None else self.wpe(pos.clamp(0, self.cfg.seq_len - 1)).view(B, T, -1))
         for blk in self.blocks:
-            x = blk(x)
-        logits = F.linear(self.ln_f(x), self.wte.weight)    # tied output embedding
+            x = blk(x, pos, cu, mask)
+        x = self.ln_f(x)
+        if targets is not None and native:
+            return decoder.linear_cross_entropy(x, self.wte.weight, targets)
+        logits = F.linear(x, self.wte.weight)    # tied output embedding
         if targets is None:
             return logits
         return F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.view(-1))
