@@ -123,7 +123,11 @@ __device__ __forceinline__ void zero_out(char* base, long long first, int rows, 
 }
 
 // ------------------------------------------------------------------ forward
-constexpr int kFwdThreads = 320;      // warps 0-3 and 4-7: rows of the two tiles; 8: loads; 9: products
+// Warps 0-3 and 4-7: rows of the two tiles; 8: loads; 9 and 10: products of the two tiles (one thread each); 11: zeros.
+// What bounds the kernel is the chain score -> softmax -> product of one tile, so nothing waits that need not: each tile has
+// a thread of its own for its products, P is handed over in halves, and the code of a turn is kept small (packed fp32
+// arithmetic, three-way maxima), as four warps' turns through a long one evict the other warps' instructions.
+constexpr int kFwdThreads = 384;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -131,14 +135,14 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
              const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[14];
+  __shared__ __align__(8) unsigned long long bars[18];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   __shared__ Work work;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t qfull = bar0, kfull = bar0 + 16, kempty = bar0 + 32, vfull = bar0 + 48, vempty = bar0 + 64, sfull = bar0 + 80,
-                 pfull = bar0 + 96;      // (two of each; the outputs' barrier is the scores' last phase)
+                 pfull = bar0 + 96, vready = bar0 + 128;      // (two of each, of P's halves four; the outputs are the scores' last phase)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, p.group, &work);
@@ -160,12 +164,17 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       if (n[u]) zero_out(p.o, w.start + tile[u] * TILE, min(TILE, w.len - tile[u] * TILE), p.heads, head[u], p.D);
     return;
   }
+  const bool ragged = n[0] * TILE > w.len;      // the last tile of keys reaches past the sequence
   if (threadIdx.x == 0) {
     fault.raised = 0;
     fault.status = p.status;
-    for (int i = 0; i < 12; ++i) bar_init(bar0 + 8 * i, 1);
-    bar_init(pfull, 128);
-    bar_init(pfull + 8, 128);
+    for (int i = 0; i < 18; ++i) bar_init(bar0 + 8 * i, 1);
+    for (int i = 0; i < 4; ++i) bar_init(pfull + 8 * i, 128);
+    const int tiles = n[1] ? 2 : 1;
+    for (int i = 0; i < 2; ++i) {
+      bar_init(kempty + 8 * i, tiles);
+      bar_init(vempty + 8 * i, tiles + ragged);
+    }
     bar_init_done();
   }
   if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
@@ -174,96 +183,113 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
   fence_after();
   const uint32_t tmem = tmem_;
   const uint32_t sq = smem, sk = smem + 2 * TB, sv = smem + 4 * TB;
-  const int ksteps = (p.D + 15) / 16;
 
   if (warp == 8) {
-    if (lane == 0) {
-      const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+    const bool one = elect();
+    const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+      if (one) {
+        bar_expect(bar, TB);
 #pragma unroll
         for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
-      };
-      bool ok = true;
-      for (int i = 0; i < n[0] && ok; ++i) {
-        const int s = i & 1;
-        const unsigned ph = ((i >> 1) & 1) ^ 1u;
-        if (i == 0) {
-          bar_expect(qfull, TB);
-          load_tile(sq, &mq, w.start + tile[0] * TILE, head[0], qfull);
-        }
-        if (!(ok = bar_wait(kempty + 8 * s, ph, &fault))) break;
-        bar_expect(kfull + 8 * s, TB);
-        load_tile(sk + s * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s);
-        if (i == 0 && n[1]) {
-          bar_expect(qfull + 8, TB);
-          load_tile(sq + TB, &mq, w.start + tile[1] * TILE, head[1], qfull + 8);
-        }
-        if (!(ok = bar_wait(vempty + 8 * s, ph, &fault))) break;
-        bar_expect(vfull + 8 * s, TB);
-        load_tile(sv + s * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s);
-      }
-    }
-  } else if (warp == 9) {
-    const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
-    const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
-    const auto scores = [&](int u, int i) {
-      if (lane == 0) {
-        const uint64_t a = operand(sq + u * TB), b = operand(sk + (i & 1) * TB);
-        for (int k = 0; k < ksteps; ++k) mma_ss(tmem + u * TILE, along(a, k), along(b, k), dscore, k > 0);
-        commit(sfull + 8 * u);
       }
       __syncwarp();
     };
-    bool ok = bar_wait_warp(kfull, 0, &fault);
-    for (int u = 0; u < 2 && ok; ++u)
-      if (n[u]) {
-        if (!(ok = bar_wait_warp(qfull + 8 * u, 0, &fault))) break;
-        fence_after();
-        scores(u, 0);
-      }
-    if (ok && lane == 0) commit(kempty);
-    for (int i = 0; i < n[0] && ok; ++i) {
+    load_tile(sq, &mq, w.start + tile[0] * TILE, head[0], qfull);
+    for (int i = 0; i < n[0]; ++i) {
       const int s = i & 1;
-      for (int u = 0; u < 2 && ok; ++u) {
-        if (i >= n[u]) continue;
-        if (u == 0) {
-          if (!(ok = bar_wait_warp(vfull + 8 * s, (i >> 1) & 1, &fault))) break;
-          if ((i + 1) * TILE > w.len) zero_rows(smem_p + 4 * TB + s * TB, ATOMS, w.len - i * TILE);
-          if (i + 1 < n[0] && !(ok = bar_wait_warp(kfull + 8 * (s ^ 1), ((i + 1) >> 1) & 1, &fault))) break;
-        }
-        if (!(ok = bar_wait_warp(pfull + 8 * u, i & 1, &fault))) break;
-        fence_after();
-        if (lane == 0) {
-          const uint64_t b = operand(sv + s * TB, kAtom);
+      const unsigned ph = ((i >> 1) & 1) ^ 1u;
+      if (!bar_wait_warp(kempty + 8 * s, ph, &fault)) break;
+      load_tile(sk + s * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s);
+      if (i == 0 && n[1]) load_tile(sq + TB, &mq, w.start + tile[1] * TILE, head[1], qfull + 8);
+      if (!bar_wait_warp(vempty + 8 * s, ph, &fault)) break;
+      load_tile(sv + s * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s);
+    }
+  } else if (warp == 11) {
+    // where the last tile is ragged every tile of values goes through this warp's hands (it keeps its place in the ring so)
+    for (int i = 0; i < n[0] && ragged; ++i) {
+      const int s = i & 1;
+      if (!bar_wait_warp(vfull + 8 * s, (i >> 1) & 1, &fault)) break;
+      if (i == n[0] - 1) zero_rows(smem_p + 4 * TB + s * TB, ATOMS, w.len - i * TILE);
+      if (lane == 0) {
+        bar_arrive(vready + 8 * s);
+        bar_arrive(vempty + 8 * s);
+      }
+    }
+  } else if (warp >= 9) {
+    const int u = warp - 9, nu = n[u];
+    if (nu) {
+      const bool one = elect();
+      const int ksteps = (p.D + 15) / 16;
+      const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
+      const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
+      const uint32_t ts = tmem + u * TILE, to = tmem + 2 * TILE + u * DP, ready = sfull + 8 * u, pf = pfull + 16 * u,
+                     values = ragged ? vready : vfull;
+      const uint64_t a = operand(sq + u * TB), k0 = operand(sk), v0 = operand(sv, kAtom);
+      const auto scores = [&](int s) {
+        const uint64_t b = k0 + (uint64_t)(s * (TB >> 4));
+        if (one) {
 #pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)
-            mma_ts(tmem + 2 * TILE + u * DP, tmem + u * TILE + 8 * k, across(b, k), dout, i > 0 || k > 0);
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < ksteps) mma_ss(ts, along(a, k), along(b, k), dscore, k > 0);
+          commit(ready);
+          commit(kempty + 8 * s);
         }
-        // the next scores go over P, behind the products that read it (a last commit stands for the output)
-        if (i + 1 < n[u]) scores(u, i + 1);
-        else if (lane == 0) commit(sfull + 8 * u);
+        __syncwarp();
+      };
+      bool ok = bar_wait_warp(qfull + 8 * u, 0, &fault) && bar_wait_warp(kfull, 0, &fault);
+      if (ok) scores(0);
+#pragma unroll 1
+      for (int i = 0; i < nu && ok; ++i) {
+        const int s = i & 1;
+        const uint64_t b = v0 + (uint64_t)(s * (TB >> 4));
+        if (!(ok = bar_wait_warp(values + 8 * s, (i >> 1) & 1, &fault))) break;
+        if (!(ok = bar_wait_warp(pf, i & 1, &fault))) break;
+        fence_after();
+        if (one) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ts(to, ts + 8 * k, across(b, k), dout, i > 0 || k > 0);
+        }
+        __syncwarp();
+        // (the wait for the next keys comes before the one for the second half of P: it is over by then)
+        if (i + 1 < nu && !(ok = bar_wait_warp(kfull + 8 * (s ^ 1), ((i + 1) >> 1) & 1, &fault))) break;
+        if (!(ok = bar_wait_warp(pf + 8, i & 1, &fault))) break;
+        fence_after();
+        if (one) {
+#pragma unroll
+          for (int k = 4; k < 8; ++k) mma_ts(to, ts + 8 * k, across(b, k), dout, true);
+        }
+        __syncwarp();
+        // the next scores go over P, behind the products that read it
+        if (i + 1 < nu) scores(s ^ 1);
+        else if (one) commit(ready);      // (stands for the output)
+        __syncwarp();
+        if (one) commit(vempty + 8 * s);
         __syncwarp();
       }
-      if (ok && lane == 0) {
-        commit(vempty + 8 * s);
-        if (i + 1 < n[0]) commit(kempty + 8 * (s ^ 1));
+      if (ok && nu < n[0] && bar_wait_warp(kfull + 8 * (nu & 1), (nu >> 1) & 1, &fault)) {
+        // tile 1 ends one turn before tile 0: its last arrivals
+        if (one) bar_arrive(kempty + 8 * (nu & 1));
+        if (bar_wait_warp(vfull + 8 * (nu & 1), (nu >> 1) & 1, &fault) && one) bar_arrive(vempty + 8 * (nu & 1));
       }
-      __syncwarp();
     }
   } else {
     const int u = warp >> 2, nu = n[u];
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + u * TILE + lanes, to = tmem + 2 * TILE + u * DP + lanes;
+    const uint32_t ts = tmem + u * TILE + lanes, to = tmem + 2 * TILE + u * DP + lanes, ready = sfull + 8 * u, pf = pfull + 16 * u;
     const int row = tile[u] * TILE + (warp & 3) * 32 + lane;
     const float sl = p.scale_log2;
-    float ref = -INFINITY, sum = 0.f;      // (ref: the maximum that the sums are relative to, times scale log2 e)
+    const uint64_t sl2 = pair(sl, sl);
+    float ref = 0.f;                       // the maximum that the sums are relative to, times scale log2 e
+    uint64_t sum2[2] = {0ull, 0ull};       // (two zeros each)
     bool ok = nu > 0;
+#pragma unroll 1
     for (int i = 0; i < nu; ++i) {
-      if (!(ok = bar_wait_warp(sfull + 8 * u, i & 1, &fault))) break;
+      if (!(ok = bar_wait_warp(ready, i & 1, &fault))) break;
       fence_after();
       uint32_t r[TILE];
 #pragma unroll
       for (int c = 0; c < TILE; c += 32) ld32(ts + c, r + c);
-      wait_ld();
+      wait_ld(r);
       if (i == nu - 1) {
 #pragma unroll
         for (int c = 0; c < TILE; ++c)
@@ -271,50 +297,52 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       }
       float m4[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) m4[c] = __uint_as_float(r[c]);
+      for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
 #pragma unroll
-      for (int c = 4; c < TILE; ++c) m4[c & 3] = fmaxf(m4[c & 3], __uint_as_float(r[c]));
-      const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sl;
+      for (int c = 4; c < TILE / 2; ++c) m4[c & 3] = max3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      const float top = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * sl;
       if (i == 0) {
         ref = top == -INFINITY ? 0.f : top;
       } else if (__any_sync(0xffffffffu, top > ref + 8.f)) {
         // (the commit that signalled these scores came behind the products of the tile before: the output rests)
         const float next = fmaxf(ref, top), f = ex2(ref - next);
+        const uint64_t f2 = pair(f, f);
         ref = next;
-        sum *= f;
+        sum2[0] = mul2(sum2[0], f2);
+        sum2[1] = mul2(sum2[1], f2);
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
           ld32(to + c, o);
-          wait_ld();
+          wait_ld(o);
 #pragma unroll
           for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
           st32(to + c, o);
         }
         wait_st();
       }
-      float a4[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t nref2 = pair(-ref, -ref);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t pk[32];
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          const float x = ex2(fmaf(__uint_as_float(r[64 * h + 2 * c]), sl, -ref)), y = ex2(fmaf(__uint_as_float(r[64 * h + 2 * c + 1]), sl, -ref));
-          a4[(2 * c) & 3] += x;
-          a4[(2 * c + 1) & 3] += y;
+          const float2 t = unpair(fma2(pair(r[64 * h + 2 * c], r[64 * h + 2 * c + 1]), sl2, nref2));
+          const float x = ex2(t.x), y = ex2(t.y);
+          sum2[c & 1] = add2(sum2[c & 1], pair(x, y));
           pk[c] = pack2<T>(x, y);
         }
         st32(ts + 32 * h, pk);
+        wait_st();
+        fence_before();
+        bar_arrive(pf + 8 * h);
       }
-      sum += (a4[0] + a4[1]) + (a4[2] + a4[3]);
-      wait_st();
-      fence_before();
-      bar_arrive(pfull + 8 * u);
     }
-    if (ok && bar_wait_warp(sfull + 8 * u, nu & 1, &fault)) {
+    if (ok && bar_wait_warp(ready, nu & 1, &fault)) {
       fence_after();
+      const float2 a = unpair(add2(sum2[0], sum2[1]));
+      const float sum = a.x + a.y, f = 1.f / sum;
       const bool in = row < w.len;
-      const float f = 1.f / sum;
       if (in) p.lse[(long long)head[u] * p.T + w.start + row] = ref + log2f(sum);
       char* out = p.o + ((long long)(w.start + row) * p.heads + head[u]) * p.D * 2;
 #pragma unroll 1
@@ -322,7 +350,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
         uint32_t r[32];
         __syncwarp();
         ld32(to + c, r);
-        wait_ld();
+        wait_ld(r);
         if (in) store_cols<T>(out, c, p.D, r, f);
       }
     }
@@ -343,9 +371,20 @@ __device__ __forceinline__ bool fits(const char* end, const char* dynamic) {
 
 // ------------------------------------------------------------------ backward
 // Both kernels: warps 0-7 hold the tile's rows twice, each half of the 128 columns (P and dS of a half go over the first half
-// of its scores' columns, so no thread writes where another reads); warp 8 loads, warp 9 issues the products.  Shared memory:
-// the CTA's own two tiles, three slots of the operand that is used by two products and two of the other.
-constexpr int kBwdThreads = 320;
+// of its scores' columns, so no thread writes where another reads); warp 8 loads, a thread of warp 9 issues the products,
+// warp 10 writes the zeros.  Shared memory: the CTA's own two tiles, three slots of the operand that is used by two products
+// and two of the other.
+constexpr int kBwdThreads = 352;
+
+// 64 scores of a row: P = exp2(scale S - lse)
+__device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_t nlse2) {
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const float2 t = unpair(fma2(pair(r[2 * c], r[2 * c + 1]), sl2, nlse2));
+    r[2 * c] = __float_as_uint(ex2(t.x));
+    r[2 * c + 1] = __float_as_uint(ex2(t.y));
+  }
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -353,7 +392,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[16];
+  __shared__ __align__(8) unsigned long long bars[18];
   __shared__ float part[2][TILE];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
@@ -361,7 +400,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t qfull = bar0, kfull = bar0 + 8, kempty = bar0 + 32, vfull = bar0 + 56, vempty = bar0 + 72, sfull = bar0 + 88,
-                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120;
+                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.heads, 0, &work);
@@ -374,10 +413,15 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
     zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D);
     return;
   }
+  const bool ragged = n * TILE > w.len;
   if (threadIdx.x == 0) {
     fault.raised = 0;
     fault.status = p.status;
-    for (int i = 0; i < 16; ++i) bar_init(bar0 + 8 * i, bar0 + 8 * i == dsfull ? 256 : 1);
+    for (int i = 0; i < 18; ++i) bar_init(bar0 + 8 * i, 1);
+    bar_init(qfull, 2);      // Q and dO
+    for (int i = 0; i < 3; ++i) bar_init(kempty + 8 * i, 1 + ragged);
+    for (int i = 0; i < 2; ++i) bar_init(vempty + 8 * i, 1 + ragged);
+    bar_init(dsfull, 256);
     bar_init_done();
   }
   if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
@@ -387,50 +431,69 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   const uint32_t tmem = tmem_;
   const uint32_t sq = smem, sdo = smem + TB, sk = smem + 2 * TB, sv = smem + 5 * TB;
   const uint32_t tdp = tmem + 2 * TILE, tdq = tmem + 3 * TILE;
-  const int ksteps = (p.D + 15) / 16;
 
   if (warp == 8) {
-    if (lane == 0) {
-      const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+    const bool one = elect();
+    const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+      if (one) {
+        bar_expect(bar, TB);
 #pragma unroll
         for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
-      };
-      bar_expect(qfull, 2 * TB);
-      load_tile(sq, &mq, w.start + tile * TILE, head, qfull);
-      load_tile(sdo, &mdo, w.start + tile * TILE, head, qfull);
-      for (int i = 0; i < n; ++i) {
-        const int s3 = i % 3, s2 = i & 1;
-        if (!bar_wait(kempty + 8 * s3, ((i / 3) & 1) ^ 1u, &fault)) break;
-        bar_expect(kfull + 8 * s3, TB);
-        load_tile(sk + s3 * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s3);
-        if (!bar_wait(vempty + 8 * s2, ((i >> 1) & 1) ^ 1u, &fault)) break;
-        bar_expect(vfull + 8 * s2, TB);
-        load_tile(sv + s2 * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s2);
+      }
+      __syncwarp();
+    };
+    load_tile(sq, &mq, w.start + tile * TILE, head, qfull);
+    load_tile(sdo, &mdo, w.start + tile * TILE, head, qfull);
+    for (int i = 0, s3 = 0, ph3 = 1; i < n; ++i) {
+      const int s2 = i & 1;
+      if (!bar_wait_warp(kempty + 8 * s3, ph3, &fault)) break;
+      load_tile(sk + s3 * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s3);
+      if (!bar_wait_warp(vempty + 8 * s2, ((i >> 1) & 1) ^ 1, &fault)) break;
+      load_tile(sv + s2 * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s2);
+      if (++s3 == 3) { s3 = 0; ph3 ^= 1; }
+    }
+  } else if (warp == 10) {
+    for (int i = 0; i < n && ragged; ++i) {
+      const int s3 = i % 3, s2 = i & 1;
+      if (!bar_wait_warp(kfull + 8 * s3, (i / 3) & 1, &fault) || !bar_wait_warp(vfull + 8 * s2, (i >> 1) & 1, &fault)) break;
+      if (i == n - 1) {
+        zero_rows(smem_p + 2 * TB + s3 * TB, ATOMS, w.len - i * TILE);
+        zero_rows(smem_p + 5 * TB + s2 * TB, ATOMS, w.len - i * TILE);
+      }
+      if (lane == 0) {
+        bar_arrive(ready + 8 * s2);
+        bar_arrive(kempty + 8 * s3);
+        bar_arrive(vempty + 8 * s2);
       }
     }
   } else if (warp == 9) {
+    const bool one = elect();
+    const int ksteps = (p.D + 15) / 16;
     const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
     const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
+    const uint64_t aq = operand(sq), ado = operand(sdo), k0 = operand(sk), v0 = operand(sv), kt0 = operand(sk, kAtom);
+    const uint32_t values = ragged ? ready : vfull;
+    const auto product = [&](uint32_t acc, uint64_t a, uint64_t b) {
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < ksteps) mma_ss(acc, along(a, k), along(b, k), dscore, k > 0);
+    };
     // scores of tile i, over the dS of tile i - 2
     const auto scores = [&](int i) {
-      if (!bar_wait_warp(kfull + 8 * (i % 3), (i / 3) & 1, &fault)) return false;
-      if ((i + 1) * TILE > w.len) zero_rows(smem_p + 2 * TB + (i % 3) * TB, ATOMS, w.len - i * TILE);
-      fence_after();
-      if (lane == 0) {
-        const uint64_t a = operand(sq), b = operand(sk + (i % 3) * TB);
-        for (int k = 0; k < ksteps; ++k) mma_ss(tmem + (i & 1) * TILE, along(a, k), along(b, k), dscore, k > 0);
+      const int s3 = i % 3;
+      const uint32_t bar = ragged ? ready + 8 * (i & 1) : kfull + 8 * s3;
+      if (!bar_wait_warp(bar, ragged ? (i >> 1) & 1 : (i / 3) & 1, &fault)) return false;
+      if (one) {
+        product(tmem + (i & 1) * TILE, aq, k0 + (uint64_t)(s3 * (TB >> 4)));
         commit(sfull + 8 * (i & 1));
       }
       __syncwarp();
       return true;
     };
     const auto dprobs = [&](int i) {
-      if (!bar_wait_warp(vfull + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
-      if ((i + 1) * TILE > w.len) zero_rows(smem_p + 5 * TB + (i & 1) * TB, ATOMS, w.len - i * TILE);
-      fence_after();
-      if (lane == 0) {
-        const uint64_t a = operand(sdo), b = operand(sv + (i & 1) * TB);
-        for (int k = 0; k < ksteps; ++k) mma_ss(tdp, along(a, k), along(b, k), dscore, k > 0);
+      if (!bar_wait_warp(values + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (one) {
+        product(tdp, ado, v0 + (uint64_t)((i & 1) * (TB >> 4)));
         commit(dpfull);
         commit(vempty + 8 * (i & 1));
       }
@@ -438,12 +501,13 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       return true;
     };
     bool ok = bar_wait_warp(qfull, 0, &fault) && scores(0) && dprobs(0) && (n < 2 || scores(1));
+#pragma unroll 1
     for (int i = 0; i < n && ok; ++i) {
       if (!(ok = bar_wait_warp(dsfull, i & 1, &fault))) break;
       fence_after();
       if (i + 1 < n && !(ok = dprobs(i + 1))) break;
-      if (lane == 0) {
-        const uint64_t b = operand(sk + (i % 3) * TB, kAtom);
+      const uint64_t b = kt0 + (uint64_t)((i % 3) * (TB >> 4));
+      if (one) {
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k)
           mma_ts(tdq, tmem + (i & 1) * TILE + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, i > 0 || k > 0);
@@ -478,8 +542,9 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
     const float delta = part[0][r0] + part[1][r0];
     const float lse = in ? __ldcg(p.lse + at) : 0.f;
     if (in && half == 0) p.delta[at] = delta;
-    const float sl = p.scale_log2;
+    const uint64_t sl2 = pair(p.scale_log2, p.scale_log2), nlse2 = pair(-lse, -lse), ndelta2 = pair(-delta, -delta);
     bool ok = true;
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
       if (!(ok = bar_wait_warp(sfull + 8 * (i & 1), (i >> 1) & 1, &fault))) break;
       fence_after();
@@ -487,29 +552,31 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       uint32_t r[64];
       ld32(ts, r);
       ld32(ts + 32, r + 32);
-      wait_ld();
-#pragma unroll
-      for (int c = 0; c < 64; ++c) r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl, -lse)));
+      wait_ld(r);
+      probabilities(r, sl2, nlse2);
       if (!(ok = bar_wait_warp(dpfull, i & 1, &fault))) break;
       fence_after();
-      const int first = i == n - 1 ? row - i * TILE - half * 64 : 64;      // last column that the row sees
+      uint32_t g[64];
+      ld32(tdp + half * 64 + lanes, g);
+      ld32(tdp + half * 64 + 32 + lanes, g + 32);
+      wait_ld(g);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t g[32], o[16];
-        ld32(tdp + half * 64 + 32 * q + lanes, g);
-        wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) g[c] = __float_as_uint(__uint_as_float(r[32 * q + c]) * (__uint_as_float(g[c]) - delta));
-        if (i == n - 1) {      // (selected: above the diagonal anything may stand)
-          const int last = row == 0 ? -1 : first;      // (a row that sees one key has a probability of 1, whatever its score)
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (32 * q + c > last) g[c] = 0u;
-        }
-#pragma unroll
-        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
-        st16(ts + 16 * q, o);
+      for (int c = 0; c < 32; ++c) {
+        const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), add2(pair(g[2 * c], g[2 * c + 1]), ndelta2)));
+        g[2 * c] = __float_as_uint(t.x);
+        g[2 * c + 1] = __float_as_uint(t.y);
       }
+      if (i == n - 1) {
+        // the last column that the row sees (selected: above the diagonal anything may stand); a row that sees one key has a
+        // probability of 1, whatever its score
+        const int last = row == 0 ? -1 : r0 - half * 64;
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c > last) g[c] = 0u;
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c) g[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
+      st32(ts, g);
       wait_st();
       fence_before();
       bar_arrive(dsfull);
@@ -522,7 +589,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         uint32_t r[32];
         __syncwarp();
         ld32(tdq + c + lanes, r);
-        wait_ld();
+        wait_ld(r);
         if (in) store_cols<T>(out, c, p.D, r, p.scale);
       }
     }
@@ -540,15 +607,15 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
          const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[16];
-  __shared__ float2 rows[2][TILE];      // of the walked queries: lse, D
+  __shared__ __align__(8) unsigned long long bars[18];
+  __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   __shared__ Work work;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
-                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120;
+                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, 0, &work);
@@ -563,6 +630,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
     return;
   }
+  const bool ragged = nt * TILE > w.len;      // every head's last tile of queries reaches past the sequence
   if (threadIdx.x == 0) {
     fault.raised = 0;
     fault.status = p.status;
@@ -570,7 +638,15 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       fault.raised = 1;
       atomicExch(p.status, 1u);
     }
-    for (int i = 0; i < 16; ++i) bar_init(bar0 + 8 * i, bar0 + 8 * i == dsfull || bar0 + 8 * i == pfull ? 256 : 1);
+    for (int i = 0; i < 18; ++i) bar_init(bar0 + 8 * i, 1);
+    bar_init(own, 2);        // K and V
+    for (int i = 0; i < 3; ++i) bar_init(qempty + 8 * i, 1 + ragged);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(gfull + 8 * i, 2);      // the load of dO, and lse and D
+      bar_init(gempty + 8 * i, 1 + ragged);
+    }
+    bar_init(pfull, 256);
+    bar_init(dsfull, 256);
     bar_init_done();
   }
   if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
@@ -585,142 +661,180 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   }
   const uint32_t sk = smem, sv = smem + TB, sq = smem + 2 * TB, sg = smem + 5 * TB;
   const uint32_t tdp = tmem + TILE, tdv = tmem + 2 * TILE, tdk = tmem + 3 * TILE;
-  const int ksteps = (p.D + 15) / 16;
 
   if (warp == 8) {
+    const bool one = elect();
     const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
+      if (one) {
+        bar_expect(bar, TB);
 #pragma unroll
-      for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
-    };
-    if (lane == 0) {
-      bar_expect(own, 2 * TB);
-      load_tile(sk, &mk, w.start + tile * TILE, kvh, own);
-      load_tile(sv, &mv, w.start + tile * TILE, kvh, own);
-    }
-    for (int i = 0; i < n; ++i) {
-      const int s3 = i % 3, s2 = i & 1, head = kvh * p.group + i / per_head, q0 = (tile + i % per_head) * TILE;
-      if (!bar_wait_warp(qempty + 8 * s3, ((i / 3) & 1) ^ 1u, &fault)) break;
-      if (lane == 0) {
-        bar_expect(qfull + 8 * s3, TB);
-        load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
+        for (int a = 0; a < ATOMS; ++a) load3(dst + a * kAtom, m, 64 * a, row, h, bar);
       }
-      if (!bar_wait_warp(gempty + 8 * s2, ((i >> 1) & 1) ^ 1u, &fault)) break;
-      // lse and D of the queries; behind the sequence's end P becomes 0
+      __syncwarp();
+    };
+    load_tile(sk, &mk, w.start + tile * TILE, kvh, own);
+    load_tile(sv, &mv, w.start + tile * TILE, kvh, own);
+    for (int i = 0, head = kvh * p.group, q = tile; i < n; ++i) {
+      const int s3 = i % 3, s2 = i & 1, q0 = q * TILE;
+      if (!bar_wait_warp(qempty + 8 * s3, ((i / 3) & 1) ^ 1, &fault)) break;
+      load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
+      if (!bar_wait_warp(gempty + 8 * s2, ((i >> 1) & 1) ^ 1, &fault)) break;
+      load_tile(sg + s2 * TB, &mdo, w.start + q0, head, gfull + 8 * s2);
+      // behind the sequence's end P becomes 0
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = lane + 32 * j;
         const long long at = (long long)head * p.T + w.start + q0 + r;
         const bool in = q0 + r < w.len;
-        rows[s2][r] = make_float2(in ? __ldcg(p.lse + at) : INFINITY, in ? __ldcg(p.delta + at) : 0.f);
+        nlse[s2][r] = in ? -__ldcg(p.lse + at) : -INFINITY;
+        ndelta[s2][r] = in ? -__ldcg(p.delta + at) : 0.f;
       }
       __syncwarp();
+      if (one) bar_arrive(gfull + 8 * s2);
+      if (++q == nt) {
+        q = tile;
+        ++head;
+      }
+    }
+  } else if (warp == 10) {
+    for (int i = 0, q = tile; i < n && ragged; ++i) {
+      const int s3 = i % 3, s2 = i & 1;
+      if (!bar_wait_warp(qfull + 8 * s3, (i / 3) & 1, &fault) || !bar_wait_warp(gfull + 8 * s2, (i >> 1) & 1, &fault)) break;
+      if (++q == nt) {
+        q = tile;
+        zero_rows(smem_p + 2 * TB + s3 * TB, ATOMS, w.len - (nt - 1) * TILE);
+        zero_rows(smem_p + 5 * TB + s2 * TB, ATOMS, w.len - (nt - 1) * TILE);
+      }
       if (lane == 0) {
-        bar_expect(gfull + 8 * s2, TB);
-        load_tile(sg + s2 * TB, &mdo, w.start + q0, head, gfull + 8 * s2);
+        bar_arrive(ready + 8 * s2);
+        bar_arrive(qempty + 8 * s3);
+        bar_arrive(gempty + 8 * s2);
       }
     }
   } else if (warp == 9) {
+    const bool one = elect();
+    const int ksteps = (p.D + 15) / 16;
     const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
     const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
-    const auto past = [&](int i) { return (tile + i % per_head + 1) * TILE - w.len; };      // rows behind the sequence's end
+    const uint64_t ak = operand(sk), av = operand(sv), q0 = operand(sq), g0 = operand(sg), qt0 = operand(sq, kAtom), gt0 = operand(sg, kAtom);
+    const uint32_t douts = ragged ? ready : gfull;
+    const auto product = [&](uint32_t acc, uint64_t a, uint64_t b) {
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < ksteps) mma_ss(acc, along(a, k), along(b, k), dscore, k > 0);
+    };
     const auto scores = [&](int i) {
-      if (!bar_wait_warp(qfull + 8 * (i % 3), (i / 3) & 1, &fault)) return false;
-      if (past(i) > 0) zero_rows(smem_p + 2 * TB + (i % 3) * TB, ATOMS, TILE - past(i));
-      fence_after();
-      if (lane == 0) {
-        const uint64_t a = operand(sk), b = operand(sq + (i % 3) * TB);
-        for (int k = 0; k < ksteps; ++k) mma_ss(tmem, along(a, k), along(b, k), dscore, k > 0);
+      const int s3 = i % 3;
+      const uint32_t bar = ragged ? ready + 8 * (i & 1) : qfull + 8 * s3;
+      if (!bar_wait_warp(bar, ragged ? (i >> 1) & 1 : (i / 3) & 1, &fault)) return false;
+      if (one) {
+        product(tmem, ak, q0 + (uint64_t)(s3 * (TB >> 4)));
         commit(sfull);
       }
       __syncwarp();
       return true;
     };
     const auto dprobs = [&](int i) {
-      if (!bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
-      if (past(i) > 0) zero_rows(smem_p + 5 * TB + (i & 1) * TB, ATOMS, TILE - past(i));
-      fence_after();
-      if (lane == 0) {
-        const uint64_t a = operand(sv), b = operand(sg + (i & 1) * TB);
-        for (int k = 0; k < ksteps; ++k) mma_ss(tdp, along(a, k), along(b, k), dscore, k > 0);
+      if (!bar_wait_warp(douts + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (one) {
+        product(tdp, av, g0 + (uint64_t)((i & 1) * (TB >> 4)));
         commit(dpfull);
       }
       __syncwarp();
       return true;
     };
-    const auto outputs = [&](uint32_t acc, uint32_t a, uint32_t tile_addr, bool add) {
-      const uint64_t b = operand(tile_addr, kAtom);
+    const auto outputs = [&](uint32_t acc, uint32_t a, uint64_t b, bool add) {
 #pragma unroll
       for (int k = 0; k < TILE / 16; ++k) mma_ts(acc, a + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, add || k > 0);
     };
     bool ok = bar_wait_warp(own, 0, &fault) && scores(0) && dprobs(0);
+#pragma unroll 1
     for (int i = 0; i < n && ok; ++i) {
       if (!(ok = bar_wait_warp(pfull, i & 1, &fault))) break;
       fence_after();
-      if (lane == 0) outputs(tdv, tmem, sg + (i & 1) * TB, i > 0);
+      if (one) outputs(tdv, tmem, gt0 + (uint64_t)((i & 1) * (TB >> 4)), i > 0);
       __syncwarp();
       if (i + 1 < n && !(ok = scores(i + 1))) break;
       if (!(ok = bar_wait_warp(dsfull, i & 1, &fault))) break;
       fence_after();
-      if (lane == 0) {
+      if (one) {
         commit(gempty + 8 * (i & 1));      // dO, lse and D of tile i are no longer read
-        outputs(tdk, tdp, sq + (i % 3) * TB, i > 0);
-        commit(i + 1 < n ? qempty + 8 * (i % 3) : done);
+        outputs(tdk, tdp, qt0 + (uint64_t)((i % 3) * (TB >> 4)), i > 0);
+        if (i + 1 == n) commit(done);
       }
       __syncwarp();
-      if (i + 1 < n) ok = dprobs(i + 1);
+      if (i + 1 < n) {
+        if (!(ok = dprobs(i + 1))) break;
+        if (one) commit(qempty + 8 * (i % 3));
+        __syncwarp();
+      }
     }
   } else {
     const int half = warp >> 2, r0 = (warp & 3) * 32 + lane, row = tile * TILE + r0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + half * 64 + lanes, tp = tdp + half * 64 + lanes;
-    const float sl = p.scale_log2;
+    const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
+    const int first = r0 - half * 64;      // on the diagonal: the first column (query) of this half that sees the row (key)
     bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const float2* rw = rows[i & 1] + half * 64;
+#pragma unroll 1
+    for (int i = 0, q = tile; i < n; ++i) {
+      const float4* l4 = reinterpret_cast<const float4*>(nlse[i & 1] + half * 64);
+      const float4* d4 = reinterpret_cast<const float4*>(ndelta[i & 1] + half * 64);
+      const bool diagonal = q == tile;
+      if (++q == nt) q = tile;
       if (!(ok = bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault) && bar_wait_warp(sfull, i & 1, &fault))) break;
       fence_after();
-      const bool diagonal = i % per_head == 0;
-      const int first = r0 - half * 64;      // first column (query) of this half that sees the row (key)
       uint32_t r[64];
       ld32(ts, r);
       ld32(ts + 32, r + 32);
-      wait_ld();
+      wait_ld(r);
 #pragma unroll
-      for (int c = 0; c < 64; ++c) r[c] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c]), sl, -rw[c].x)));
+      for (int c = 0; c < 16; ++c) {
+        const float4 l = l4[c];
+        const float2 a = unpair(fma2(pair(r[4 * c], r[4 * c + 1]), sl2, pair(l.x, l.y)));
+        const float2 b = unpair(fma2(pair(r[4 * c + 2], r[4 * c + 3]), sl2, pair(l.z, l.w)));
+        r[4 * c] = __float_as_uint(ex2(a.x));
+        r[4 * c + 1] = __float_as_uint(ex2(a.y));
+        r[4 * c + 2] = __float_as_uint(ex2(b.x));
+        r[4 * c + 3] = __float_as_uint(ex2(b.y));
+      }
       if (diagonal) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
           if (c < first) r[c] = 0u;
       }
+      uint32_t o[32];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t o[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(r[32 * q + 2 * c]), __uint_as_float(r[32 * q + 2 * c + 1]));
-        st16(ts + 16 * q, o);
-      }
+      for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      st32(ts, o);
       wait_st();
       fence_before();
       bar_arrive(pfull);
       if (!(ok = bar_wait_warp(dpfull, i & 1, &fault))) break;
       fence_after();
+      uint32_t g[64];
+      ld32(tp, g);
+      ld32(tp + 32, g + 32);
+      wait_ld(g);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint32_t g[32], o[16];
-        ld32(tp + 32 * q, g);
-        wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) g[c] = __float_as_uint(__uint_as_float(r[32 * q + c]) * (__uint_as_float(g[c]) - rw[32 * q + c].y));
-        if (diagonal) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (32 * q + c < first) g[c] = 0u;
-          if (tile == 0 && half == 0 && q == 0) g[0] = 0u;      // (the first query sees one key: its probability is 1)
-        }
-#pragma unroll
-        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
-        st16(tp + 16 * q, o);
+      for (int c = 0; c < 16; ++c) {
+        const float4 l = d4[c];
+        const float2 a = unpair(mul2(pair(r[4 * c], r[4 * c + 1]), add2(pair(g[4 * c], g[4 * c + 1]), pair(l.x, l.y))));
+        const float2 b = unpair(mul2(pair(r[4 * c + 2], r[4 * c + 3]), add2(pair(g[4 * c + 2], g[4 * c + 3]), pair(l.z, l.w))));
+        g[4 * c] = __float_as_uint(a.x);
+        g[4 * c + 1] = __float_as_uint(a.y);
+        g[4 * c + 2] = __float_as_uint(b.x);
+        g[4 * c + 3] = __float_as_uint(b.y);
       }
+      if (diagonal) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c < first) g[c] = 0u;
+        if (tile == 0 && half == 0) g[0] = 0u;      // (the first query sees one key: its probability is 1)
+      }
+#pragma unroll
+      for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
+      st32(tp, o);
       wait_st();
       fence_before();
       bar_arrive(dsfull);
@@ -734,11 +848,11 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         uint32_t r[32];
         __syncwarp();
         ld32(tdv + c + lanes, r);
-        wait_ld();
+        wait_ld(r);
         if (in) store_cols<T>(p.dv + at, c, p.D, r, 1.f);
         __syncwarp();
         ld32(tdk + c + lanes, r);
-        wait_ld();
+        wait_ld(r);
         if (in) store_cols<T>(p.dk + at, c, p.D, r, p.scale);
       }
     }

@@ -108,51 +108,60 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
   auto m_of = [&](int t) { return MODE == LSE || MODE == GRAD ? t % mt : t / nt; };
   auto n_of = [&](int t) { return MODE == LSE || MODE == GRAD ? t / mt : t % nt; };
 
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {
+    const bool one = elect();
     int s = 0;
     unsigned ph = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
       const int m0 = m_of(t) * BM, n0 = n_of(t) * BN;
       for (int k = 0; k < nk; ++k) {
-        if (!(ok = bar_wait(empty + 8 * s, ph ^ 1u, &fault))) break;
+        if (!(ok = bar_wait_warp(empty + 8 * s, ph ^ 1u, &fault))) break;
         const uint32_t bar = full + 8 * s, a = smem + s * kStageBytes, b = a + BM * BK * 2;
-        bar_expect(bar, kStageBytes);
+        if (one) {
+          bar_expect(bar, kStageBytes);
 #pragma unroll
-        for (int j = 0; j < BM / 64; ++j) {
-          if (a_mn) load2(a + j * kBox, &ma, m0 + 64 * j, k * BK, bar);
-          else load2(a + j * kBox, &ma, k * BK, m0 + 64 * j, bar);
-        }
+          for (int j = 0; j < BM / 64; ++j) {
+            if (a_mn) load2(a + j * kBox, &ma, m0 + 64 * j, k * BK, bar);
+            else load2(a + j * kBox, &ma, k * BK, m0 + 64 * j, bar);
+          }
 #pragma unroll
-        for (int j = 0; j < BN / 64; ++j) {
-          if (MODE == DX) load2(b + j * kBox, &mb, n0 + 64 * j, p.v0 + k * BK, bar);
-          else if (MODE == DW) load2(b + j * kBox, &mb, n0 + 64 * j, k * BK, bar);
-          else load2(b + j * kBox, &mb, k * BK, p.v0 + n0 + 64 * j, bar);
+          for (int j = 0; j < BN / 64; ++j) {
+            if (MODE == DX) load2(b + j * kBox, &mb, n0 + 64 * j, p.v0 + k * BK, bar);
+            else if (MODE == DW) load2(b + j * kBox, &mb, n0 + 64 * j, k * BK, bar);
+            else load2(b + j * kBox, &mb, k * BK, p.v0 + n0 + 64 * j, bar);
+          }
         }
+        __syncwarp();
         if (++s == kStages) { s = 0; ph ^= 1u; }
       }
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     constexpr uint32_t desc = product_desc<T>(BM, BN, a_mn, b_mn);
+    const bool one = elect();
     int s = 0, buf = 0;
     unsigned ph = 0, bph = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok && nk; t += gridDim.x) {
-      if (!(ok = bar_wait(free_b + 8 * buf, bph ^ 1u, &fault))) break;
+      if (!(ok = bar_wait_warp(free_b + 8 * buf, bph ^ 1u, &fault))) break;
       fence_after();
       for (int k = 0; k < nk; ++k) {
-        if (!(ok = bar_wait(full + 8 * s, ph, &fault))) break;
+        if (!(ok = bar_wait_warp(full + 8 * s, ph, &fault))) break;
         fence_after();
         const uint32_t a = smem + s * kStageBytes, b = a + BM * BK * 2;
         const uint64_t da = operand(a, a_mn ? kBox : 16), db = operand(b, b_mn ? kBox : 16);
+        if (one) {
 #pragma unroll
-        for (int i = 0; i < BK / 16; ++i)
-          mma_ss(tmem + buf * BN, da + i * (a_mn ? 128 : 2), db + i * (b_mn ? 128 : 2), desc, k > 0 || i > 0);
-        commit(empty + 8 * s);
+          for (int i = 0; i < BK / 16; ++i)
+            mma_ss(tmem + buf * BN, da + i * (a_mn ? 128 : 2), db + i * (b_mn ? 128 : 2), desc, k > 0 || i > 0);
+          commit(empty + 8 * s);
+        }
+        __syncwarp();
         if (++s == kStages) { s = 0; ph ^= 1u; }
       }
       if (!ok) break;
-      commit(done + 8 * buf);
+      if (one) commit(done + 8 * buf);
+      __syncwarp();
       if (++buf == 2) { buf = 0; bph ^= 1u; }
     }
   } else if (warp >= 4) {
@@ -177,7 +186,7 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
           uint32_t r[32];
           __syncwarp();
           ld32(src + c, r);
-          wait_ld();
+          wait_ld(r);
           if (MODE == LSE) {
             if (c + 32 > cols) {
 #pragma unroll
@@ -233,7 +242,7 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
           uint32_t r[32];
           __syncwarp();
           ld32(src + c, r);
-          wait_ld();
+          wait_ld(r);
           if (!nk) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0;

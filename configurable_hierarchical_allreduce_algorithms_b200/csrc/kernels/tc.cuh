@@ -66,13 +66,20 @@ static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, unsigned parity,
 // Waits for the phase of the given parity to complete; false: given up (the caller leaves its loops).
 __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, Fault* fault) {
 #pragma unroll 1
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 256; ++i)      // (the slow way begins by reading the global timer, which takes most of a microsecond)
     if (bar_try(bar, parity)) return true;
   return bar_wait_slow(bar, parity, fault);
 }
 // The same by a whole warp, with one answer for all its lanes (what follows is often a warp-wide instruction).
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, unsigned parity, Fault* fault) {
   return __all_sync(0xffffffffu, bar_wait(bar, parity, fault));
+}
+// True in one lane of a converged warp: the one that issues the warp's products.  The loops around them are left to the
+// whole warp, as their operands are kept in registers of the warp.
+__device__ __forceinline__ bool elect() {
+  unsigned one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
 }
 // End of a CTA whose waits ran out: copies and products already issued end within microseconds; nothing tells when, so
 // their shared and tensor memory is kept for a millisecond more.
@@ -106,7 +113,13 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, int cols) {           /
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Loads from tensor memory have arrived.  The registers pass through here, so that no use of them can be moved ahead.
+template <int N>
+__device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 columns of the warp's 32 lanes: thread l gets / gives lane l
@@ -173,6 +186,42 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two fp32 operations an instruction; the pairs are neighbouring registers
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);      // a in the low half
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
