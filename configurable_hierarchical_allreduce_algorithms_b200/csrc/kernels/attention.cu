@@ -123,26 +123,40 @@ __device__ __forceinline__ void zero_out(char* base, long long first, int rows, 
 }
 
 // ------------------------------------------------------------------ forward
-// Warps 0-3 and 4-7: rows of the two tiles; 8: loads; 9 and 10: products of the two tiles (one thread each); 11: zeros.
-// What bounds the kernel is the chain score -> softmax -> product of one tile, so nothing waits that need not: each tile has
-// a thread of its own for its products, P is handed over in halves, and the code of a turn is kept small (packed fp32
-// arithmetic, three-way maxima), as four warps' turns through a long one evict the other warps' instructions.
-constexpr int kFwdThreads = 384;
+// Warps 0-7 and 8-15: rows of the two tiles, each row twice, half of the 128 columns a thread; 16: loads; 17 and 18: products
+// of the two tiles; 19: zeros.
+// What bounds the kernel is the chain scores -> softmax -> product of one tile (per tile of 128 x 128: 1024 clocks of products
+// at D = 128, 1024 of the special function unit, and latencies between them), so each tile has a warp of its own for its
+// products, and four warps a scheduler hide the latencies in a softmax (16384 tokens, 16 / 4 heads of 128: 858 us; with two
+// warps a scheduler 1066 us, or 917 us with tile 1 held back by half a turn).
+constexpr int kFwdThreads = 640;
+
+// Whether any of a tile's 256 threads wants it; barrier 1 + tile
+__device__ __forceinline__ bool any_of_tile(int tile, bool want) {
+  unsigned r;
+  asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, 256, p;\n selp.u32 %0, 1, 0, q;\n}"
+               : "=r"(r) : "r"((unsigned)want), "r"(1 + tile) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void sync_tile(int tile) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(1 + tile) : "memory"); }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
              const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
+  // At DP = 64 tensor memory has room for P beside the scores, and the next scores are made as soon as these are read.
+  constexpr bool kApart = DP == 64;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[18];
+  __shared__ __align__(8) unsigned long long bars[20];
+  __shared__ float joint[2][2][TILE];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   __shared__ Work work;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t qfull = bar0, kfull = bar0 + 16, kempty = bar0 + 32, vfull = bar0 + 48, vempty = bar0 + 64, sfull = bar0 + 80,
-                 pfull = bar0 + 96, vready = bar0 + 128;      // (two of each, of P's halves four; the outputs are the scores' last phase)
+                 pfull = bar0 + 96, vready = bar0 + 112, sread = bar0 + 128, odone = bar0 + 144;      // (two of each)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, p.group, &work);
@@ -168,23 +182,29 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
   if (threadIdx.x == 0) {
     fault.raised = 0;
     fault.status = p.status;
-    for (int i = 0; i < 18; ++i) bar_init(bar0 + 8 * i, 1);
-    for (int i = 0; i < 4; ++i) bar_init(pfull + 8 * i, 128);
     const int tiles = n[1] ? 2 : 1;
     for (int i = 0; i < 2; ++i) {
+      bar_init(qfull + 8 * i, 1);
+      bar_init(kfull + 8 * i, 1);
       bar_init(kempty + 8 * i, tiles);
+      bar_init(vfull + 8 * i, 1);
       bar_init(vempty + 8 * i, tiles + ragged);
+      bar_init(sfull + 8 * i, 1);
+      bar_init(pfull + 8 * i, 256);
+      bar_init(vready + 8 * i, 1);
+      bar_init(sread + 8 * i, 256);
+      bar_init(odone + 8 * i, 1);
     }
     bar_init_done();
   }
-  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
+  if (warp == 17) tmem_alloc(smem_u32(&tmem_), 512);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tmem_;
   const uint32_t sq = smem, sk = smem + 2 * TB, sv = smem + 4 * TB;
 
-  if (warp == 8) {
+  if (warp == 16) {
     const bool one = elect();
     const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
       if (one) {
@@ -204,7 +224,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       if (!bar_wait_warp(vempty + 8 * s, ph, &fault)) break;
       load_tile(sv + s * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s);
     }
-  } else if (warp == 11) {
+  } else if (warp == 19) {
     // where the last tile is ragged every tile of values goes through this warp's hands (it keeps its place in the ring so)
     for (int i = 0; i < n[0] && ragged; ++i) {
       const int s = i & 1;
@@ -215,15 +235,16 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
         bar_arrive(vempty + 8 * s);
       }
     }
-  } else if (warp >= 9) {
-    const int u = warp - 9, nu = n[u];
+  } else if (warp >= 17) {
+    const int u = warp - 17, nu = n[u];
     if (nu) {
       const bool one = elect();
       const int ksteps = (p.D + 15) / 16;
       const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
       const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
-      const uint32_t ts = tmem + u * TILE, to = tmem + 2 * TILE + u * DP, ready = sfull + 8 * u, pf = pfull + 16 * u,
+      const uint32_t ts = tmem + u * TILE, to = tmem + 2 * TILE + u * DP, tp = kApart ? tmem + 3 * TILE + u * 64 : ts,
                      values = ragged ? vready : vfull;
+      constexpr int kHalf = kApart ? 32 : 64;      // columns from one half of P to the other
       const uint64_t a = operand(sq + u * TB), k0 = operand(sk), v0 = operand(sv, kAtom);
       const auto scores = [&](int s) {
         const uint64_t b = k0 + (uint64_t)(s * (TB >> 4));
@@ -231,7 +252,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)
             if (k < ksteps) mma_ss(ts, along(a, k), along(b, k), dscore, k > 0);
-          commit(ready);
+          commit(sfull + 8 * u);
           commit(kempty + 8 * s);
         }
         __syncwarp();
@@ -242,27 +263,23 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       for (int i = 0; i < nu && ok; ++i) {
         const int s = i & 1;
         const uint64_t b = v0 + (uint64_t)(s * (TB >> 4));
-        if (!(ok = bar_wait_warp(values + 8 * s, (i >> 1) & 1, &fault))) break;
-        if (!(ok = bar_wait_warp(pf, i & 1, &fault))) break;
-        fence_after();
-        if (one) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ts(to, ts + 8 * k, across(b, k), dout, i > 0 || k > 0);
-        }
-        __syncwarp();
-        // (the wait for the next keys comes before the one for the second half of P: it is over by then)
         if (i + 1 < nu && !(ok = bar_wait_warp(kfull + 8 * (s ^ 1), ((i + 1) >> 1) & 1, &fault))) break;
-        if (!(ok = bar_wait_warp(pf + 8, i & 1, &fault))) break;
+        if (kApart && i + 1 < nu) {
+          if (!(ok = bar_wait_warp(sread + 8 * u, i & 1, &fault))) break;
+          fence_after();
+          scores(s ^ 1);
+        }
+        if (!(ok = bar_wait_warp(values + 8 * s, (i >> 1) & 1, &fault))) break;
+        if (!(ok = bar_wait_warp(pfull + 8 * u, i & 1, &fault))) break;
         fence_after();
         if (one) {
 #pragma unroll
-          for (int k = 4; k < 8; ++k) mma_ts(to, ts + 8 * k, across(b, k), dout, true);
+          for (int k = 0; k < 8; ++k) mma_ts(to, tp + (k >> 2) * kHalf + (k & 3) * 8, across(b, k), dout, i > 0 || k > 0);
+          if (kApart || i + 1 == nu) commit(odone + 8 * u);
         }
         __syncwarp();
         // the next scores go over P, behind the products that read it
-        if (i + 1 < nu) scores(s ^ 1);
-        else if (one) commit(ready);      // (stands for the output)
-        __syncwarp();
+        if (!kApart && i + 1 < nu) scores(s ^ 1);
         if (one) commit(vempty + 8 * s);
         __syncwarp();
       }
@@ -273,85 +290,103 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       }
     }
   } else {
-    const int u = warp >> 2, nu = n[u];
+    const int u = warp >> 3, half = (warp >> 2) & 1, nu = n[u], r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + u * TILE + lanes, to = tmem + 2 * TILE + u * DP + lanes, ready = sfull + 8 * u, pf = pfull + 16 * u;
-    const int row = tile[u] * TILE + (warp & 3) * 32 + lane;
+    const uint32_t ts = tmem + u * TILE + half * 64 + lanes, tp = kApart ? tmem + 3 * TILE + u * 64 + half * 32 + lanes : ts,
+                   to = tmem + 2 * TILE + u * DP + half * (DP / 2) + lanes;
+    const int row = tile[u] * TILE + r0;
     const float sl = p.scale_log2;
     const uint64_t sl2 = pair(sl, sl);
     float ref = 0.f;                       // the maximum that the sums are relative to, times scale log2 e
     uint64_t sum2[2] = {0ull, 0ull};       // (two zeros each)
-    bool ok = nu > 0;
+    // The warps of a tile meet at barriers that cannot give up, so none of them leaves the loop: once a wait ran out all waits
+    // end at once, and the turns that are left go over whatever the scores hold.
 #pragma unroll 1
     for (int i = 0; i < nu; ++i) {
-      if (!(ok = bar_wait_warp(ready, i & 1, &fault))) break;
+      bar_wait_warp(sfull + 8 * u, i & 1, &fault);
       fence_after();
-      uint32_t r[TILE];
-#pragma unroll
-      for (int c = 0; c < TILE; c += 32) ld32(ts + c, r + c);
+      uint32_t r[64];
+      ld32(ts, r);
+      ld32(ts + 32, r + 32);
       wait_ld(r);
+      if (kApart) {
+        fence_before();
+        bar_arrive(sread + 8 * u);
+      }
       if (i == nu - 1) {
+        const int last = r0 - half * 64;
 #pragma unroll
-        for (int c = 0; c < TILE; ++c)
-          if (i * TILE + c > row) r[c] = __float_as_uint(-INFINITY);
+        for (int c = 0; c < 64; ++c)
+          if (c > last) r[c] = __float_as_uint(-INFINITY);
       }
       float m4[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
 #pragma unroll
-      for (int c = 4; c < TILE / 2; ++c) m4[c & 3] = max3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+      for (int c = 4; c < 32; ++c) m4[c & 3] = max3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
       const float top = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * sl;
-      if (i == 0) {
-        ref = top == -INFINITY ? 0.f : top;
-      } else if (__any_sync(0xffffffffu, top > ref + 8.f)) {
-        // (the commit that signalled these scores came behind the products of the tile before: the output rests)
-        const float next = fmaxf(ref, top), f = ex2(ref - next);
-        const uint64_t f2 = pair(f, f);
-        ref = next;
-        sum2[0] = mul2(sum2[0], f2);
-        sum2[1] = mul2(sum2[1], f2);
+      const bool grows = any_of_tile(u, i == 0 || top > ref + 8.f);
+      if (kApart && i > 0) bar_wait_warp(odone + 8 * u, (i - 1) & 1, &fault);
+      if (grows) {
+        joint[u][half][r0] = top;
+        sync_tile(u);
+        const float both = fmaxf(top, joint[u][half ^ 1][r0]);
+        sync_tile(u);
+        if (i == 0) {
+          ref = both == -INFINITY ? 0.f : both;
+        } else {
+          // (the output rests: the products of the tile before are done, as the scores' commit came behind them or odone says so)
+          fence_after();
+          const float next = fmaxf(ref, both), f = ex2(ref - next);
+          const uint64_t f2 = pair(f, f);
+          ref = next;
+          sum2[0] = mul2(sum2[0], f2);
+          sum2[1] = mul2(sum2[1], f2);
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
-          ld32(to + c, o);
-          wait_ld(o);
+          for (int c = 0; c < DP / 2; c += 16) {
+            uint32_t o[16];
+            ld16(to + c, o);
+            wait_ld(o);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-          st32(to + c, o);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            st16(to + c, o);
+          }
+          wait_st();
         }
-        wait_st();
       }
       const uint64_t nref2 = pair(-ref, -ref);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t pk[32];
+        uint32_t pk[16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float2 t = unpair(fma2(pair(r[64 * h + 2 * c], r[64 * h + 2 * c + 1]), sl2, nref2));
-          const float x = ex2(t.x), y = ex2(t.y);
-          sum2[c & 1] = add2(sum2[c & 1], pair(x, y));
-          pk[c] = pack2<T>(x, y);
+        for (int c = 0; c < 16; ++c) {
+          const float2 e = ex2_pair(fma2(pair(r[32 * h + 2 * c], r[32 * h + 2 * c + 1]), sl2, nref2));
+          sum2[c & 1] = add2(sum2[c & 1], pair(e.x, e.y));
+          pk[c] = pack2<T>(e.x, e.y);
         }
-        st32(ts + 32 * h, pk);
-        wait_st();
-        fence_before();
-        bar_arrive(pf + 8 * h);
+        st16(tp + 16 * h, pk);
       }
+      wait_st();
+      fence_before();
+      bar_arrive(pfull + 8 * u);
     }
-    if (ok && bar_wait_warp(ready, nu & 1, &fault)) {
+    if (nu) {
+      bar_wait_warp(odone + 8 * u, kApart ? (nu - 1) & 1 : 0, &fault);
       fence_after();
       const float2 a = unpair(add2(sum2[0], sum2[1]));
-      const float sum = a.x + a.y, f = 1.f / sum;
+      joint[u][half][r0] = a.x + a.y;
+      sync_tile(u);
+      const float sum = joint[u][0][r0] + joint[u][1][r0], f = 1.f / sum;
       const bool in = row < w.len;
-      if (in) p.lse[(long long)head[u] * p.T + w.start + row] = ref + log2f(sum);
+      if (in && half == 0) p.lse[(long long)head[u] * p.T + w.start + row] = ref + log2f(sum);
       char* out = p.o + ((long long)(w.start + row) * p.heads + head[u]) * p.D * 2;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = 0; c < DP / 2; c += 32) {
         uint32_t r[32];
         __syncwarp();
         ld32(to + c, r);
         wait_ld(r);
-        if (in) store_cols<T>(out, c, p.D, r, f);
+        if (in) store_cols<T>(out, half * (DP / 2) + c, p.D, r, f);
       }
     }
   }
@@ -359,7 +394,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
   __syncthreads();
   fence_after();
   if (fault.raised) drain_after_abort();
-  if (warp == 9) tmem_free(tmem, 512);
+  if (warp == 17) tmem_free(tmem, 512);
 }
 
 // The kernel below fills the shared memory of an SM to the last kilobyte: what aligning the tiles leaves is checked.
@@ -380,9 +415,9 @@ constexpr int kBwdThreads = 352;
 __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_t nlse2) {
 #pragma unroll
   for (int c = 0; c < 32; ++c) {
-    const float2 t = unpair(fma2(pair(r[2 * c], r[2 * c + 1]), sl2, nlse2));
-    r[2 * c] = __float_as_uint(ex2(t.x));
-    r[2 * c + 1] = __float_as_uint(ex2(t.y));
+    const float2 e = ex2_pair(fma2(pair(r[2 * c], r[2 * c + 1]), sl2, nlse2));
+    r[2 * c] = __float_as_uint(e.x);
+    r[2 * c + 1] = __float_as_uint(e.y);
   }
 }
 
@@ -791,12 +826,12 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
         const float4 l = l4[c];
-        const float2 a = unpair(fma2(pair(r[4 * c], r[4 * c + 1]), sl2, pair(l.x, l.y)));
-        const float2 b = unpair(fma2(pair(r[4 * c + 2], r[4 * c + 3]), sl2, pair(l.z, l.w)));
-        r[4 * c] = __float_as_uint(ex2(a.x));
-        r[4 * c + 1] = __float_as_uint(ex2(a.y));
-        r[4 * c + 2] = __float_as_uint(ex2(b.x));
-        r[4 * c + 3] = __float_as_uint(ex2(b.y));
+        const float2 a = ex2_pair(fma2(pair(r[4 * c], r[4 * c + 1]), sl2, pair(l.x, l.y)));
+        const float2 b = ex2_pair(fma2(pair(r[4 * c + 2], r[4 * c + 3]), sl2, pair(l.z, l.w)));
+        r[4 * c] = __float_as_uint(a.x);
+        r[4 * c + 1] = __float_as_uint(a.y);
+        r[4 * c + 2] = __float_as_uint(b.x);
+        r[4 * c + 3] = __float_as_uint(b.y);
       }
       if (diagonal) {
 #pragma unroll
