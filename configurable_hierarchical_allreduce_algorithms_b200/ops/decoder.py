@@ -26,7 +26,7 @@ N.optional("chb_linear_ce_bytes", i32, [i64, i32, i32, C.POINTER(i64), C.POINTER
 N.optional("chb_linear_ce_forward", i32, [i32, vp, i64, vp, vp, i64, i32, i32, i64, i32, vp, vp, vp, vp])
 N.optional("chb_linear_ce_backward", i32, [i32, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp])
 
-N.optional("chb_head_rope_ctas", i32, [C.POINTER(i32)])
+N.optional("chb_head_rope_rows", i32, [i32, i32, C.POINTER(i32)])
 N.optional("chb_head_rope", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, vp, i32, f32, C.c_double, i32, vp, vp, vp])
 N.optional("chb_attention_forward", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp])
 N.optional("chb_attention_backward", i32, [i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp, vp, vp])
@@ -144,7 +144,7 @@ class _HeadNormRope(torch.autograd.Function):
             x, w = (_heads(saved[0]), _heads(saved[1])), (_aligned(saved[2]), _aligned(saved[3]))
             if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
                 dw = torch.empty_like(w[0]), torch.empty_like(w[1])
-                part = torch.empty(_rope_ctas(gq.device) * 2 * gq.shape[2], dtype=torch.float32, device=gq.device)
+                part = torch.empty(_rope_rows(gq.device, *heads) * gq.shape[2], dtype=torch.float32, device=gq.device)
         if len(gq):
             _head_rope(x, dy, dx, heads, w, pos, eps, base, interleaved, part, dw)
         elif dw:
@@ -153,10 +153,10 @@ class _HeadNormRope(torch.autograd.Function):
 
 
 @lru_cache(maxsize=None)
-def _rope_ctas(device: torch.device) -> int:
+def _rope_rows(device: torch.device, heads_q: int, heads_k: int) -> int:
     n = i32(0)
     with _on(device):
-        _check(N.lib().chb_head_rope_ctas(C.byref(n)), "chb_head_rope_ctas")
+        _check(N.lib().chb_head_rope_rows(heads_q, heads_k, C.byref(n)), "chb_head_rope_rows")
     return n.value
 
 
