@@ -9,7 +9,6 @@ so they can be captured into CUDA graphs.  The reference stops at the collective
 models whose gradients this package's data-parallel paths move."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import struct
 from functools import lru_cache
@@ -32,6 +31,7 @@ N.optional("chb_attention_forward", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i3
 N.optional("chb_attention_backward", i32, [i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp, vp, vp])
 
 _HALF = (torch.bfloat16, torch.float16)
+_ROPE_TYPES = (*_HALF, torch.float32)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
@@ -39,18 +39,23 @@ class OperatorError(RuntimeError):
     pass
 
 
-def _check(rc: int, what: str):
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_functions: dict = {}
+
+
+def _call(name: str, device: torch.device, *args) -> None:
+    """One entry of the native library on the current stream of ``device``."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(N.lib(), name)
+    index = device.index
+    if index == _current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
-        raise OperatorError(f"{what} failed: {N.ERR_NAMES.get(rc, rc)}")
-
-
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch if it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+        raise OperatorError(f"{name} failed: {N.ERR_NAMES.get(rc, rc)}")
 
 
 def _need(ok: bool, message: str):
@@ -66,87 +71,94 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix whose rows are contiguous and start on 16-byte boundaries (copied if they do not)."""
-    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+    row, one = t.stride()
+    if one == 1 and row % 8 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
     return _aligned(t)
+
+
+def _first_order(backward):
+    """A backward pass that is not differentiable itself.  Gradients are asked for without a graph nearly always, and then
+    nothing of that has to be arranged."""
+    slow = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
 
 
 def check_operators(device=None):
     """Synchronise the current stream and raise :class:`OperatorError` if a bounded wait inside a matrix kernel of this
     module ran out since the last call (its outputs are not to be used then)."""
     device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
-    with _on(device):
-        word = C.c_uint(0)
-        _check(N.lib().chb_matrix_status(C.byref(word), _stream(device)), "chb_matrix_status")
+    word = C.c_uint(0)
+    _call("chb_matrix_status", device, C.byref(word))
     if word.value:
         raise OperatorError("a wait inside a matrix kernel ran out")
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """[T, H, D] whose heads are contiguous and start on 16-byte boundaries (copied if they do not)."""
-    size = t.element_size()
-    if t.stride(2) == 1 and all(t.stride(i) * size % 16 == 0 for i in (0, 1)) and t.data_ptr() % 16 == 0:
+    st, sh, one = t.stride()
+    if one == 1 and not ((st | sh) * t.element_size() | t.data_ptr()) & 15:
         return t
     return _aligned(t)
 
 
-def _table(*tensors) -> bytes:
-    """Device pointers as a C array (packed bytes: a tenth of the time of a ctypes array)."""
-    return _pack_table[len(tensors)](*[0 if t is None else t.data_ptr() for t in tensors])
-
-
-_pack_table = {k: struct.Struct(f"{k}Q").pack for k in (2,)}
-_pack_strides = struct.Struct("8q").pack
+_two = struct.Struct("2Q").pack        # (device pointers as a C array: packed bytes take a tenth of the time of a ctypes array)
+_eight = struct.Struct("8q").pack
 
 
 # ---------------------------------------------------------------------------------------- head norm and position rotation
 
 def _head_rope(x, dy, y, heads, w, pos, eps, base, interleaved, part=None, dw=None):
     q, k = y
-    sx, sd = (((t.stride(0), t.stride(1)) if t is not None else (0, 0) for t in ts) for ts in (x, dy or (None, None)))
-    (a, b), (c, d) = sx
-    (e, f), (g, h) = sd
-    dev = q.device
-    with _on(dev):
-        rc = N.lib().chb_head_rope(DTYPES[q.dtype], _table(*x), _table(*dy) if dy else None, _table(q, k), _pack_strides(a, b, c, d, e, f, g, h),
-                                   q.shape[0], heads[0], heads[1], q.shape[2], _table(*w) if w else None,
-                                   DTYPES[w[0].dtype] if w else 0, pos.data_ptr() if pos is not None else None,
-                                   int(pos is not None and pos.dtype == torch.int64), eps, base, interleaved,
-                                   part.data_ptr() if part is not None else None, _table(*dw) if dw else None, _stream(dev))
-    _check(rc, "head_norm_rope")
+    a = b = c = d = e = f = g = h = 0
+    if x is not None:
+        (a, b, _), (c, d, _) = x[0].stride(), x[1].stride()
+    if dy is not None:
+        (e, f, _), (g, h, _) = dy[0].stride(), dy[1].stride()
+    _call("chb_head_rope", q.device, DTYPES[q.dtype], _two(0, 0) if x is None else _two(x[0].data_ptr(), x[1].data_ptr()),
+          None if dy is None else _two(dy[0].data_ptr(), dy[1].data_ptr()), _two(q.data_ptr(), k.data_ptr()), _eight(a, b, c, d, e, f, g, h),
+          q.shape[0], heads[0], heads[1], q.shape[2], None if w is None else _two(w[0].data_ptr(), w[1].data_ptr()),
+          0 if w is None else DTYPES[w[0].dtype], None if pos is None else pos.data_ptr(), pos is not None and pos.dtype == torch.int64,
+          eps, base, interleaved, None if part is None else part.data_ptr(), None if dw is None else _two(dw[0].data_ptr(), dw[1].data_ptr()))
+
+
+def _rope_forward(q, k, wq, wk, pos, eps, base, interleaved):
+    # (not empty_like: the outputs are contiguous whatever q and k are)
+    y = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.shape[0]:
+        _head_rope((_heads(q), _heads(k)), None, y, (q.shape[1], k.shape[1]), None if wq is None else (_aligned(wq), _aligned(wk)), pos, eps,
+                   base, interleaved)
+    return y
 
 
 class _HeadNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, pos, eps, base, interleaved):
-        heads = q.shape[1], k.shape[1]
-        x = _heads(q), _heads(k)
-        y = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        w = None if wq is None else (_aligned(wq), _aligned(wk))
-        if len(q):
-            _head_rope(x, None, y, heads, w, pos, eps, base, interleaved)
-        ctx.normed = w is not None
-        ctx.save_for_backward(*((q, k, wq, wk) if w else ()), *((pos,) if pos is not None else ()))
-        ctx.args = eps, base, interleaved, pos is not None
-        return y
+        if wq is None:
+            ctx.save_for_backward(pos)
+        else:
+            ctx.save_for_backward(pos, q, k, wq, wk)
+        ctx.args = eps, base, interleaved
+        return _rope_forward(q, k, wq, wk, pos, eps, base, interleaved)
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gq, gk):
-        eps, base, interleaved, has_pos = ctx.args
         saved = ctx.saved_tensors
-        pos = saved[-1] if has_pos else None
-        dy = _heads(gq), _heads(gk)
-        heads = gq.shape[1], gk.shape[1]
+        pos = saved[0]
         dx = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device), torch.empty(gk.shape, dtype=gk.dtype, device=gk.device)
-        x, w, part, dw = (None, None), None, None, None
-        if ctx.normed:
-            x, w = (_heads(saved[0]), _heads(saved[1])), (_aligned(saved[2]), _aligned(saved[3]))
+        heads = gq.shape[1], gk.shape[1]
+        x = w = part = dw = None
+        if len(saved) > 1:
+            x, w = (_heads(saved[1]), _heads(saved[2])), (_aligned(saved[3]), _aligned(saved[4]))
             if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
                 dw = torch.empty_like(w[0]), torch.empty_like(w[1])
                 part = torch.empty(_rope_rows(gq.device, *heads) * gq.shape[2], dtype=torch.float32, device=gq.device)
-        if len(gq):
-            _head_rope(x, dy, dx, heads, w, pos, eps, base, interleaved, part, dw)
+        if gq.shape[0]:
+            _head_rope(x, (_heads(gq), _heads(gk)), dx, heads, w, pos, *ctx.args, part, dw)
         elif dw:
             dw = torch.zeros_like(w[0]), torch.zeros_like(w[1])
         return (*dx, *(dw or (None, None)), None, None, None, None)
@@ -155,9 +167,19 @@ class _HeadNormRope(torch.autograd.Function):
 @lru_cache(maxsize=None)
 def _rope_rows(device: torch.device, heads_q: int, heads_k: int) -> int:
     n = i32(0)
-    with _on(device):
-        _check(N.lib().chb_head_rope_rows(heads_q, heads_k, C.byref(n)), "chb_head_rope_rows")
+    with torch.cuda.device(device):
+        rc = N.lib().chb_head_rope_rows(heads_q, heads_k, C.byref(n))
+    if rc:
+        raise OperatorError(f"chb_head_rope_rows failed: {N.ERR_NAMES.get(rc, rc)}")
     return n.value
+
+
+def _wants_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
@@ -170,69 +192,73 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
     where their heads start on 16-byte boundaries).  ``q_weight``, ``k_weight`` [D]: fp32 or the type of ``q``, both or
     neither (no norm then).  ``positions``: int32 or int64, any value; None: 0, 1, 2, ...  ``interleaved``: pair i is
     elements 2i and 2i + 1, else i and i + D / 2.  Returns contiguous tensors of the types of ``q`` and ``k``."""
-    _need(q.dim() == 3 and k.dim() == 3 and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2] and q.shape[1] > 0 and k.shape[1] > 0,
-          "head_norm_rope: q [T, H, D] and k [T, Hk, D] expected")
-    _need(q.dtype in (*_HALF, torch.float32) and k.dtype == q.dtype, "head_norm_rope: q and k have to be bf16, fp16 or fp32, and alike")
-    d = q.shape[2]
-    _need(d % 8 == 0 and 0 < d <= 256 and q.shape[0] < 1 << 31, "head_norm_rope: D has to be a multiple of 8, at most 256")
-    _need((q_weight is None) == (k_weight is None), "head_norm_rope: weights for both or for neither")
-    tensors = [q, k]
+    qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
+    if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or qs[1] == 0 or ks[1] == 0:
+        raise ValueError("head_norm_rope: q [T, H, D] and k [T, Hk, D] expected")
+    if dtype not in _ROPE_TYPES or k.dtype != dtype:
+        raise ValueError("head_norm_rope: q and k have to be bf16, fp16 or fp32, and alike")
+    d = qs[2]
+    if d % 8 or not 0 < d <= 256 or qs[0] >= 1 << 31:
+        raise ValueError("head_norm_rope: D has to be a multiple of 8, at most 256")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("head_norm_rope: weights for both or for neither")
+    devices = k.device == dev
     if q_weight is not None:
-        tensors += [q_weight, k_weight]
-        _need(all(w.shape == (d,) and w.dtype in (q.dtype, torch.float32) for w in tensors[2:]) and q_weight.dtype == k_weight.dtype,
-              "head_norm_rope: weights [D] of fp32 or the type of q expected")
+        if q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype not in (dtype, torch.float32) or k_weight.dtype != q_weight.dtype:
+            raise ValueError("head_norm_rope: weights [D] of fp32 or the type of q expected")
+        devices = devices and q_weight.device == dev and k_weight.device == dev
     if positions is not None:
-        tensors.append(positions)
-        _need(positions.shape == (q.shape[0],) and positions.dtype in (torch.int32, torch.int64),
-              "head_norm_rope: int32 or int64 positions [T] expected")
-    _need(base > 0 and eps >= 0, "head_norm_rope: base has to be positive, eps not negative")
-    _need(q.is_cuda and all(t.device == q.device for t in tensors), "head_norm_rope: tensors of one CUDA device expected")
-    return _HeadNormRope.apply(q, k, q_weight, k_weight, None if positions is None else positions.contiguous(), float(eps),
-                               float(base), bool(interleaved))
+        if positions.shape != (qs[0],) or positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("head_norm_rope: int32 or int64 positions [T] expected")
+        devices = devices and positions.device == dev
+        positions = positions.contiguous()
+    if not (base > 0 and eps >= 0):
+        raise ValueError("head_norm_rope: base has to be positive, eps not negative")
+    if dev.type != "cuda" or not devices:
+        raise ValueError("head_norm_rope: tensors of one CUDA device expected")
+    args = q, k, q_weight, k_weight, positions, float(eps), float(base), bool(interleaved)
+    return _HeadNormRope.apply(*args) if _wants_grad(q, k, q_weight, k_weight) else _rope_forward(*args)
 
 
 # ------------------------------------------------------------------------------------------------------ causal attention
 
-def _strides(*tensors) -> bytes:
-    s = [x for t in tensors for x in (t.stride(0), t.stride(1))]
-    return _pack_strides(*s, *(0,) * (8 - len(s)))
+def _attention_forward(q, k, v, cu, scale):
+    shape, dev = q.shape, q.device
+    T, h, d = shape
+    o = torch.empty(shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((h, T), dtype=torch.float32, device=dev)
+    if T:
+        q, k, v = _heads(q), _heads(k), _heads(v)
+        (a, b, _), (c, e, _), (f, g, _) = q.stride(), k.stride(), v.stride()
+        _call("chb_attention_forward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), _eight(a, b, c, e, f, g, 0, 0), T, h,
+              k.shape[1], d, None if cu is None else cu.data_ptr(), 0 if cu is None else cu.shape[0] - 1, scale, o.data_ptr(), lse.data_ptr())
+    return o, lse
 
 
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, scale):
-        T, h, d = q.shape
-        o = torch.empty(T, h, d, dtype=q.dtype, device=q.device)
-        lse = torch.empty(h, T, dtype=torch.float32, device=q.device)
-        if T:
-            qs, ks, vs = _heads(q), _heads(k), _heads(v)
-            with _on(q.device):
-                rc = N.lib().chb_attention_forward(DTYPES[q.dtype], qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), _strides(qs, ks, vs), T, h,
-                                                   k.shape[1], d, cu.data_ptr() if cu is not None else None,
-                                                   cu.numel() - 1 if cu is not None else 0, scale, o.data_ptr(), lse.data_ptr(),
-                                                   _stream(q.device))
-            _check(rc, "causal_attention")
-        ctx.save_for_backward(q, k, v, o, lse, *(() if cu is None else (cu,)))
+        o, lse = _attention_forward(q, k, v, cu, scale)
+        ctx.save_for_backward(q, k, v, o, lse, cu)
         ctx.scale = scale
         return o
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
-        q, k, v, o, lse, *rest = ctx.saved_tensors
-        cu = rest[0] if rest else None
+        q, k, v, o, lse, cu = ctx.saved_tensors
+        dev = q.device
         T, h, d = q.shape
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        kv = k.shape
+        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        dk = torch.empty(kv, dtype=q.dtype, device=dev)
+        dv = torch.empty(kv, dtype=q.dtype, device=dev)
         if T:
-            qs, ks, vs, g = _heads(q), _heads(k), _heads(v), _heads(grad)
-            delta = torch.empty(h, T, dtype=torch.float32, device=q.device)
-            with _on(q.device):
-                rc = N.lib().chb_attention_backward(DTYPES[q.dtype], qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), o.data_ptr(), g.data_ptr(),
-                                                    _strides(qs, ks, vs, g), lse.data_ptr(), T, h, k.shape[1], d,
-                                                    cu.data_ptr() if cu is not None else None, cu.numel() - 1 if cu is not None else 0,
-                                                    ctx.scale, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                                    _stream(q.device))
-            _check(rc, "causal_attention backward")
+            q, k, v, grad = _heads(q), _heads(k), _heads(v), _heads(grad)
+            (a, b, _), (c, e, _), (f, g, _), (m, n, _) = q.stride(), k.stride(), v.stride(), grad.stride()
+            delta = torch.empty((h, T), dtype=torch.float32, device=dev)
+            _call("chb_attention_backward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), grad.data_ptr(),
+                  _eight(a, b, c, e, f, g, m, n), lse.data_ptr(), T, h, kv[1], d, None if cu is None else cu.data_ptr(),
+                  0 if cu is None else cu.shape[0] - 1, ctx.scale, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         return dq, dk, dv, None, None
 
 
@@ -246,59 +272,74 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     most (not checked; bounds are clamped to 0 and T); lengths of zero are fine, rows outside all sequences get zeros and no
     gradient, and no sequence is reached by what another holds, infinities and NaN included.  None: one sequence.
     ``scale`` (default D ** -0.5) has to be positive.  Returns [T, H, D], contiguous."""
-    _need(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and q.shape[0] == k.shape[0] and q.shape[2] == k.shape[2],
-          "causal_attention: q [T, H, D], k and v [T, Hk, D] expected")
-    _need(q.dtype in _HALF and k.dtype == q.dtype and v.dtype == q.dtype, "causal_attention: q, k and v have to be bf16 or fp16, and alike")
-    h, hk, d = q.shape[1], k.shape[1], q.shape[2]
-    _need(hk > 0 and h > 0 and h % hk == 0, "causal_attention: the number of heads has to be a multiple of the key heads'")
-    _need(d % 8 == 0 and 0 < d <= 128, "causal_attention: D has to be a multiple of 8, at most 128")
+    qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or qs[0] != ks[0] or qs[2] != ks[2]:
+        raise ValueError("causal_attention: q [T, H, D], k and v [T, Hk, D] expected")
+    if dtype not in _HALF or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError("causal_attention: q, k and v have to be bf16 or fp16, and alike")
+    h, hk, d = qs[1], ks[1], qs[2]
+    if hk == 0 or h == 0 or h % hk:
+        raise ValueError("causal_attention: the number of heads has to be a multiple of the key heads'")
+    if d % 8 or not 0 < d <= 128:
+        raise ValueError("causal_attention: D has to be a multiple of 8, at most 128")
+    devices = k.device == dev and v.device == dev
     if cu_seqlens is not None:
-        _need(cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1 and cu_seqlens.dtype == torch.int32, "causal_attention: int32 cu_seqlens [B + 1] expected")
+        if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.dtype != torch.int32:
+            raise ValueError("causal_attention: int32 cu_seqlens [B + 1] expected")
+        devices = devices and cu_seqlens.device == dev
+        cu_seqlens = cu_seqlens.contiguous()
     scale = d ** -0.5 if scale is None else float(scale)
-    _need(0.0 < scale < float("inf"), "causal_attention: scale has to be positive")
-    _need(q.is_cuda and all(t.device == q.device for t in (k, v, cu_seqlens) if t is not None), "causal_attention: tensors of one CUDA device expected")
-    return _CausalAttention.apply(q, k, v, None if cu_seqlens is None else cu_seqlens.contiguous(), scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("causal_attention: scale has to be positive")
+    if dev.type != "cuda" or not devices:
+        raise ValueError("causal_attention: tensors of one CUDA device expected")
+    if _wants_grad(q, k, v):
+        return _CausalAttention.apply(q, k, v, cu_seqlens, scale)
+    return _attention_forward(q, k, v, cu_seqlens, scale)[0]
 
 
 # ---------------------------------------------------------------------------------------------- output layer and loss
 
+@lru_cache(maxsize=256)
+def _loss_bytes(n: int, d: int, v: int):
+    sizes = i64(0), i64(0), i64(0)
+    rc = N.lib().chb_linear_ce_bytes(n, d, v, *(C.byref(x) for x in sizes))
+    if rc:
+        raise OperatorError(f"chb_linear_ce_bytes failed: {N.ERR_NAMES.get(rc, rc)}")
+    return tuple(x.value for x in sizes)
+
+
+def _loss_forward(x, weight, targets, ignore_index, reduction):
+    (n, d), v, dev = x.shape, weight.shape[0], x.device
+    kept, temporary, _ = _loss_bytes(n, d, v)
+    saved = torch.empty(kept, dtype=torch.uint8, device=dev)
+    work = torch.empty(temporary, dtype=torch.uint8, device=dev)
+    loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+    x, w, t = _rows(x), _aligned(weight), targets.contiguous()
+    _call("chb_linear_ce_forward", dev, DTYPES[x.dtype], x.data_ptr(), x.stride(0), w.data_ptr(), t.data_ptr(), n, d, v, ignore_index, reduction,
+          loss.data_ptr(), saved.data_ptr(), work.data_ptr())
+    return loss, saved
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, ignore_index, reduction):
-        n, d = x.shape
-        v = weight.shape[0]
-        sizes = (i64 * 3)()
-        at = C.addressof(sizes)
-        ptr = lambda i: C.cast(at + 8 * i, C.POINTER(i64))      # noqa: E731
-        lib, code = N.lib(), DTYPES[x.dtype]
-        _check(lib.chb_linear_ce_bytes(n, d, v, ptr(0), ptr(1), ptr(2)), "chb_linear_ce_bytes")
-        byte = lambda k: torch.empty(k, dtype=torch.uint8, device=x.device)     # noqa: E731
-        saved, work = byte(sizes[0]), byte(sizes[1])
-        loss = torch.empty(n if reduction == 0 else (), dtype=torch.float32, device=x.device)
-        xr, w, t = _rows(x), _aligned(weight), targets.contiguous()
-        with _on(x.device):
-            rc = lib.chb_linear_ce_forward(code, xr.data_ptr(), xr.stride(0), w.data_ptr(), t.data_ptr(), n, d, v, ignore_index,
-                                           reduction, loss.data_ptr(), saved.data_ptr(), work.data_ptr(), _stream(x.device))
-        _check(rc, "linear_cross_entropy")
+        loss, saved = _loss_forward(x, weight, targets, ignore_index, reduction)
         ctx.save_for_backward(weight, saved)
-        ctx.sizes = n, d, v, sizes[2], reduction, code
+        ctx.args = x.shape[0], reduction
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         weight, saved = ctx.saved_tensors
-        n, d, v, nbytes, reduction, code = ctx.sizes
-        dev = weight.device
-        dx = torch.empty(n, d, dtype=weight.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(v, d, dtype=weight.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        n, reduction = ctx.args
+        (v, d), dev, dtype = weight.shape, weight.device, weight.dtype
+        dx = torch.empty((n, d), dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((v, d), dtype=dtype, device=dev) if ctx.needs_input_grad[1] else None
+        work = torch.empty(_loss_bytes(n, d, v)[2], dtype=torch.uint8, device=dev)
         w, g = _aligned(weight), grad.to(torch.float32).contiguous()
-        with _on(dev):
-            rc = N.lib().chb_linear_ce_backward(code, w.data_ptr(), g.data_ptr(), n, d, v, reduction, saved.data_ptr(),
-                                                work.data_ptr(), dx.data_ptr() if dx is not None else None,
-                                                dw.data_ptr() if dw is not None else None, _stream(dev))
-        _check(rc, "linear_cross_entropy backward")
+        _call("chb_linear_ce_backward", dev, DTYPES[dtype], w.data_ptr(), g.data_ptr(), n, d, v, reduction, saved.data_ptr(), work.data_ptr(),
+              None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())
         return dx, dw, None, None, None
 
 
@@ -322,5 +363,6 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     if targets.numel() == 0:
         zero = x.float().sum() + 0.0 * weight[:1].float().sum()
         return x.float().sum(-1) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
-    loss = _LinearCrossEntropy.apply(x.reshape(-1, d), weight, targets.reshape(-1), int(ignore_index), _REDUCTIONS[reduction])
+    args = x.reshape(-1, d), weight, targets.reshape(-1), int(ignore_index), _REDUCTIONS[reduction]
+    loss = _LinearCrossEntropy.apply(*args) if _wants_grad(x, weight) else _loss_forward(*args)[0]
     return loss.view(targets.shape) if reduction == "none" else loss
