@@ -7,7 +7,7 @@
 // Forward: rows with a label are gathered (a row without one costs nothing, and whatever its x holds, infinities
 // included, reaches neither the loss nor dW); one product whose epilogue keeps maximum and sum of exponentials of 256
 // columns; a small kernel joins them.  Backward, for each piece of the vocabulary: the product again with an epilogue
-// that writes G, then dW (complete for the piece) and dx (summed over the pieces in fp32) from G.
+// that writes G, then one launch for dW (complete for the piece) and dx (summed over the pieces in fp32) from G.
 //
 // Sums are fp32.  G is rounded to the operands' type, as the tensor cores need it; an fp16 G is kept 2^14 times larger
 // and relative to the largest |g_r|, or softmax tails would fall below fp16's range.
@@ -20,13 +20,15 @@ namespace {
 
 using namespace tc;
 
-constexpr int BM = 128, BN = 256, BK = 64, kStages = 4;
+constexpr int BM = 128, BK = 64;
 constexpr int kBox = 64 * 128;                               // bytes of one load: 64 rows of 64 elements
-constexpr int kStageBytes = (BM + BN) * BK * 2;
-constexpr int kGemmSmem = kStages * kStageBytes + 1024;      // (1024: the swizzle's alignment)
+// 192 KB of operands in flight; tiles of 256 columns run at the tensor cores' rate, tiles of 128 leave fewer SMs idle
+template <int BN> constexpr int kStages = BN == 256 ? 4 : 6;
+template <int BN> constexpr int kStageBytes = (BM + BN) * BK * 2;
+template <int BN> constexpr int kGemmSmem = kStages<BN> * kStageBytes<BN> + 1024;      // (1024: the swizzle's alignment)
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum Mode { LSE, GRAD, DX, DW };
+enum Mode { LSE, GRAD, BOTH };      // BOTH: dW and dx of a piece in one launch
 
 // Kept from forward to backward.
 struct Saved {
@@ -42,7 +44,6 @@ struct GemmArgs {
   const int* count;
   int N, V, v0, vn;          // rows of x at most; vocabulary, first column and width of the piece
   int D;
-  int K;                     // extent of the summed axis (0: the rows)
   // LSE
   float2* part;
   float* tlogit;
@@ -53,12 +54,14 @@ struct GemmArgs {
   const float* gs;
   char* g;
   long long ldg;
-  // DX / DW
-  float* acc;
+  // BOTH
+  int split_w, split_x;      // shares of the summed axis; more than one: fp32 sums in slabs, joined by ce_finish
+  float* slab_w;             // [split_w][vn][D]
+  float* slab_x;             // [split_x][rows_pad][D], summed over the pieces
   int first, last;
   const float* coef;
   const int* idx;
-  char* out;
+  char *dx, *dw;             // null: not wanted
   unsigned* status;
 };
 
@@ -70,14 +73,49 @@ __device__ __forceinline__ void st256(void* p, const uint32_t* v) {
 template <typename T> struct GScale { static constexpr float up = 1.f, down = 1.f; };
 template <> struct GScale<__half> { static constexpr float up = 16384.f, down = 1.f / 16384.f; };
 
+// 32 columns of a finished fp32 row, to the 16-bit row `out` or, added to what is there if `add`, to the fp32 row `sum`
+template <typename T>
+__device__ __forceinline__ void finish_cols(const uint32_t* r, int col, int D, float* sum, bool add, char* out, float coef) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int c = col + 8 * q;
+    if (c >= D) break;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * q + j]);
+    if (add) {
+      const float4 x = reinterpret_cast<const float4*>(sum + c)[0], y = reinterpret_cast<const float4*>(sum + c)[1];
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    if (out) {
+      uint4 o;
+      o.x = pack2<T>(v[0] * coef, v[1] * coef);
+      o.y = pack2<T>(v[2] * coef, v[3] * coef);
+      o.z = pack2<T>(v[4] * coef, v[5] * coef);
+      o.w = pack2<T>(v[6] * coef, v[7] * coef);
+      *reinterpret_cast<uint4*>(out + c * 2) = o;
+    } else {
+      reinterpret_cast<float4*>(sum + c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(sum + c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+}
+
+// One tile of a launch: its rows, columns and summed range (in steps of BK)
+struct TilePlace {
+  bool w;                    // BOTH: a tile of dW (else of dx)
+  int m0, n0, k0, k1, split;
+};
+
 // One persistent CTA per SM; warp 0 loads, warp 1 issues the products, warps 4 to 7 finish a tile (thread = row) while the
-// next one is summed in the other half of tensor memory.
-template <typename T, int MODE>
+// next one is summed in the other half of tensor memory.  Maps: LSE and GRAD gathered rows and W; BOTH also G.
+template <typename T, int MODE, int BN>
 __global__ void __launch_bounds__(256, 1)
-ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const GemmArgs p) {
-  constexpr bool a_mn = MODE == DW, b_mn = MODE == DX || MODE == DW;
+ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mg, const GemmArgs p) {
+  constexpr int STAGES = kStages<BN>, STAGE = kStageBytes<BN>;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long full_[kStages], empty_[kStages], done_[2], free_[2];
+  __shared__ __align__(8) unsigned long long full_[STAGES], empty_[STAGES], done_[2], free_[2];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -86,27 +124,45 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
   if (threadIdx.x == 0) {
     fault.raised = 0;
     fault.status = p.status;
-    for (int i = 0; i < kStages; ++i) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
+    for (int i = 0; i < STAGES; ++i) { bar_init(full + 8 * i, 1); bar_init(empty + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) { bar_init(done + 8 * i, 1); bar_init(free_b + 8 * i, 128); }
     bar_init_done();
-    prefetch_map(&ma);
-    prefetch_map(&mb);
+    prefetch_map(&mx);
+    prefetch_map(&mw);
+    if (MODE == BOTH) prefetch_map(&mg);
   }
-  if (warp == 1) tmem_alloc(smem_u32(&tmem_), 512);
+  if (warp == 1) tmem_alloc(smem_u32(&tmem_), 2 * BN);
   fence_before();
   __syncthreads();
   fence_after();
   dependent_launch();
   const uint32_t tmem = tmem_;
   const int count = *(volatile const int*)p.count;
-  const int mt = MODE == DW ? (p.vn + BM - 1) / BM : (count + BM - 1) / BM;
-  const int ncols = MODE == LSE || MODE == GRAD ? p.vn : p.D;
-  const int nt = (ncols + BN - 1) / BN;
-  const int nk = ((MODE == DW ? count : p.K) + BK - 1) / BK;
-  const int tiles = mt * nt;
-  // neighbouring CTAs share the operand that is read from HBM: the rows of W (LSE, GRAD) or of G (DX, DW)
-  auto m_of = [&](int t) { return MODE == LSE || MODE == GRAD ? t % mt : t / nt; };
-  auto n_of = [&](int t) { return MODE == LSE || MODE == GRAD ? t / mt : t % nt; };
+  const int rows_t = (count + BM - 1) / BM, nt = ((MODE == BOTH ? p.D : p.vn) + BN - 1) / BN;
+  const int voc_t = (p.vn + BM - 1) / BM;
+  const int kd = (p.D + BK - 1) / BK, kw = (count + BK - 1) / BK, kx = (p.vn + BK - 1) / BK;
+  const int tiles_w = MODE == BOTH && p.dw ? voc_t * nt * p.split_w : 0;
+  const int tiles = MODE == BOTH ? tiles_w + (p.dx ? rows_t * nt * p.split_x : 0) : rows_t * nt;
+  // neighbouring CTAs share the operand that is read from HBM: the rows of W (LSE, GRAD) or of G (BOTH, the longer sums first)
+  const auto place = [&](int t) {
+    TilePlace q{};
+    if (MODE != BOTH) {
+      q.m0 = t % rows_t * BM;
+      q.n0 = t / rows_t * BN;
+      q.k1 = kd;
+      return q;
+    }
+    q.w = t < tiles_w;
+    if (!q.w) t -= tiles_w;
+    const int per = (q.w ? voc_t : rows_t) * nt, k = q.w ? kw : kx, splits = q.w ? p.split_w : p.split_x;
+    q.split = t / per;
+    t -= q.split * per;
+    q.m0 = t / nt * BM;
+    q.n0 = t % nt * BN;
+    q.k0 = (int)((long long)k * q.split / splits);
+    q.k1 = (int)((long long)k * (q.split + 1) / splits);
+    return q;
+  };
 
   if (warp == 0) {
     const bool one = elect();
@@ -114,50 +170,59 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
     unsigned ph = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      const int m0 = m_of(t) * BM, n0 = n_of(t) * BN;
-      for (int k = 0; k < nk; ++k) {
+      const TilePlace q = place(t);
+      for (int k = q.k0; k < q.k1; ++k) {
         if (!(ok = bar_wait_warp(empty + 8 * s, ph ^ 1u, &fault))) break;
-        const uint32_t bar = full + 8 * s, a = smem + s * kStageBytes, b = a + BM * BK * 2;
+        const uint32_t bar = full + 8 * s, a = smem + s * STAGE, b = a + BM * BK * 2;
         if (one) {
-          bar_expect(bar, kStageBytes);
+          bar_expect(bar, STAGE);
+          if (MODE != BOTH) {
 #pragma unroll
-          for (int j = 0; j < BM / 64; ++j) {
-            if (a_mn) load2(a + j * kBox, &ma, m0 + 64 * j, k * BK, bar);
-            else load2(a + j * kBox, &ma, k * BK, m0 + 64 * j, bar);
-          }
+            for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mx, k * BK, q.m0 + 64 * j, bar);
 #pragma unroll
-          for (int j = 0; j < BN / 64; ++j) {
-            if (MODE == DX) load2(b + j * kBox, &mb, n0 + 64 * j, p.v0 + k * BK, bar);
-            else if (MODE == DW) load2(b + j * kBox, &mb, n0 + 64 * j, k * BK, bar);
-            else load2(b + j * kBox, &mb, k * BK, p.v0 + n0 + 64 * j, bar);
+            for (int j = 0; j < BN / 64; ++j) load2(b + j * kBox, &mw, k * BK, p.v0 + q.n0 + 64 * j, bar);
+          } else if (q.w) {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mg, q.m0 + 64 * j, k * BK, bar);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) load2(b + j * kBox, &mx, q.n0 + 64 * j, k * BK, bar);
+          } else {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mg, k * BK, q.m0 + 64 * j, bar);
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) load2(b + j * kBox, &mw, q.n0 + 64 * j, p.v0 + k * BK, bar);
           }
         }
         __syncwarp();
-        if (++s == kStages) { s = 0; ph ^= 1u; }
+        if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
     }
   } else if (warp == 1) {
-    constexpr uint32_t desc = product_desc<T>(BM, BN, a_mn, b_mn);
     const bool one = elect();
     int s = 0, buf = 0;
     unsigned ph = 0, bph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok && nk; t += gridDim.x) {
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const TilePlace q = place(t);
+      if (q.k0 == q.k1) continue;
+      const bool a_mn = MODE == BOTH && q.w;
+      constexpr bool b_mn = MODE == BOTH;
+      const uint32_t desc = a_mn ? product_desc<T>(BM, BN, true, b_mn) : product_desc<T>(BM, BN, false, b_mn);
+      const uint32_t a_step = a_mn ? 128 : 2;
       if (!(ok = bar_wait_warp(free_b + 8 * buf, bph ^ 1u, &fault))) break;
       fence_after();
-      for (int k = 0; k < nk; ++k) {
+      for (int k = q.k0; k < q.k1; ++k) {
         if (!(ok = bar_wait_warp(full + 8 * s, ph, &fault))) break;
         fence_after();
-        const uint32_t a = smem + s * kStageBytes, b = a + BM * BK * 2;
+        const uint32_t a = smem + s * STAGE, b = a + BM * BK * 2;
         const uint64_t da = operand(a, a_mn ? kBox : 16), db = operand(b, b_mn ? kBox : 16);
         if (one) {
 #pragma unroll
-          for (int i = 0; i < BK / 16; ++i)
-            mma_ss(tmem + buf * BN, da + i * (a_mn ? 128 : 2), db + i * (b_mn ? 128 : 2), desc, k > 0 || i > 0);
+          for (int i = 0; i < BK / 16; ++i) mma_ss(tmem + buf * BN, da + i * a_step, db + i * (b_mn ? 128 : 2), desc, k > q.k0 || i > 0);
           commit(empty + 8 * s);
         }
         __syncwarp();
-        if (++s == kStages) { s = 0; ph ^= 1u; }
+        if (++s == STAGES) { s = 0; ph ^= 1u; }
       }
       if (!ok) break;
       if (one) commit(done + 8 * buf);
@@ -169,12 +234,13 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
     unsigned bph = 0;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const int m0 = m_of(t) * BM, n0 = n_of(t) * BN;
-      const int row = m0 + (warp & 3) * 32 + lane;
-      if (nk && !bar_wait_warp(done + 8 * buf, bph, &fault)) break;
+      const TilePlace q = place(t);
+      const bool nothing = q.k0 == q.k1;      // (no row has a label: zeros)
+      const int row = q.m0 + (warp & 3) * 32 + lane, n0 = q.n0;
+      if (!nothing && !bar_wait_warp(done + 8 * buf, bph, &fault)) break;
       fence_after();
       const uint32_t src = tmem + buf * BN + lanes;
-      if (MODE == LSE || MODE == GRAD) {
+      if (MODE != BOTH) {
         const bool in = row < count;
         const int tg = in ? p.tgt[row] - p.v0 - n0 : -1;
         const int cols = min(BN, p.V - p.v0 - n0);
@@ -225,65 +291,81 @@ ce_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensor
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-            char* d = p.g + ((long long)row * p.ldg + n0 + c) * 2;
-            st256(d, o);
-            st256(d + 32, o + 8);
+            if (n0 + c < p.ldg) {      // (a piece is as wide as its G: its last tile may be wider)
+              char* d = p.g + ((long long)row * p.ldg + n0 + c) * 2;
+              st256(d, o);
+              st256(d + 32, o + 8);
+            }
           }
         }
         if (MODE == LSE && in) p.part[(long long)(n0 / BN) * p.rows_pad + row] = make_float2(m, sum);
       } else {
-        const bool in = row < (MODE == DX ? count : min(p.vn, p.V - p.v0));
+        const bool in = row < (q.w ? min(p.vn, p.V - p.v0) : count);
         const float coef = *p.coef * GScale<T>::down;
-        const bool fin = MODE == DW || p.last;
-        long long orow = 0;
-        if (in) orow = MODE == DX ? (long long)p.idx[row] * p.D : (long long)(p.v0 + row) * p.D;
+        float* sum = nullptr;
+        char* out = nullptr;
+        bool add = false;
+        if (q.w) {
+          if (p.split_w > 1) sum = p.slab_w + ((long long)q.split * p.vn + row) * p.D;
+          else out = p.dw + (long long)(p.v0 + row) * p.D * 2;
+        } else {
+          sum = p.slab_x + ((long long)q.split * p.rows_pad + row) * p.D;
+          add = !p.first;
+          if (in && p.last && p.split_x == 1) out = p.dx + (long long)p.idx[row] * p.D * 2;
+        }
 #pragma unroll 1
         for (int c = 0; c < BN; c += 32) {
           uint32_t r[32];
           __syncwarp();
           ld32(src + c, r);
           wait_ld(r);
-          if (!nk) {
+          if (nothing) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0;
           }
-          if (!in) continue;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int col = n0 + c + 8 * q;
-            if (col >= p.D) break;
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * q + j]);
-            float4* ac = reinterpret_cast<float4*>(p.acc + (long long)row * p.D + col);
-            if (MODE == DX && !p.first) {
-              const float4 x = ac[0], y = ac[1];
-              v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-              v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-            }
-            if (fin) {
-              uint4 o;
-              o.x = pack2<T>(v[0] * coef, v[1] * coef);
-              o.y = pack2<T>(v[2] * coef, v[3] * coef);
-              o.z = pack2<T>(v[4] * coef, v[5] * coef);
-              o.w = pack2<T>(v[6] * coef, v[7] * coef);
-              *reinterpret_cast<uint4*>(p.out + (orow + col) * 2) = o;
-            } else {
-              ac[0] = make_float4(v[0], v[1], v[2], v[3]);
-              ac[1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
-          }
+          if (in) finish_cols<T>(r, n0 + c, p.D, sum, add, out, coef);
         }
       }
       fence_before();
-      if (nk) bar_arrive(free_b + 8 * buf);
+      if (nothing) continue;
+      bar_arrive(free_b + 8 * buf);
       if (++buf == 2) { buf = 0; bph ^= 1u; }
     }
   }
   __syncthreads();
   if (fault.raised) drain_after_abort();
   __syncthreads();
-  if (warp == 1) tmem_free(tmem, 512);
+  if (warp == 1) tmem_free(tmem, 2 * BN);
+}
+
+// Joins the slabs of a split sum, in their order: rows of dx go where they came from, rows of dW stay (blockIdx.y).
+template <typename T>
+__global__ void __launch_bounds__(256) ce_finish(const GemmArgs p) {
+  dependent_launch();
+  const bool w = blockIdx.y == 0;
+  const int splits = w ? p.split_w : p.split_x;
+  if (splits < 2 || !(w ? p.dw : p.dx)) return;
+  const int count = *(volatile const int*)p.count;
+  const float coef = *p.coef * GScale<T>::down;
+  const long long words = p.D / 8, rows = w ? p.vn : count, apart = (long long)(w ? p.vn : p.rows_pad) * p.D;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * words; i += (long long)gridDim.x * 256) {
+    const long long row = i / words;
+    const float* f = (w ? p.slab_w : p.slab_x) + i * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(f + k * apart)), y = __ldcg(reinterpret_cast<const float4*>(f + k * apart) + 1);
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    uint4 o;
+    o.x = pack2<T>(v[0] * coef, v[1] * coef);
+    o.y = pack2<T>(v[2] * coef, v[3] * coef);
+    o.z = pack2<T>(v[4] * coef, v[5] * coef);
+    o.w = pack2<T>(v[6] * coef, v[7] * coef);
+    char* out = w ? p.dw + i * 16 : p.dx + ((long long)p.idx[row] * words + i % words) * 16;
+    *reinterpret_cast<uint4*>(out) = o;
+  }
 }
 
 // Which rows have a label: positions among them by a scan (one CTA; thread = a run of neighbouring rows).
@@ -483,29 +565,78 @@ struct Fwd { float2* part; float* tlogit; double* sums; };
 long long fwd_layout(char* base, long long N, int V, Fwd* w) {
   Carve c{base};
   const long long pad = up(N, BM);
-  w->part = c.take<float2>(pad * 8 * ((V + BN - 1) / BN));
+  w->part = c.take<float2>(pad * 8 * ((V + 127) / 128));
   w->tlogit = c.take<float>(pad * 4);
   w->sums = c.take<double>(pad / 32 * 8);
   return c.at;
 }
 
-// Width of a piece of the vocabulary: its G takes kPieceBytes at most (it stays in L2 from the kernel that writes it to
-// those that read it), and the pieces are even.
-int piece_width(long long N, int V) {
-  const long long pad = up(N, BM), most = kPieceBytes / (pad * 2) / BN * BN;
-  const long long one = most < BN ? BN : most;
-  const long long pieces = (V + one - 1) / one;
-  return (int)up((V + pieces - 1) / pieces, BN);
+// Tiles of 128 columns where those of 256 would leave so many SMs without one in the last round that the narrower ones, which
+// run at 0.8 of the rate, are done sooner (33 rows, 50257 columns of 1024: 22.7 -> 18 us).
+bool narrow(long long rows_t, long long columns, int sms) {
+  const long long wide = (rows_t * ((columns + 255) / 256) + sms - 1) / sms, thin = (rows_t * ((columns + 127) / 128) + sms - 1) / sms;
+  return thin * 10 < wide * 16;
 }
 
-struct Bwd { float* gs; float* coef; float* acc; char* g; };
-long long bwd_layout(char* base, long long N, int D, int V, Bwd* w) {
+// How the backward pass is cut for N rows: the width of a piece of the vocabulary (its G takes kPieceBytes at most, so that
+// much of it is still in L2 when it is read), and into how many shares the sums of dW and dx are split where there are too
+// few tiles for the SMs.
+struct Plan { int width, pieces, split_w, split_x; bool narrow_g, narrow_d; };
+
+// The longest CTA of a launch in which CTA c takes the tiles c, c + sms, ...: `first` tiles of length `a`, then `second` of length
+// `b`.  What a CTA has changes only at the remainders of the two counts.
+long long longest(long long first, long long a, long long second, long long b, int sms) {
+  long long most = 0;
+  for (const long long c : {0ll, first % sms, (first + second) % sms}) {
+    const long long n = (first + second - c + sms - 1) / sms, n1 = (first - c + sms - 1) / sms;
+    const long long l = n1 * a + (n - n1) * b;
+    if (l > most) most = l;
+  }
+  return most;
+}
+
+Plan make_plan(long long N, int D, int V, int sms) {
+  const long long pad = up(N, BM), rows_t = pad / BM, kw = (N + BK - 1) / BK;
+  Plan q{};
+  q.narrow_d = D <= 128 || narrow(1, D, 1);
+  const int bn = q.narrow_d ? 128 : 256;
+  const long long nt = (D + bn - 1) / bn;
+  long long most = kPieceBytes / (pad * 2) / BM * BM;
+  if (most < 256) most = 256;
+  if (most > up(V, BM)) most = up(V, BM);
+  // the width at which the launches' last rounds waste least: products of G in tiles, then dW and dx together
+  long long best = -1;
+  const long long step = up(most / 64, BM);
+  for (long long width = most; width >= 256 && width * 2 > most; width -= step) {
+    const long long pieces = (V + width - 1) / width, g = (rows_t * ((width + 255) / 256) + sms - 1) / sms * ((D + BK - 1) / BK) * 2;
+    const long long d = longest(width / BM * nt, kw, rows_t * nt, width / BK, sms) * (bn / 128);
+    const long long cost = pieces * (g + d + 8);      // (8: a launch's first loads and last stores, in steps)
+    if (best < 0 || cost < best) {
+      best = cost;
+      q.width = (int)width;
+    }
+  }
+  if (best < 0) q.width = (int)most;
+  q.pieces = (V + q.width - 1) / q.width;
+  const long long voc_t = (q.width + BM - 1) / BM, kx = q.width / BK;
+  long long target = (voc_t * nt * kw + rows_t * nt * kx + sms - 1) / sms;
+  if (target < 8) target = 8;
+  const auto split = [&](long long k) { const long long n = 2 * k > 3 * target ? (k + target - 1) / target : 1; return (int)(n > 32 ? 32 : n); };
+  q.split_x = split(kx);
+  q.split_w = q.pieces == 1 ? split(kw) : 1;
+  q.narrow_g = narrow(rows_t, q.width, sms);
+  return q;
+}
+
+struct Bwd { float* gs; float* coef; float* slab_x; float* slab_w; char* g; };
+long long bwd_layout(char* base, long long N, int D, int V, const Plan& q, Bwd* w) {
   Carve c{base};
   const long long pad = up(N, BM);
   w->gs = c.take<float>(pad * 4);
   w->coef = c.take<float>(4);
-  w->acc = c.take<float>(pad * D * 4);
-  w->g = c.take<char>(pad * piece_width(N, V) * 2);
+  w->slab_x = c.take<float>(pad * D * 4 * q.split_x);
+  w->slab_w = c.take<float>(q.split_w > 1 ? (long long)q.width * D * 4 * q.split_w : 0);
+  w->g = c.take<char>(pad * q.width * 2);
   return c.at;
 }
 
@@ -515,9 +646,9 @@ int sm_count() {
   return n;
 }
 
-template <typename T, int MODE>
-cudaError_t gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, long long tiles, int sms, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(ce_gemm<T, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
+template <typename T, int MODE, int BN>
+cudaError_t gemm_of(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& g, const GemmArgs& p, long long tiles, int sms, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(ce_gemm<T, MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
@@ -525,11 +656,15 @@ cudaError_t gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, 
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)(tiles < sms ? tiles : sms));
   cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = kGemmSmem;
+  cfg.dynamicSmemBytes = kGemmSmem<BN>;
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, ce_gemm<T, MODE>, a, b, p);
+  return cudaLaunchKernelEx(&cfg, ce_gemm<T, MODE, BN>, x, w, g, p);
+}
+template <typename T, int MODE>
+cudaError_t gemm(bool thin, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& g, const GemmArgs& p, long long tiles, int sms, cudaStream_t stream) {
+  return thin ? gemm_of<T, MODE, 128>(x, w, g, p, tiles, sms, stream) : gemm_of<T, MODE, 256>(x, w, g, p, tiles, sms, stream);
 }
 
 bool map2(CUtensorMap* m, int dtype, const void* base, long long inner, long long rows, long long ld) {
@@ -543,36 +678,32 @@ bool sizes_ok(int dtype, long long N, int D, int V, int reduction) {
 }
 
 template <typename T>
-int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, const Bwd& b, char* dx, char* dw, int sms,
+int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, const Bwd& b, const Plan& q, char* dx, char* dw, int sms,
              cudaStream_t stream) {
   const long long pad = up(N, BM);
-  const int width = piece_width(N, V);
   CUtensorMap mx, mw, mg;
-  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D) || !map2(&mg, dtype, b.g, width, pad, width)) return CHB_ERR_CUDA;
+  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D) || !map2(&mg, dtype, b.g, q.width, pad, q.width)) return CHB_ERR_CUDA;
   GemmArgs p{};
   p.count = sv.head;
   p.N = N; p.V = V; p.D = D;
-  p.tgt = sv.tgt; p.lse2 = sv.lse2; p.gs = b.gs; p.g = b.g; p.ldg = width;
-  p.acc = b.acc; p.coef = b.coef; p.idx = sv.idx;
+  p.tgt = sv.tgt; p.lse2 = sv.lse2; p.gs = b.gs; p.g = b.g; p.ldg = q.width;
+  p.slab_x = b.slab_x; p.slab_w = b.slab_w; p.split_x = q.split_x; p.split_w = q.split_w;
+  p.rows_pad = (int)pad;
+  p.coef = b.coef; p.idx = sv.idx; p.dx = dx; p.dw = dw;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;
-  const long long mt = pad / BM, dt = (D + BN - 1) / BN;
-  for (int v0 = 0; v0 < V; v0 += width) {
+  const long long rows_t = pad / BM, bg = q.narrow_g ? 128 : 256, bd = q.narrow_d ? 128 : 256, nt = (D + bd - 1) / bd;
+  for (int v0 = 0; v0 < V; v0 += q.width) {
     p.v0 = v0;
-    p.vn = V - v0 < width ? V - v0 : width;
+    p.vn = V - v0 < q.width ? V - v0 : q.width;
     p.first = v0 == 0;
-    p.last = v0 + width >= V;
-    p.K = D;
-    if (gemm<T, GRAD>(mx, mw, p, mt * ((p.vn + BN - 1) / BN), sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
-    if (dw) {
-      p.out = dw;
-      if (gemm<T, DW>(mg, mx, p, (p.vn + BM - 1) / BM * dt, sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
-    }
-    if (dx) {
-      p.out = dx;
-      p.K = p.vn;
-      if (gemm<T, DX>(mg, mw, p, mt * dt, sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
-    }
+    p.last = v0 + q.width >= V;
+    if (gemm<T, GRAD>(q.narrow_g, mx, mw, mg, p, rows_t * ((p.vn + bg - 1) / bg), sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
+    const long long tiles = (dw ? (p.vn + BM - 1) / BM * nt * q.split_w : 0) + (dx ? rows_t * nt * q.split_x : 0);
+    if (gemm<T, BOTH>(q.narrow_d, mx, mw, mg, p, tiles, sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
+  }
+  if (q.split_x > 1 || q.split_w > 1) {
+    if (launch_overlapped(ce_finish<T>, dim3((unsigned)(2 * sms), 2), dim3(256), stream, p) != cudaSuccess) return CHB_ERR_CUDA;
   }
   return CHB_SUCCESS;
 }
@@ -591,7 +722,9 @@ int chb_linear_ce_bytes(long long N, int D, int V, long long* saved, long long* 
   Bwd b;
   *saved = saved_layout(nullptr, N, D, &sv);
   *forward = fwd_layout(nullptr, N, V, &f);
-  *backward = bwd_layout(nullptr, N, D, V, &b);
+  const int sms = sm_count();
+  if (!sms) return CHB_ERR_CUDA;
+  *backward = bwd_layout(nullptr, N, D, V, make_plan(N, D, V, sms), &b);
   return CHB_SUCCESS;
 }
 
@@ -604,21 +737,24 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
   saved_layout(static_cast<char*>(saved), N, D, &sv);
   fwd_layout(static_cast<char*>(work), N, V, &f);
   const long long pad = up(N, BM);
-  const int sms = sm_count(), nt = (V + BN - 1) / BN, n = (int)N;
+  const int sms = sm_count(), n = (int)N;
+  if (!sms) return CHB_ERR_CUDA;
+  const bool thin = narrow(pad / BM, V, sms);
+  const int bn = thin ? 128 : 256, nt = (V + bn - 1) / bn;
   CUtensorMap mx, mw;
-  if (!sms || !map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D)) return CHB_ERR_CUDA;
+  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D)) return CHB_ERR_CUDA;
   if (launch_overlapped(ce_rows, dim3(1), dim3(1024), stream, targets, n, V, ignore_index, sv) != cudaSuccess) return CHB_ERR_CUDA;
   if (launch_overlapped(ce_gather, dim3((unsigned)(pad / 8)), dim3(256), stream, (const char*)x, ldx, n, D, sv,
                         reduction == 0 ? loss : nullptr) != cudaSuccess) return CHB_ERR_CUDA;
   GemmArgs p{};
   p.count = sv.head;
-  p.N = n; p.V = V; p.D = D; p.K = D; p.vn = V;
+  p.N = n; p.V = V; p.D = D; p.vn = V;
   p.part = f.part; p.tlogit = f.tlogit; p.tgt = sv.tgt; p.rows_pad = (int)pad;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;
   const long long tiles = pad / BM * nt;
-  const cudaError_t e = dtype == CHB_F16 ? gemm<__half, LSE>(mx, mw, p, tiles, sms, stream)
-                                         : gemm<__nv_bfloat16, LSE>(mx, mw, p, tiles, sms, stream);
+  const cudaError_t e = dtype == CHB_F16 ? gemm<__half, LSE>(thin, mx, mw, mw, p, tiles, sms, stream)
+                                         : gemm<__nv_bfloat16, LSE>(thin, mx, mw, mw, p, tiles, sms, stream);
   if (e != cudaSuccess) return CHB_ERR_CUDA;
   if (launch_overlapped(ce_join, dim3((unsigned)(pad / 32)), dim3(256), stream, (const float2*)f.part, (const float*)f.tlogit, nt, (int)pad,
                         reduction, sv, f.sums, loss) != cudaSuccess) return CHB_ERR_CUDA;
@@ -630,19 +766,20 @@ int chb_linear_ce_backward(int dtype, const void* w, const float* grad, long lon
   if (!sizes_ok(dtype, N, D, V, reduction) || !w || !grad || !saved || !work || (reinterpret_cast<uintptr_t>(w) & 15u)) return CHB_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15u) return CHB_ERR_ARG;
   if (!dx && !dw) return CHB_SUCCESS;
-  Saved sv;
-  Bwd b;
-  saved_layout(static_cast<char*>(const_cast<void*>(saved)), N, D, &sv);
-  bwd_layout(static_cast<char*>(work), N, D, V, &b);
   const int sms = sm_count();
   if (!sms) return CHB_ERR_CUDA;
+  Saved sv;
+  Bwd b;
+  const Plan q = make_plan(N, D, V, sms);
+  saved_layout(static_cast<char*>(const_cast<void*>(saved)), N, D, &sv);
+  bwd_layout(static_cast<char*>(work), N, D, V, q, &b);
   const long long rows8 = (N + 7) / 8;
   if (launch_overlapped(ce_weights, dim3((unsigned)(rows8 < 2 * sms ? rows8 : 2 * sms)), dim3(256), stream, grad, reduction, (int)N, D,
                         sv, b.gs, b.coef, static_cast<char*>(dx)) != cudaSuccess) return CHB_ERR_CUDA;
   char *x = static_cast<char*>(dx), *v = static_cast<char*>(dw);
   const char* ww = static_cast<const char*>(w);
-  return dtype == CHB_F16 ? backward<__half>(dtype, ww, (int)N, D, V, sv, b, x, v, sms, stream)
-                          : backward<__nv_bfloat16>(dtype, ww, (int)N, D, V, sv, b, x, v, sms, stream);
+  return dtype == CHB_F16 ? backward<__half>(dtype, ww, (int)N, D, V, sv, b, q, x, v, sms, stream)
+                          : backward<__nv_bfloat16>(dtype, ww, (int)N, D, V, sv, b, q, x, v, sms, stream);
 }
 
 }  // extern "C"

@@ -301,9 +301,10 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 # ---------------------------------------------------------------------------------------------- output layer and loss
 
 @lru_cache(maxsize=256)
-def _loss_bytes(n: int, d: int, v: int):
+def _loss_bytes(device: torch.device, n: int, d: int, v: int):
     sizes = i64(0), i64(0), i64(0)
-    rc = N.lib().chb_linear_ce_bytes(n, d, v, *(C.byref(x) for x in sizes))
+    with torch.cuda.device(device):
+        rc = N.lib().chb_linear_ce_bytes(n, d, v, *(C.byref(x) for x in sizes))
     if rc:
         raise OperatorError(f"chb_linear_ce_bytes failed: {N.ERR_NAMES.get(rc, rc)}")
     return tuple(x.value for x in sizes)
@@ -311,7 +312,7 @@ def _loss_bytes(n: int, d: int, v: int):
 
 def _loss_forward(x, weight, targets, ignore_index, reduction):
     (n, d), v, dev = x.shape, weight.shape[0], x.device
-    kept, temporary, _ = _loss_bytes(n, d, v)
+    kept, temporary, _ = _loss_bytes(dev, n, d, v)
     saved = torch.empty(kept, dtype=torch.uint8, device=dev)
     work = torch.empty(temporary, dtype=torch.uint8, device=dev)
     loss = torch.empty((n,) if reduction == 0 else (), dtype=torch.float32, device=dev)
@@ -336,7 +337,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         (v, d), dev, dtype = weight.shape, weight.device, weight.dtype
         dx = torch.empty((n, d), dtype=dtype, device=dev) if ctx.needs_input_grad[0] else None
         dw = torch.empty((v, d), dtype=dtype, device=dev) if ctx.needs_input_grad[1] else None
-        work = torch.empty(_loss_bytes(n, d, v)[2], dtype=torch.uint8, device=dev)
+        work = torch.empty(_loss_bytes(dev, n, d, v)[2], dtype=torch.uint8, device=dev)
         w, g = _aligned(weight), grad.to(torch.float32).contiguous()
         _call("chb_linear_ce_backward", dev, DTYPES[dtype], w.data_ptr(), g.data_ptr(), n, d, v, reduction, saved.data_ptr(), work.data_ptr(),
               None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr())

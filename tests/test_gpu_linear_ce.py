@@ -82,7 +82,7 @@ def test_matches_the_formula(cuda, dtype, reduction, n, d, v, ignored):
 
 
 def test_several_pieces_of_the_vocabulary(cuda):
-    check(*make(8192, 64, 7001, torch.bfloat16, 0.2), "mean")      # 114 MB of G: two pieces
+    check(*make(8192, 64, 7001, torch.bfloat16, 0.2), "mean")      # 114 MB of G: several pieces
 
 
 def test_negative_and_zero_gradients(cuda):
