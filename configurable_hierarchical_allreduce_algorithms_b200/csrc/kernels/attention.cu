@@ -906,23 +906,6 @@ bool map3(CUtensorMap* m, int dtype, const void* base, long long T, int heads, i
   return make_map(m, dtype, base, 3, d, s, TILE);
 }
 
-template <typename K, typename... A>
-cudaError_t launch(K kernel, int smem, dim3 grid, int threads, cudaStream_t stream, A... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Units (tiles, or pairs of (tile, head)) that T rows in so many sequences can make at most; each sequence has a tile more than
 // its rows fill, and there may be rows before the first and behind the last.
 long long most_units(long long T, int seqs, bool bounds, int group) {
@@ -954,18 +937,23 @@ AttnArgs common_args(long long T, int heads, int kv_heads, int D, const int* cu,
 
 template <typename T, int DP>
 int run_forward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaStream_t s) {
-  return launch(attn_forward<T, DP>, 6 * DP / 64 * kAtom + 1024, dim3((unsigned)(p.kv_heads * units)), kFwdThreads, s, m[0], m[1], m[2], p) ==
+  static std::atomic<unsigned long long> done{0};
+  return launch_big(attn_forward<T, DP>, 6 * DP / 64 * kAtom + 1024, (unsigned)(p.kv_heads * units), kFwdThreads, s, done, m[0], m[1], m[2], p) ==
                  cudaSuccess ? CHB_SUCCESS : CHB_ERR_CUDA;
 }
 template <typename T, int DP>
 int run_backward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaStream_t s) {
-  constexpr int kMost = 227 * 1024;      // of a CTA, static and dynamic
-  const int smem = 7 * DP / 64 * kAtom + 1024;
-  cudaFuncAttributes f{};
-  if (cudaFuncGetAttributes(&f, attn_dkv<T, DP>) != cudaSuccess) return CHB_ERR_CUDA;
-  const int left = kMost - (int)f.sharedSizeBytes;
-  if (launch(attn_dq<T, DP>, smem, dim3((unsigned)(p.heads * units)), kBwdThreads, s, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
-      launch(attn_dkv<T, DP>, smem < left ? smem : left, dim3((unsigned)(p.kv_heads * units)), kBwdThreads, s, m[0], m[1], m[2], m[3], p) != cudaSuccess)
+  constexpr int kMost = 227 * 1024, kNeed = 7 * DP / 64 * kAtom + 1024;      // (of a CTA, static and dynamic)
+  static std::atomic<unsigned long long> done_q{0}, done_kv{0};
+  static std::atomic<int> own{0};      // static shared memory of attn_dkv
+  if (!own.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes f{};
+    if (cudaFuncGetAttributes(&f, attn_dkv<T, DP>) != cudaSuccess) return CHB_ERR_CUDA;
+    own.store((int)f.sharedSizeBytes, std::memory_order_relaxed);
+  }
+  const int left = kMost - own.load(std::memory_order_relaxed);
+  if (launch_big(attn_dq<T, DP>, kNeed, (unsigned)(p.heads * units), kBwdThreads, s, done_q, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
+      launch_big(attn_dkv<T, DP>, kNeed < left ? kNeed : left, (unsigned)(p.kv_heads * units), kBwdThreads, s, done_kv, m[0], m[1], m[2], m[3], p) != cudaSuccess)
     return CHB_ERR_CUDA;
   return CHB_SUCCESS;
 }

@@ -343,12 +343,6 @@ cudaError_t launch(const RopeArgs& a, const Turns& t, bool interleaved, bool bac
   return interleaved ? launch_order<T, V, true>(a, t, back, sms, s) : launch_order<T, V, false>(a, t, back, sms, s);
 }
 
-int device_sms() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return sms;
-}
-
 // The fractions of a turn for one base and D, kept from call to call (as a program keeps its tables): the last few.
 const Turns& turns_of(double base, int D) {
   struct Entry { double base; int D; Turns t; };
@@ -375,7 +369,7 @@ extern "C" {
 
 // Most rows of partial sums of a backward launch on the current device (of D floats each).
 int chb_head_rope_rows(int heads_q, int heads_k, int* out) {
-  const int sms = device_sms();
+  const int sms = tc::sm_count();
   if (!out || heads_q < 1 || heads_k < 1) return CHB_ERR_ARG;
   if (!sms) return CHB_ERR_CUDA;
   // (a share is a head at least, so there are no more shares than heads)
@@ -421,7 +415,7 @@ int chb_head_rope(int dtype, const void* const* x, const void* const* dy, void* 
   while (a.group < a.lanes) a.group *= 2;
   a.eps = eps;
   a.part = dy && w ? part : nullptr;
-  const int sms = device_sms();
+  const int sms = tc::sm_count();
   if (!sms) return CHB_ERR_CUDA;
   const bool back = dy != nullptr, in = interleaved != 0;
   share_out(&a, sms);

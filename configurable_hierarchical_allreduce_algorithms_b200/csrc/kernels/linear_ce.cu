@@ -20,12 +20,10 @@ namespace {
 
 using namespace tc;
 
-constexpr int BM = 128, BK = 64;
-constexpr int kBox = 64 * 128;                               // bytes of one load: 64 rows of 64 elements
-// 192 KB of operands in flight; tiles of 256 columns run at the tensor cores' rate, tiles of 128 leave fewer SMs idle
-template <int BN> constexpr int kStages = BN == 256 ? 4 : 6;
-template <int BN> constexpr int kStageBytes = (BM + BN) * BK * 2;
-template <int BN> constexpr int kGemmSmem = kStages<BN> * kStageBytes<BN> + 1024;      // (1024: the swizzle's alignment)
+constexpr int BM = 128, BN = 256, BK = 64, kStages = 4;      // (BN: a tile's columns at most)
+constexpr int kBox = 64 * 128;                               // bytes of 64 rows of 64 elements
+constexpr int kStageBytes = (BM + BN) * BK * 2;
+constexpr int kGemmSmem = kStages * kStageBytes + 1024;      // (1024: the swizzle's alignment)
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode { LSE, GRAD, BOTH };      // BOTH: dW and dx of a piece in one launch
@@ -44,6 +42,7 @@ struct GemmArgs {
   const int* count;
   int N, V, v0, vn;          // rows of x at most; vocabulary, first column and width of the piece
   int D;
+  int bn;                    // columns of a tile: a multiple of 32 (GRAD and BOTH: of 64)
   // LSE
   float2* part;
   float* tlogit;
@@ -109,11 +108,12 @@ struct TilePlace {
 };
 
 // One persistent CTA per SM; warp 0 loads, warp 1 issues the products, warps 4 to 7 finish a tile (thread = row) while the
-// next one is summed in the other half of tensor memory.  Maps: LSE and GRAD gathered rows and W; BOTH also G.
-template <typename T, int MODE, int BN>
+// next one is summed in the other half of tensor memory.  Maps: gathered rows, W (LSE and GRAD: boxes of a tile's columns, else
+// of 64), and BOTH: G.
+template <typename T, int MODE>
 __global__ void __launch_bounds__(256, 1)
 ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mg, const GemmArgs p) {
-  constexpr int STAGES = kStages<BN>, STAGE = kStageBytes<BN>;
+  constexpr int STAGES = kStages, STAGE = kStageBytes;
   extern __shared__ char smem_raw[];
   __shared__ __align__(8) unsigned long long full_[STAGES], empty_[STAGES], done_[2], free_[2];
   __shared__ uint32_t tmem_;
@@ -138,7 +138,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
   dependent_launch();
   const uint32_t tmem = tmem_;
   const int count = *(volatile const int*)p.count;
-  const int rows_t = (count + BM - 1) / BM, nt = ((MODE == BOTH ? p.D : p.vn) + BN - 1) / BN;
+  const int bn = p.bn, rows_t = (count + BM - 1) / BM, nt = ((MODE == BOTH ? p.D : p.vn) + bn - 1) / bn;
   const int voc_t = (p.vn + BM - 1) / BM;
   const int kd = (p.D + BK - 1) / BK, kw = (count + BK - 1) / BK, kx = (p.vn + BK - 1) / BK;
   const int tiles_w = MODE == BOTH && p.dw ? voc_t * nt * p.split_w : 0;
@@ -148,7 +148,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
     TilePlace q{};
     if (MODE != BOTH) {
       q.m0 = t % rows_t * BM;
-      q.n0 = t / rows_t * BN;
+      q.n0 = t / rows_t * bn;
       q.k1 = kd;
       return q;
     }
@@ -158,7 +158,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
     q.split = t / per;
     t -= q.split * per;
     q.m0 = t / nt * BM;
-    q.n0 = t % nt * BN;
+    q.n0 = t % nt * bn;
     q.k0 = (int)((long long)k * q.split / splits);
     q.k1 = (int)((long long)k * (q.split + 1) / splits);
     return q;
@@ -175,22 +175,19 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
         if (!(ok = bar_wait_warp(empty + 8 * s, ph ^ 1u, &fault))) break;
         const uint32_t bar = full + 8 * s, a = smem + s * STAGE, b = a + BM * BK * 2;
         if (one) {
-          bar_expect(bar, STAGE);
+          bar_expect(bar, (BM + bn) * BK * 2);
           if (MODE != BOTH) {
 #pragma unroll
             for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mx, k * BK, q.m0 + 64 * j, bar);
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j) load2(b + j * kBox, &mw, k * BK, p.v0 + q.n0 + 64 * j, bar);
+            load2(b, &mw, k * BK, p.v0 + q.n0, bar);
           } else if (q.w) {
 #pragma unroll
             for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mg, q.m0 + 64 * j, k * BK, bar);
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j) load2(b + j * kBox, &mx, q.n0 + 64 * j, k * BK, bar);
+            for (int j = 0; j < bn / 64; ++j) load2(b + j * kBox, &mx, q.n0 + 64 * j, k * BK, bar);
           } else {
 #pragma unroll
             for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mg, k * BK, q.m0 + 64 * j, bar);
-#pragma unroll
-            for (int j = 0; j < BN / 64; ++j) load2(b + j * kBox, &mw, q.n0 + 64 * j, p.v0 + k * BK, bar);
+            for (int j = 0; j < bn / 64; ++j) load2(b + j * kBox, &mw, q.n0 + 64 * j, p.v0 + k * BK, bar);
           }
         }
         __syncwarp();
@@ -207,7 +204,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
       if (q.k0 == q.k1) continue;
       const bool a_mn = MODE == BOTH && q.w;
       constexpr bool b_mn = MODE == BOTH;
-      const uint32_t desc = a_mn ? product_desc<T>(BM, BN, true, b_mn) : product_desc<T>(BM, BN, false, b_mn);
+      const uint32_t desc = product_desc<T>(BM, bn, a_mn, b_mn);
       const uint32_t a_step = a_mn ? 128 : 2;
       if (!(ok = bar_wait_warp(free_b + 8 * buf, bph ^ 1u, &fault))) break;
       fence_after();
@@ -243,12 +240,12 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
       if (MODE != BOTH) {
         const bool in = row < count;
         const int tg = in ? p.tgt[row] - p.v0 - n0 : -1;
-        const int cols = min(BN, p.V - p.v0 - n0);
+        const int cols = min(bn, p.V - p.v0 - n0);
         float m = -INFINITY, sum = 0.f;
         float lse = 0.f, gs = 0.f;
         if (MODE == GRAD && in) { lse = p.lse2[row]; gs = p.gs[row] * GScale<T>::up; }
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = 0; c < bn; c += 32) {
           uint32_t r[32];
           __syncwarp();
           ld32(src + c, r);
@@ -298,7 +295,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
             }
           }
         }
-        if (MODE == LSE && in) p.part[(long long)(n0 / BN) * p.rows_pad + row] = make_float2(m, sum);
+        if (MODE == LSE && in) p.part[(long long)(n0 / bn) * p.rows_pad + row] = make_float2(m, sum);
       } else {
         const bool in = row < (q.w ? min(p.vn, p.V - p.v0) : count);
         const float coef = *p.coef * GScale<T>::down;
@@ -314,7 +311,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
           if (in && p.last && p.split_x == 1) out = p.dx + (long long)p.idx[row] * p.D * 2;
         }
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
+        for (int c = 0; c < bn; c += 32) {
           uint32_t r[32];
           __syncwarp();
           ld32(src + c, r);
@@ -429,6 +426,67 @@ __global__ void __launch_bounds__(256) ce_gather(const char* x, long long ldx, i
   if (r >= count && r < pad) {
     uint4* d = reinterpret_cast<uint4*>(sv.xc + (long long)r * D * 2);
     for (int i = lane; i < words; i += 32) d[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// Both in one launch for few rows: every CTA counts the labels ahead of its own eight rows for itself (and all of them, for the
+// zeros behind the last).
+constexpr int kCountedRows = 4096;
+__global__ void __launch_bounds__(256)
+ce_gather_few(const long long* targets, const char* x, long long ldx, int N, int D, int V, long long ignore, Saved sv, float* loss_rows) {
+  __shared__ int before_[8], all_[8];
+  dependent_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.x * 8;
+  int before = 0, all = 0;
+  for (int r = threadIdx.x; r < N; r += 256) {
+    const int in = targets[r] != ignore;
+    all += in;
+    before += r < r0 ? in : 0;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (lane == 0) {
+    before_[warp] = before;
+    all_[warp] = all;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int k = 0; k < 8; ++k) {
+    before += before_[k];
+    all += all_[k];
+  }
+  const int r = r0 + warp;
+  const long long mine = lane < 8 && r0 + lane < N ? targets[r0 + lane] : ignore;
+  const unsigned in = __ballot_sync(0xffffffffu, mine != ignore);
+  const int at = before + __popc(in & ((1u << warp) - 1u)), words = D / 8;
+  const long long t = __shfl_sync(0xffffffffu, mine, warp);
+  if (r < N) {
+    const bool has = (in >> warp) & 1u;
+    if (lane == 0) {
+      sv.pos[r] = has ? at : -1;
+      if (has) {
+        sv.idx[at] = r;
+        sv.tgt[at] = t >= 0 && t < V ? (int)t : -1;
+      } else if (loss_rows) {
+        loss_rows[r] = 0.f;
+      }
+    }
+    if (has) {
+      const uint4* s = reinterpret_cast<const uint4*>(x + (long long)r * ldx * 2);
+      uint4* d = reinterpret_cast<uint4*>(sv.xc + (long long)at * D * 2);
+      for (int i = lane; i < words; i += 32) d[i] = s[i];
+    }
+  }
+  if (r >= all && r < (all + BM - 1) / BM * BM) {
+    uint4* d = reinterpret_cast<uint4*>(sv.xc + (long long)r * D * 2);
+    for (int i = lane; i < words; i += 32) d[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    sv.head[0] = all;
+    sv.head[1] = 0;
   }
 }
 
@@ -562,26 +620,38 @@ long long saved_layout(char* base, long long N, int D, Saved* sv) {
 }
 
 struct Fwd { float2* part; float* tlogit; double* sums; };
-long long fwd_layout(char* base, long long N, int V, Fwd* w) {
+long long fwd_layout(char* base, long long N, int V, int bn, Fwd* w) {
   Carve c{base};
   const long long pad = up(N, BM);
-  w->part = c.take<float2>(pad * 8 * ((V + 127) / 128));
+  w->part = c.take<float2>(pad * 8 * ((V + bn - 1) / bn));
   w->tlogit = c.take<float>(pad * 4);
   w->sums = c.take<double>(pad / 32 * 8);
   return c.at;
 }
 
-// Tiles of 128 columns where those of 256 would leave so many SMs without one in the last round that the narrower ones, which
-// run at 0.8 of the rate, are done sooner (33 rows, 50257 columns of 1024: 22.7 -> 18 us).
-bool narrow(long long rows_t, long long columns, int sms) {
-  const long long wide = (rows_t * ((columns + 255) / 256) + sms - 1) / sms, thin = (rows_t * ((columns + 127) / 128) + sms - 1) / sms;
-  return thin * 10 < wide * 16;
+// Columns of a tile of rows times W: 256 where there are many tiles, else the width at which the SMs' last round is fullest (33
+// rows, 50257 columns: 148 SMs have two tiles of 192 each instead of one or two of 256).
+int tile_columns(long long rows_t, long long columns, int sms, int unit) {
+  int best = BN;
+  long long least = -1;
+  for (long long rounds = 1; rounds <= 8; ++rounds) {
+    const long long across = rounds * sms / rows_t;      // column tiles that so many rounds have room for
+    if (!across) continue;
+    const long long bn = up((columns + across - 1) / across, unit);
+    if (bn > BN) continue;
+    const long long cost = rounds * ((bn < 128 ? 128 : bn) + 16);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = (int)bn;
+    }
+  }
+  return best;
 }
 
 // How the backward pass is cut for N rows: the width of a piece of the vocabulary (its G takes kPieceBytes at most, so that
 // much of it is still in L2 when it is read), and into how many shares the sums of dW and dx are split where there are too
 // few tiles for the SMs.
-struct Plan { int width, pieces, split_w, split_x; bool narrow_g, narrow_d; };
+struct Plan { int width, pieces, split_w, split_x, bn_g, bn_d; };
 
 // The longest CTA of a launch in which CTA c takes the tiles c, c + sms, ...: `first` tiles of length `a`, then `second` of length
 // `b`.  What a CTA has changes only at the remainders of the two counts.
@@ -598,9 +668,8 @@ long long longest(long long first, long long a, long long second, long long b, i
 Plan make_plan(long long N, int D, int V, int sms) {
   const long long pad = up(N, BM), rows_t = pad / BM, kw = (N + BK - 1) / BK;
   Plan q{};
-  q.narrow_d = D <= 128 || narrow(1, D, 1);
-  const int bn = q.narrow_d ? 128 : 256;
-  const long long nt = (D + bn - 1) / bn;
+  const long long nt = (D + BN - 1) / BN;
+  q.bn_d = (int)up((D + nt - 1) / nt, 64);
   long long most = kPieceBytes / (pad * 2) / BM * BM;
   if (most < 256) most = 256;
   if (most > up(V, BM)) most = up(V, BM);
@@ -609,7 +678,7 @@ Plan make_plan(long long N, int D, int V, int sms) {
   const long long step = up(most / 64, BM);
   for (long long width = most; width >= 256 && width * 2 > most; width -= step) {
     const long long pieces = (V + width - 1) / width, g = (rows_t * ((width + 255) / 256) + sms - 1) / sms * ((D + BK - 1) / BK) * 2;
-    const long long d = longest(width / BM * nt, kw, rows_t * nt, width / BK, sms) * (bn / 128);
+    const long long d = longest(width / BM * nt, kw, rows_t * nt, width / BK, sms) * q.bn_d / 128;
     const long long cost = pieces * (g + d + 8);      // (8: a launch's first loads and last stores, in steps)
     if (best < 0 || cost < best) {
       best = cost;
@@ -624,7 +693,7 @@ Plan make_plan(long long N, int D, int V, int sms) {
   const auto split = [&](long long k) { const long long n = 2 * k > 3 * target ? (k + target - 1) / target : 1; return (int)(n > 32 ? 32 : n); };
   q.split_x = split(kx);
   q.split_w = q.pieces == 1 ? split(kw) : 1;
-  q.narrow_g = narrow(rows_t, q.width, sms);
+  q.bn_g = tile_columns(rows_t, q.width, sms, 64);      // (dx sums over G in steps of 64: all of them have to be written)
   return q;
 }
 
@@ -640,36 +709,15 @@ long long bwd_layout(char* base, long long N, int D, int V, const Plan& q, Bwd* 
   return c.at;
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return n;
-}
-
-template <typename T, int MODE, int BN>
-cudaError_t gemm_of(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& g, const GemmArgs& p, long long tiles, int sms, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(ce_gemm<T, MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem<BN>);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(tiles < sms ? tiles : sms));
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = kGemmSmem<BN>;
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, ce_gemm<T, MODE, BN>, x, w, g, p);
-}
 template <typename T, int MODE>
-cudaError_t gemm(bool thin, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& g, const GemmArgs& p, long long tiles, int sms, cudaStream_t stream) {
-  return thin ? gemm_of<T, MODE, 128>(x, w, g, p, tiles, sms, stream) : gemm_of<T, MODE, 256>(x, w, g, p, tiles, sms, stream);
+cudaError_t gemm(const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& g, const GemmArgs& p, long long tiles, int sms, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  return launch_big(ce_gemm<T, MODE>, kGemmSmem, (unsigned)(tiles < sms ? tiles : sms), 256, stream, done, x, w, g, p);
 }
 
-bool map2(CUtensorMap* m, int dtype, const void* base, long long inner, long long rows, long long ld) {
+bool map2(CUtensorMap* m, int dtype, const void* base, long long inner, long long rows, long long ld, int box_rows = 64) {
   const unsigned long long d[2] = {(unsigned long long)inner, (unsigned long long)rows}, s[1] = {(unsigned long long)ld};
-  return make_map(m, dtype, base, 2, d, s, 64);
+  return make_map(m, dtype, base, 2, d, s, (unsigned)box_rows);
 }
 
 bool sizes_ok(int dtype, long long N, int D, int V, int reduction) {
@@ -681,8 +729,9 @@ template <typename T>
 int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, const Bwd& b, const Plan& q, char* dx, char* dw, int sms,
              cudaStream_t stream) {
   const long long pad = up(N, BM);
-  CUtensorMap mx, mw, mg;
-  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D) || !map2(&mg, dtype, b.g, q.width, pad, q.width)) return CHB_ERR_CUDA;
+  CUtensorMap mx, mw, mt, mg;
+  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D) || !map2(&mt, dtype, w, D, V, D, q.bn_g) ||
+      !map2(&mg, dtype, b.g, q.width, pad, q.width)) return CHB_ERR_CUDA;
   GemmArgs p{};
   p.count = sv.head;
   p.N = N; p.V = V; p.D = D;
@@ -692,15 +741,17 @@ int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, con
   p.coef = b.coef; p.idx = sv.idx; p.dx = dx; p.dw = dw;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;
-  const long long rows_t = pad / BM, bg = q.narrow_g ? 128 : 256, bd = q.narrow_d ? 128 : 256, nt = (D + bd - 1) / bd;
+  const long long rows_t = pad / BM, nt = (D + q.bn_d - 1) / q.bn_d;
   for (int v0 = 0; v0 < V; v0 += q.width) {
     p.v0 = v0;
     p.vn = V - v0 < q.width ? V - v0 : q.width;
     p.first = v0 == 0;
     p.last = v0 + q.width >= V;
-    if (gemm<T, GRAD>(q.narrow_g, mx, mw, mg, p, rows_t * ((p.vn + bg - 1) / bg), sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
+    p.bn = q.bn_g;
+    if (gemm<T, GRAD>(mx, mt, mg, p, rows_t * ((p.vn + p.bn - 1) / p.bn), sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
     const long long tiles = (dw ? (p.vn + BM - 1) / BM * nt * q.split_w : 0) + (dx ? rows_t * nt * q.split_x : 0);
-    if (gemm<T, BOTH>(q.narrow_d, mx, mw, mg, p, tiles, sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
+    p.bn = q.bn_d;
+    if (gemm<T, BOTH>(mx, mw, mg, p, tiles, sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
   }
   if (q.split_x > 1 || q.split_w > 1) {
     if (launch_overlapped(ce_finish<T>, dim3((unsigned)(2 * sms), 2), dim3(256), stream, p) != cudaSuccess) return CHB_ERR_CUDA;
@@ -721,9 +772,9 @@ int chb_linear_ce_bytes(long long N, int D, int V, long long* saved, long long* 
   Fwd f;
   Bwd b;
   *saved = saved_layout(nullptr, N, D, &sv);
-  *forward = fwd_layout(nullptr, N, V, &f);
   const int sms = sm_count();
   if (!sms) return CHB_ERR_CUDA;
+  *forward = fwd_layout(nullptr, N, V, tile_columns(up(N, BM) / BM, V, sms, 32), &f);
   *backward = bwd_layout(nullptr, N, D, V, make_plan(N, D, V, sms), &b);
   return CHB_SUCCESS;
 }
@@ -734,27 +785,31 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15u) return CHB_ERR_ARG;
   Saved sv;
   Fwd f;
-  saved_layout(static_cast<char*>(saved), N, D, &sv);
-  fwd_layout(static_cast<char*>(work), N, V, &f);
   const long long pad = up(N, BM);
   const int sms = sm_count(), n = (int)N;
   if (!sms) return CHB_ERR_CUDA;
-  const bool thin = narrow(pad / BM, V, sms);
-  const int bn = thin ? 128 : 256, nt = (V + bn - 1) / bn;
+  const int bn = tile_columns(pad / BM, V, sms, 32), nt = (V + bn - 1) / bn;
+  saved_layout(static_cast<char*>(saved), N, D, &sv);
+  fwd_layout(static_cast<char*>(work), N, V, bn, &f);
   CUtensorMap mx, mw;
-  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D)) return CHB_ERR_CUDA;
-  if (launch_overlapped(ce_rows, dim3(1), dim3(1024), stream, targets, n, V, ignore_index, sv) != cudaSuccess) return CHB_ERR_CUDA;
-  if (launch_overlapped(ce_gather, dim3((unsigned)(pad / 8)), dim3(256), stream, (const char*)x, ldx, n, D, sv,
-                        reduction == 0 ? loss : nullptr) != cudaSuccess) return CHB_ERR_CUDA;
+  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D, bn)) return CHB_ERR_CUDA;
+  float* const loss_rows = reduction == 0 ? loss : nullptr;
+  const char* const xs = static_cast<const char*>(x);
+  if (n <= kCountedRows) {
+    if (launch_overlapped(ce_gather_few, dim3((unsigned)(pad / 8)), dim3(256), stream, targets, xs, ldx, n, D, V, ignore_index, sv, loss_rows) != cudaSuccess) return CHB_ERR_CUDA;
+  } else if (launch_overlapped(ce_rows, dim3(1), dim3(1024), stream, targets, n, V, ignore_index, sv) != cudaSuccess ||
+             launch_overlapped(ce_gather, dim3((unsigned)(pad / 8)), dim3(256), stream, xs, ldx, n, D, sv, loss_rows) != cudaSuccess) {
+    return CHB_ERR_CUDA;
+  }
   GemmArgs p{};
   p.count = sv.head;
-  p.N = n; p.V = V; p.D = D; p.vn = V;
+  p.N = n; p.V = V; p.D = D; p.vn = V; p.bn = bn;
   p.part = f.part; p.tlogit = f.tlogit; p.tgt = sv.tgt; p.rows_pad = (int)pad;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;
   const long long tiles = pad / BM * nt;
-  const cudaError_t e = dtype == CHB_F16 ? gemm<__half, LSE>(thin, mx, mw, mw, p, tiles, sms, stream)
-                                         : gemm<__nv_bfloat16, LSE>(thin, mx, mw, mw, p, tiles, sms, stream);
+  const cudaError_t e = dtype == CHB_F16 ? gemm<__half, LSE>(mx, mw, mw, p, tiles, sms, stream)
+                                         : gemm<__nv_bfloat16, LSE>(mx, mw, mw, p, tiles, sms, stream);
   if (e != cudaSuccess) return CHB_ERR_CUDA;
   if (launch_overlapped(ce_join, dim3((unsigned)(pad / 32)), dim3(256), stream, (const float2*)f.part, (const float*)f.tlogit, nt, (int)pad,
                         reduction, sv, f.sums, loss) != cudaSuccess) return CHB_ERR_CUDA;

@@ -67,6 +67,26 @@ unsigned* status_word() {
   return known[dev];
 }
 
+int sm_count() {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
+  if ((n = known[dev].load(std::memory_order_relaxed))) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+bool allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (done.load(std::memory_order_relaxed) >> dev & 1) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return true;
+}
+
 }  // namespace tc
 }  // namespace chb
 

@@ -15,6 +15,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace chb {
 namespace tc {
 
@@ -255,6 +257,28 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
 
 // ------------------------------------------------------------------ host side
 unsigned* status_word();      // of the current device; null: no device
+int sm_count();               // of the current device; 0: no device
+
+// Lets a kernel have so much dynamic shared memory on the current device: asked for once (a device's bit in `done`, which
+// belongs to the kernel), as the question takes as long as a launch.
+bool allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done);
+
+// A launch that may start while the one before it drains
+template <typename K, typename... A>
+inline cudaError_t launch_big(K kernel, int smem, unsigned ctas, int threads, cudaStream_t stream, std::atomic<unsigned long long>& done, const A&... args) {
+  if (!allow_smem(reinterpret_cast<const void*>(kernel), smem, done)) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 // Tiled view of a 16-bit tensor: `dims` extents from the innermost out, strides in elements (of dims 1..), one box of
 // 64 elements x `rows`.  False: the layout cannot be loaded this way.
