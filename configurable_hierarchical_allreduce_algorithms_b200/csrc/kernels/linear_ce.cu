@@ -42,6 +42,7 @@ struct GemmArgs {
   const int* count;
   int N, V, v0, vn;          // rows of x at most; vocabulary, first column and width of the piece
   int D;
+  int a_rows;                // LSE and GRAD: rows of x that a tile loads (all 128, or all there are: the others' results go nowhere)
   int bn;                    // columns of a tile: a multiple of 32 (GRAD and BOTH: of 64)
   // LSE
   float2* part;
@@ -108,8 +109,8 @@ struct TilePlace {
 };
 
 // One persistent CTA per SM; warp 0 loads, warp 1 issues the products, warps 4 to 7 finish a tile (thread = row) while the
-// next one is summed in the other half of tensor memory.  Maps: gathered rows, W (LSE and GRAD: boxes of a tile's columns, else
-// of 64), and BOTH: G.
+// next one is summed in the other half of tensor memory.  Maps: gathered rows and W (LSE and GRAD: boxes of a tile's rows and
+// columns, else of 64), and BOTH: G.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256, 1)
 ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mg, const GemmArgs p) {
@@ -175,10 +176,9 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
         if (!(ok = bar_wait_warp(empty + 8 * s, ph ^ 1u, &fault))) break;
         const uint32_t bar = full + 8 * s, a = smem + s * STAGE, b = a + BM * BK * 2;
         if (one) {
-          bar_expect(bar, (BM + bn) * BK * 2);
+          bar_expect(bar, ((MODE == BOTH ? BM : p.a_rows) + bn) * BK * 2);
           if (MODE != BOTH) {
-#pragma unroll
-            for (int j = 0; j < BM / 64; ++j) load2(a + j * kBox, &mx, k * BK, q.m0 + 64 * j, bar);
+            load2(a, &mx, k * BK, q.m0, bar);
             load2(b, &mw, k * BK, p.v0 + q.n0, bar);
           } else if (q.w) {
 #pragma unroll
@@ -648,6 +648,9 @@ int tile_columns(long long rows_t, long long columns, int sms, int unit) {
   return best;
 }
 
+// With few rows the way from L2 to the SMs is the limit, and a tile's 128 rows of x would take a third of it.
+int rows_loaded(long long N) { return N < BM ? (int)up(N, 8) : BM; }
+
 // How the backward pass is cut for N rows: the width of a piece of the vocabulary (its G takes kPieceBytes at most, so that
 // much of it is still in L2 when it is read), and into how many shares the sums of dW and dx are split where there are too
 // few tiles for the SMs.
@@ -729,8 +732,8 @@ template <typename T>
 int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, const Bwd& b, const Plan& q, char* dx, char* dw, int sms,
              cudaStream_t stream) {
   const long long pad = up(N, BM);
-  CUtensorMap mx, mw, mt, mg;
-  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D) || !map2(&mt, dtype, w, D, V, D, q.bn_g) ||
+  CUtensorMap ma, mx, mw, mt, mg;
+  if (!map2(&ma, dtype, sv.xc, D, pad, D, rows_loaded(N)) || !map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D) || !map2(&mt, dtype, w, D, V, D, q.bn_g) ||
       !map2(&mg, dtype, b.g, q.width, pad, q.width)) return CHB_ERR_CUDA;
   GemmArgs p{};
   p.count = sv.head;
@@ -738,6 +741,7 @@ int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, con
   p.tgt = sv.tgt; p.lse2 = sv.lse2; p.gs = b.gs; p.g = b.g; p.ldg = q.width;
   p.slab_x = b.slab_x; p.slab_w = b.slab_w; p.split_x = q.split_x; p.split_w = q.split_w;
   p.rows_pad = (int)pad;
+  p.a_rows = rows_loaded(N);
   p.coef = b.coef; p.idx = sv.idx; p.dx = dx; p.dw = dw;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;
@@ -748,7 +752,7 @@ int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, con
     p.first = v0 == 0;
     p.last = v0 + q.width >= V;
     p.bn = q.bn_g;
-    if (gemm<T, GRAD>(mx, mt, mg, p, rows_t * ((p.vn + p.bn - 1) / p.bn), sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
+    if (gemm<T, GRAD>(ma, mt, mg, p, rows_t * ((p.vn + p.bn - 1) / p.bn), sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
     const long long tiles = (dw ? (p.vn + BM - 1) / BM * nt * q.split_w : 0) + (dx ? rows_t * nt * q.split_x : 0);
     p.bn = q.bn_d;
     if (gemm<T, BOTH>(mx, mw, mg, p, tiles, sms, stream) != cudaSuccess) return CHB_ERR_CUDA;
@@ -792,7 +796,7 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
   saved_layout(static_cast<char*>(saved), N, D, &sv);
   fwd_layout(static_cast<char*>(work), N, V, bn, &f);
   CUtensorMap mx, mw;
-  if (!map2(&mx, dtype, sv.xc, D, pad, D) || !map2(&mw, dtype, w, D, V, D, bn)) return CHB_ERR_CUDA;
+  if (!map2(&mx, dtype, sv.xc, D, pad, D, rows_loaded(n)) || !map2(&mw, dtype, w, D, V, D, bn)) return CHB_ERR_CUDA;
   float* const loss_rows = reduction == 0 ? loss : nullptr;
   const char* const xs = static_cast<const char*>(x);
   if (n <= kCountedRows) {
@@ -803,7 +807,7 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
   }
   GemmArgs p{};
   p.count = sv.head;
-  p.N = n; p.V = V; p.D = D; p.vn = V; p.bn = bn;
+  p.N = n; p.V = V; p.D = D; p.vn = V; p.bn = bn; p.a_rows = rows_loaded(n);
   p.part = f.part; p.tlogit = f.tlogit; p.tgt = sv.tgt; p.rows_pad = (int)pad;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;
