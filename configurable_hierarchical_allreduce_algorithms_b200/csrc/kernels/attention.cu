@@ -100,20 +100,38 @@ __device__ __forceinline__ void zero_rows(char* tile, int atoms, int from) {
 __device__ __forceinline__ uint64_t along(uint64_t tile, int k) { return tile + (uint64_t)((k >> 2) * (kAtom >> 4) + (k & 3) * 2); }
 __device__ __forceinline__ uint64_t across(uint64_t tile, int k) { return tile + (uint64_t)(k * 128); }
 
-// 32 columns of an accumulator row, times a factor, to 32 elements of a row of D (those below D)
-template <typename T>
-__device__ __forceinline__ void store_cols(char* row, int col, int D, const uint32_t* r, float f) {
+// A warp's 32 rows of DP / 2 columns of an accumulator, times a factor, to 16-bit rows in global memory: by way of shared memory
+// (32 * DP bytes of the warp's own, whose tiles are no longer read), so that a store covers whole rows and not one 16-byte
+// word of 32 rows (an epilogue at D = 128: 5000 -> 1000 clocks).  `rows`: how many of the 32 exist, `pitch`: bytes between rows.
+template <typename T, int DP>
+__device__ __forceinline__ void store_rows(uint32_t acc, float f, char* stage, char* out, long long pitch, int rows, int col0, int D) {
+  constexpr int kWords = DP / 16;      // 16-byte words of a row's share
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int c = 0; c < DP / 2; c += 32) {
+    uint32_t r[32];
+    __syncwarp();
+    ld32(acc + c, r);
+    wait_ld(r);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (col + 8 * q < D) {
+    for (int q = 0; q < 4; ++q) {
       uint4 o;
       o.x = pack2<T>(__uint_as_float(r[8 * q]) * f, __uint_as_float(r[8 * q + 1]) * f);
       o.y = pack2<T>(__uint_as_float(r[8 * q + 2]) * f, __uint_as_float(r[8 * q + 3]) * f);
       o.z = pack2<T>(__uint_as_float(r[8 * q + 4]) * f, __uint_as_float(r[8 * q + 5]) * f);
       o.w = pack2<T>(__uint_as_float(r[8 * q + 6]) * f, __uint_as_float(r[8 * q + 7]) * f);
-      *reinterpret_cast<uint4*>(row + (col + 8 * q) * 2) = o;
+      // (words of eight neighbouring rows in different banks)
+      reinterpret_cast<uint4*>(stage)[lane * kWords + ((c / 8 + q) ^ (lane * kWords / 8 & (kWords - 1)))] = o;
     }
   }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    const int row = i * (32 / kWords) + lane / kWords, word = lane % kWords;
+    const uint4 o = reinterpret_cast<const uint4*>(stage)[row * kWords + (word ^ (row * kWords / 8 & (kWords - 1)))];
+    if (row < rows && col0 + word * 8 < D) *reinterpret_cast<uint4*>(out + row * pitch + (col0 + word * 8) * 2) = o;
+  }
+  __syncwarp();
 }
 
 __device__ __forceinline__ void zero_out(char* base, long long first, int rows, int heads, int head, int D) {
@@ -158,11 +176,18 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
   const uint32_t qfull = bar0, kfull = bar0 + 16, kempty = bar0 + 32, vfull = bar0 + 48, vempty = bar0 + 64, sfull = bar0 + 80,
                  pfull = bar0 + 96, vready = bar0 + 112, sread = bar0 + 128, odone = bar0 + 144;      // (two of each)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 17) tmem_alloc(smem_u32(&tmem_), 512);
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, p.group, &work);
+  fence_before();
   __syncthreads();
+  fence_after();
   const Work w = work;
-  if (w.len == 0) return;
+  const uint32_t tmem = tmem_;
+  if (w.len == 0) {
+    if (warp == 17) tmem_free(tmem, 512);
+    return;
+  }
   const int kvh = blockIdx.x % p.kv_heads, nt = (w.len + TILE - 1) / TILE, total = nt * p.group;
   // long tiles first; tile 1 is the same one of the next head, or the one before
   int tile[2], head[2], n[2];
@@ -176,32 +201,21 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
   if (w.nothing) {
     for (int u = 0; u < 2; ++u)
       if (n[u]) zero_out(p.o, w.start + tile[u] * TILE, min(TILE, w.len - tile[u] * TILE), p.heads, head[u], p.D);
+    if (warp == 17) tmem_free(tmem, 512);
     return;
   }
   const bool ragged = n[0] * TILE > w.len;      // the last tile of keys reaches past the sequence
-  if (threadIdx.x == 0) {
-    fault.raised = 0;
-    fault.status = p.status;
-    const int tiles = n[1] ? 2 : 1;
-    for (int i = 0; i < 2; ++i) {
-      bar_init(qfull + 8 * i, 1);
-      bar_init(kfull + 8 * i, 1);
-      bar_init(kempty + 8 * i, tiles);
-      bar_init(vfull + 8 * i, 1);
-      bar_init(vempty + 8 * i, tiles + ragged);
-      bar_init(sfull + 8 * i, 1);
-      bar_init(pfull + 8 * i, 256);
-      bar_init(vready + 8 * i, 1);
-      bar_init(sread + 8 * i, 256);
-      bar_init(odone + 8 * i, 1);
+  if (warp == 0) {
+    if (lane == 31) {
+      fault.raised = 0;
+      fault.status = p.status;
     }
+    const int tiles = n[1] ? 2 : 1, kind = lane >> 1;      // (two of each, a lane a barrier)
+    const int count = kind == 2 ? tiles : kind == 4 ? tiles + ragged : kind == 6 || kind == 8 ? 256 : 1;
+    if (kind < 10) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
-  if (warp == 17) tmem_alloc(smem_u32(&tmem_), 512);
-  fence_before();
   __syncthreads();
-  fence_after();
-  const uint32_t tmem = tmem_;
   const uint32_t sq = smem, sk = smem + 2 * TB, sv = smem + 4 * TB;
 
   if (warp == 16) {
@@ -379,15 +393,9 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       const float sum = joint[u][0][r0] + joint[u][1][r0], f = 1.f / sum;
       const bool in = row < w.len;
       if (in && half == 0) p.lse[(long long)head[u] * p.T + w.start + row] = ref + log2f(sum);
-      char* out = p.o + ((long long)(w.start + row) * p.heads + head[u]) * p.D * 2;
-#pragma unroll 1
-      for (int c = 0; c < DP / 2; c += 32) {
-        uint32_t r[32];
-        __syncwarp();
-        ld32(to + c, r);
-        wait_ld(r);
-        if (in) store_cols<T>(out, half * (DP / 2) + c, p.D, r, f);
-      }
+      const int first = tile[u] * TILE + (warp & 3) * 32;      // the warp's first row
+      store_rows<T, DP>(to, f, smem_p + u * TB + (warp & 7) * 32 * DP, p.o + ((long long)(w.start + first) * p.heads + head[u]) * p.D * 2,
+                        (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
     }
   }
   fence_before();
@@ -437,33 +445,37 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   const uint32_t qfull = bar0, kfull = bar0 + 8, kempty = bar0 + 32, vfull = bar0 + 56, vempty = bar0 + 72, sfull = bar0 + 88,
                  dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.heads, 0, &work);
+  fence_before();
   __syncthreads();
+  fence_after();
   const Work w = work;
-  if (w.len == 0) return;
+  const uint32_t tmem = tmem_;
+  if (w.len == 0) {
+    if (warp == 9) tmem_free(tmem, 512);
+    return;
+  }
   const int head = blockIdx.x % p.heads, kvh = head / p.group, nt = (w.len + TILE - 1) / TILE;
   const int tile = nt - 1 - w.unit, n = tile + 1;
   if (w.nothing) {
     zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D);
+    if (warp == 9) tmem_free(tmem, 512);
     return;
   }
   const bool ragged = n * TILE > w.len;
-  if (threadIdx.x == 0) {
-    fault.raised = 0;
-    fault.status = p.status;
-    for (int i = 0; i < 18; ++i) bar_init(bar0 + 8 * i, 1);
-    bar_init(qfull, 2);      // Q and dO
-    for (int i = 0; i < 3; ++i) bar_init(kempty + 8 * i, 1 + ragged);
-    for (int i = 0; i < 2; ++i) bar_init(vempty + 8 * i, 1 + ragged);
-    bar_init(dsfull, 256);
+  if (warp == 0) {
+    if (lane == 31) {
+      fault.raised = 0;
+      fault.status = p.status;
+    }
+    // (a lane a barrier: Q and dO arrive at one; the slots of K and V are freed by the zeros' warp too where that has them)
+    const int count = lane == 0 ? 2 : (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 1 + ragged : lane == 14 ? 256 : 1;
+    if (lane < 18) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
-  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
-  fence_before();
   __syncthreads();
-  fence_after();
-  const uint32_t tmem = tmem_;
   const uint32_t sq = smem, sdo = smem + TB, sk = smem + 2 * TB, sv = smem + 5 * TB;
   const uint32_t tdp = tmem + 2 * TILE, tdq = tmem + 3 * TILE;
 
@@ -618,15 +630,9 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
     }
     if (ok && bar_wait_warp(done, 0, &fault)) {
       fence_after();
-      char* out = p.dq + ((long long)(w.start + row) * p.heads + head) * p.D * 2;
-#pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
-        uint32_t r[32];
-        __syncwarp();
-        ld32(tdq + c + lanes, r);
-        wait_ld(r);
-        if (in) store_cols<T>(out, c, p.D, r, p.scale);
-      }
+      const int first = tile * TILE + (warp & 3) * 32;
+      store_rows<T, DP>(tdq + half * (DP / 2) + lanes, p.scale, smem_p + warp * 32 * DP,
+                        p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2, (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
     }
   }
   fence_before();
@@ -652,43 +658,40 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
                  dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
   dependent_launch();
   if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, 0, &work);
+  fence_before();
   __syncthreads();
+  fence_after();
   const Work w = work;
-  if (w.len == 0) return;
+  const uint32_t tmem = tmem_;
+  if (w.len == 0) {
+    if (warp == 9) tmem_free(tmem, 512);
+    return;
+  }
   const int kvh = blockIdx.x % p.kv_heads, nt = (w.len + TILE - 1) / TILE;
   const int tile = w.unit, per_head = nt - tile, n = per_head * p.group;
   if (w.nothing) {
     const int rows_here = min(TILE, w.len - tile * TILE);
     zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
     zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
+    if (warp == 9) tmem_free(tmem, 512);
     return;
   }
   const bool ragged = nt * TILE > w.len;      // every head's last tile of queries reaches past the sequence
-  if (threadIdx.x == 0) {
-    fault.raised = 0;
-    fault.status = p.status;
-    if (!fits(smem_p + 7 * TB, smem_raw)) {
-      fault.raised = 1;
-      atomicExch(p.status, 1u);
+  if (warp == 0) {
+    if (lane == 31) {
+      fault.raised = !fits(smem_p + 7 * TB, smem_raw);
+      fault.status = p.status;
+      if (fault.raised) atomicExch(p.status, 1u);
     }
-    for (int i = 0; i < 18; ++i) bar_init(bar0 + 8 * i, 1);
-    bar_init(own, 2);        // K and V
-    for (int i = 0; i < 3; ++i) bar_init(qempty + 8 * i, 1 + ragged);
-    for (int i = 0; i < 2; ++i) {
-      bar_init(gfull + 8 * i, 2);      // the load of dO, and lse and D
-      bar_init(gempty + 8 * i, 1 + ragged);
-    }
-    bar_init(pfull, 256);
-    bar_init(dsfull, 256);
+    // (a lane a barrier: K and V arrive at one, dO with lse and D at another; slots are freed by the zeros' warp too where that has them)
+    const int count = lane == 0 || lane == 7 || lane == 8 ? 2 : (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 1 + ragged : lane == 13 || lane == 14 ? 256 : 1;
+    if (lane < 18) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
-  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
-  fence_before();
   __syncthreads();
-  fence_after();
-  const uint32_t tmem = tmem_;
   if (fault.raised) {
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
@@ -805,7 +808,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       }
     }
   } else {
-    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane, row = tile * TILE + r0;
+    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + half * 64 + lanes, tp = tdp + half * 64 + lanes;
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
@@ -876,20 +879,10 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     }
     if (ok && bar_wait_warp(done, 0, &fault)) {
       fence_after();
-      const bool in = row < w.len;
-      const long long at = ((long long)(w.start + row) * p.kv_heads + kvh) * p.D * 2;
-#pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
-        uint32_t r[32];
-        __syncwarp();
-        ld32(tdv + c + lanes, r);
-        wait_ld(r);
-        if (in) store_cols<T>(p.dv + at, c, p.D, r, 1.f);
-        __syncwarp();
-        ld32(tdk + c + lanes, r);
-        wait_ld(r);
-        if (in) store_cols<T>(p.dk + at, c, p.D, r, p.scale);
-      }
+      const int first = tile * TILE + (warp & 3) * 32;
+      const long long at = ((long long)(w.start + first) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
+      store_rows<T, DP>(tdv + half * (DP / 2) + lanes, 1.f, smem_p + warp * 32 * DP, p.dv + at, pitch, w.len - first, half * (DP / 2), p.D);
+      store_rows<T, DP>(tdk + half * (DP / 2) + lanes, p.scale, smem_p + TB + warp * 32 * DP, p.dk + at, pitch, w.len - first, half * (DP / 2), p.D);
     }
   }
   fence_before();
