@@ -8,15 +8,19 @@
 // scores that they came from, and never to shared or global memory.  Every operand tile is loaded once and serves as K-major
 // operand of a score product and as MN-major operand of an output product.  Three kernels:
 //
-//   forward  a CTA has two tiles of queries (neighbouring in (tile, head of the group) order, so that two heads share the
-//            keys and values where there are groups): the products of one run while the other's exponentials are taken.
+//   forward  a CTA has two tiles of queries at a time (neighbouring in (tile, head of the group) order, so that two heads share
+//            the keys and values where there are groups): the products of one run while the other's exponentials are taken.
 //            One pass with a running maximum; the sums are rescaled only when a maximum grows by more than 2^8.
 //   dq       a CTA has a tile of queries and walks its keys; also writes D.
 //   dkv      a CTA has a tile of keys of one key head and walks the queries of all heads of the group that see it, so
-//            gradients of shared heads are summed in the accumulators, in one order: no atomics anywhere.
+//            gradients of shared heads are summed in the accumulators, in one order: no atomics on results anywhere.
 //
-// Sequences: the rows [cu[s], cu[s+1]); a CTA finds its own from the bounds, so lengths stay on the device.  Rows outside all
-// sequences get zeros.  A tile that reaches past its sequence holds the next one's rows: those are overwritten with zeros
+// Each has one CTA an SM that takes one piece of work after the other: the loads and first products of the next run under the
+// end of this one (8 x 1024 tokens, 16 heads of 64, forward: a CTA for each piece 53 us).  A first small kernel lists the
+// pieces, the longest first, and CTAs take them in turns forth and back, so that all end at about the same time.
+//
+// Sequences: the rows [cu[s], cu[s+1]); the list is made from the bounds on the device, so no length is needed on the host.
+// Rows outside all sequences get zeros.  A tile that reaches past its sequence holds the next one's rows: those are overwritten with zeros
 // where they would be summed over (a product 0 * infinity would carry them across).
 //
 // P and dS are rounded to the operands' type (as the tensor cores need them); maxima, sums, lse and D are fp32.
@@ -33,8 +37,9 @@ constexpr int TILE = 128;
 constexpr int kAtom = TILE * 128;        // bytes of a tile's 64 elements: 128 rows of 128 bytes
 
 struct AttnArgs {
-  const int* cu;          // null: one sequence
-  int seqs, T, heads, kv_heads, group, D;
+  const int4* list;       // pieces of work: pairs (forward) or tiles
+  const int* listed;      // how many
+  int T, heads, kv_heads, group, D;
   float scale, scale_log2;
   char* o;                // [T, heads, D] (written by forward, read by dq)
   float* lse;             // [heads, T], in units of log2
@@ -45,46 +50,102 @@ struct AttnArgs {
   unsigned* status;
 };
 
-struct Work { int start, len, unit, nothing; };      // nothing: rows outside all sequences
+// Piece number `unit` of the rows [start, start + len): a tile, or a pair of (tile, head of the group), counted so that cost
+// falls with the number; nothing: rows outside all sequences.
+struct Work { int start, len, unit, nothing; };
 
-// The sequence of unit number `unit`, by one warp: prefix sums over the sequences' numbers of units (tiles, or pairs of
-// (tile, head) where `group` is not 0).
-__device__ __forceinline__ void find_work(const AttnArgs& p, int unit, int group, Work* out) {
-  const int lane = threadIdx.x & 31;
-  const int n = p.cu ? p.seqs + 2 : 1;
-  int before = 0;
-  for (int base = 0; base < n; base += 32) {
-    const int s = base + lane;
-    int a = 0, b = 0;
-    if (s < n) {
-      if (p.cu) {
-        a = s == 0 ? 0 : min(max(p.cu[s - 1], 0), p.T);
-        b = s == n - 1 ? p.T : min(max(p.cu[s], 0), p.T);
-      } else {
-        b = p.T;
-      }
+// The pieces that this CTA takes: of the list times the heads, a row of them at a time, forth and back.  Little of it stays in
+// registers: the list is read again where a warp needs a piece's place once more.
+struct Walk {
+  unsigned row = ~0u;
+  __device__ __forceinline__ unsigned at() const { return row * gridDim.x + (row & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }      // number of the piece
+  __device__ __forceinline__ bool next(int total) {
+    for (++row; row * gridDim.x < (unsigned)total; ++row)
+      if (at() < (unsigned)total) return true;
+    return false;
+  }
+  __device__ __forceinline__ Work work(const AttnArgs& p, int heads) const {
+    const int4 e = p.list[at() / heads];
+    return Work{e.x, e.y, e.z, e.w};
+  }
+  __device__ __forceinline__ int head(int heads) const { return (int)(at() % heads); }
+};
+
+// Lists the pieces of all sequences by falling cost (tiles of keys to walk), by counting: one CTA.  Up to 1024 costs are kept
+// apart, more share a place.  plan: [0] pairs, [1] tiles, then from the fourth int4 on both lists, `most[]` entries each.
+// Sequences outside [0, T] or overlapping are clamped; what does not fit the lists is left out.
+constexpr int kPlanHead = 4, kCosts = 1024;
+__global__ void __launch_bounds__(1024) attn_plan(const int* cu, int seqs, int T, int group, int most_pairs, int most_tiles, int4* plan) {
+  __shared__ int at[2][kCosts], warps[2][32], longest_;
+  dependent_launch();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = cu ? seqs + 2 : 1;      // (with the rows before the first and behind the last)
+  const auto segment = [&](int s, int& a) {
+    int b = T;
+    a = 0;
+    if (cu) {
+      a = s == 0 ? 0 : min(max(cu[s - 1], 0), T);
+      b = s == n - 1 ? T : min(max(cu[s], 0), T);
     }
-    const int len = max(b - a, 0), tiles = (len + TILE - 1) / TILE;
-    const int units = group ? (tiles * group + 1) / 2 : tiles;
-    int inc = units;
+    return max(b - a, 0);
+  };
+  at[0][tid] = at[1][tid] = 0;
+  if (tid == 0) longest_ = 1;
+  __syncthreads();
+  for (int s = tid; s < n; s += 1024) {
+    int a;
+    const int len = segment(s, a);
+    if (len > TILE) atomicMax(&longest_, (len + TILE - 1) / TILE);
+  }
+  __syncthreads();
+  const int longest = longest_;
+  const auto place = [&](int cost) { return longest <= kCosts ? longest - cost : (int)((long long)(longest - cost) * kCosts / longest); };
+  // few sequences: a warp walks the pieces of one; many: a thread
+  const auto walk = [&](auto&& each) {
+    const bool few = n <= 64;
+    for (int s = few ? warp : tid; s < n; s += few ? 32 : 1024) {
+      int a;
+      const int len = segment(s, a), tiles = (len + TILE - 1) / TILE, nothing = cu && (s == 0 || s == n - 1);
+      for (int u = few ? lane : 0; u < tiles; u += few ? 32 : 1) each(1, a, len, u, nothing, nothing ? 1 : tiles - u);
+      for (int u = few ? lane : 0; u < (tiles * group + 1) / 2; u += few ? 32 : 1) each(0, a, len, u, nothing, nothing ? 1 : tiles - 2 * u / group);
+    }
+  };
+  walk([&](int l, int, int, int, int, int cost) { atomicAdd(&at[l][place(cost)], 1); });
+  __syncthreads();
+  int inc[2];
+#pragma unroll
+  for (int l = 0; l < 2; ++l) {
+    inc[l] = at[l][tid];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += v;
+      const int v = __shfl_up_sync(0xffffffffu, inc[l], d);
+      if (lane >= d) inc[l] += v;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, unit < before + inc);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        out->start = a;
-        out->len = len;
-        out->unit = unit - before - (inc - units);
-        out->nothing = p.cu && (s == 0 || s == n - 1);
-      }
-      return;
-    }
-    before += __shfl_sync(0xffffffffu, inc, 31);
+    if (lane == 31) warps[l][warp] = inc[l];
   }
-  if (lane == 0) out->len = 0;
+  __syncthreads();
+  if (warp < 2) {
+    int v = warps[warp][lane];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += u;
+    }
+    warps[warp][lane] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int l = 0; l < 2; ++l) {
+    const int before = warp ? warps[l][warp - 1] : 0;
+    at[l][tid] = before + inc[l] - at[l][tid];
+    if (tid == 1023) reinterpret_cast<int*>(plan)[l] = min(before + inc[l], l ? most_tiles : most_pairs);
+  }
+  __syncthreads();
+  walk([&](int l, int a, int len, int u, int nothing, int cost) {
+    // (pieces of the same cost in any order: who works on a piece has no influence on its result)
+    const int i = atomicAdd(&at[l][place(cost)], 1);
+    if (i < (l ? most_tiles : most_pairs)) plan[kPlanHead + (l ? most_pairs : 0) + i] = make_int4(a, len, u, nothing);
+  });
 }
 
 // rows [from, 128) of a tile of `atoms` x 64 elements become zero (by one warp)
@@ -100,15 +161,14 @@ __device__ __forceinline__ void zero_rows(char* tile, int atoms, int from) {
 __device__ __forceinline__ uint64_t along(uint64_t tile, int k) { return tile + (uint64_t)((k >> 2) * (kAtom >> 4) + (k & 3) * 2); }
 __device__ __forceinline__ uint64_t across(uint64_t tile, int k) { return tile + (uint64_t)(k * 128); }
 
-// A warp's 32 rows of DP / 2 columns of an accumulator, times a factor, to 16-bit rows in global memory: by way of shared memory
-// (32 * DP bytes of the warp's own, whose tiles are no longer read), so that a store covers whole rows and not one 16-byte
-// word of 32 rows (an epilogue at D = 128: 5000 -> 1000 clocks).  `rows`: how many of the 32 exist, `pitch`: bytes between rows.
-template <typename T, int DP>
-__device__ __forceinline__ void store_rows(uint32_t acc, float f, char* stage, char* out, long long pitch, int rows, int col0, int D) {
-  constexpr int kWords = DP / 16;      // 16-byte words of a row's share
+// A warp's 32 rows of `cols` columns of an accumulator, times a factor, to 16-bit rows in global memory: by way of 2 KB of shared
+// memory of the warp's own, so that a store covers 64 bytes of eight rows and not one 16-byte word of 32 (an epilogue at D = 128:
+// 5000 -> 1400 clocks).  `rows`: how many of the 32 exist, `pitch`: bytes between rows.
+template <typename T>
+__device__ __forceinline__ void store_rows(uint32_t acc, int cols, float f, char* stage, char* out, long long pitch, int rows, int col0, int D) {
   const int lane = threadIdx.x & 31;
 #pragma unroll 1
-  for (int c = 0; c < DP / 2; c += 32) {
+  for (int c = 0; c < cols; c += 32) {
     uint32_t r[32];
     __syncwarp();
     ld32(acc + c, r);
@@ -120,23 +180,24 @@ __device__ __forceinline__ void store_rows(uint32_t acc, float f, char* stage, c
       o.y = pack2<T>(__uint_as_float(r[8 * q + 2]) * f, __uint_as_float(r[8 * q + 3]) * f);
       o.z = pack2<T>(__uint_as_float(r[8 * q + 4]) * f, __uint_as_float(r[8 * q + 5]) * f);
       o.w = pack2<T>(__uint_as_float(r[8 * q + 6]) * f, __uint_as_float(r[8 * q + 7]) * f);
-      // (words of eight neighbouring rows in different banks)
-      reinterpret_cast<uint4*>(stage)[lane * kWords + ((c / 8 + q) ^ (lane * kWords / 8 & (kWords - 1)))] = o;
+      reinterpret_cast<uint4*>(stage)[lane * 4 + (q ^ (lane / 2 & 3))] = o;      // (words of neighbouring rows in different banks)
     }
-  }
-  __syncwarp();
+    __syncwarp();
+    const int col = col0 + c + lane % 4 * 8;
 #pragma unroll
-  for (int i = 0; i < kWords; ++i) {
-    const int row = i * (32 / kWords) + lane / kWords, word = lane % kWords;
-    const uint4 o = reinterpret_cast<const uint4*>(stage)[row * kWords + (word ^ (row * kWords / 8 & (kWords - 1)))];
-    if (row < rows && col0 + word * 8 < D) *reinterpret_cast<uint4*>(out + row * pitch + (col0 + word * 8) * 2) = o;
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + lane / 4;
+      const uint4 o = reinterpret_cast<const uint4*>(stage)[row * 4 + ((lane % 4) ^ (row / 2 & 3))];
+      if (row < rows && col < D) *reinterpret_cast<uint4*>(out + row * pitch + col * 2) = o;
+    }
   }
   __syncwarp();
 }
 
-__device__ __forceinline__ void zero_out(char* base, long long first, int rows, int heads, int head, int D) {
+// (by the first `threads` threads of the CTA)
+__device__ __forceinline__ void zero_out(char* base, long long first, int rows, int heads, int head, int D, int threads) {
   const int words = D / 8;
-  for (int i = threadIdx.x; i < rows * words; i += blockDim.x)
+  for (int i = threadIdx.x; i < rows * words; i += threads)
     *reinterpret_cast<uint4*>(base + (((first + i / words) * heads + head) * D + i % words * 8) * 2) = make_uint4(0u, 0u, 0u, 0u);
 }
 
@@ -158,6 +219,16 @@ __device__ __forceinline__ bool any_of_tile(int tile, bool want) {
 }
 __device__ __forceinline__ void sync_tile(int tile) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(1 + tile) : "memory"); }
 
+// What a forward CTA makes of a piece: two of the sequence's (tile, head of the group), the second the same tile of the next head
+// or the tile before.  (Members of one of the two are computed when asked for; arrays would go to local memory.)
+struct Pair {
+  int nt, unit, group, head0, len;
+  __device__ __forceinline__ Pair(const Work& w, int kvh, int group_) : nt((w.len + TILE - 1) / TILE), unit(w.unit), group(group_), head0(kvh * group_), len(w.len) {}
+  __device__ __forceinline__ int n(int u) const { return max(nt - (2 * unit + u) / group, 0); }      // tiles of keys; the tile is the last
+  __device__ __forceinline__ int head(int u) const { return head0 + (2 * unit + u) % group; }
+  __device__ __forceinline__ bool ragged() const { return n(0) * TILE > len; }      // the last tile of keys reaches past the sequence
+};
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -166,57 +237,33 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
   // At DP = 64 tensor memory has room for P beside the scores, and the next scores are made as soon as these are read.
   constexpr bool kApart = DP == 64;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[20];
-  __shared__ float joint[2][2][TILE];
+  __shared__ __align__(8) unsigned long long bars[22];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
-  __shared__ Work work;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
-  const uint32_t qfull = bar0, kfull = bar0 + 16, kempty = bar0 + 32, vfull = bar0 + 48, vempty = bar0 + 64, sfull = bar0 + 80,
-                 pfull = bar0 + 96, vready = bar0 + 112, sread = bar0 + 128, odone = bar0 + 144;      // (two of each)
+  // (two of each.  Turns go on counting from one piece of work to the next: a barrier's phase is its count of turns)
+  const uint32_t qfull = bar0, qempty = bar0 + 16, kfull = bar0 + 32, kempty = bar0 + 48, vfull = bar0 + 64, vempty = bar0 + 80, sfull = bar0 + 96,
+                 pfull = bar0 + 112, vready = bar0 + 128, sread = bar0 + 144, odone = bar0 + 160;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 17) tmem_alloc(smem_u32(&tmem_), 512);
-  dependent_launch();
-  if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, p.group, &work);
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const Work w = work;
-  const uint32_t tmem = tmem_;
-  if (w.len == 0) {
-    if (warp == 17) tmem_free(tmem, 512);
-    return;
-  }
-  const int kvh = blockIdx.x % p.kv_heads, nt = (w.len + TILE - 1) / TILE, total = nt * p.group;
-  // long tiles first; tile 1 is the same one of the next head, or the one before
-  int tile[2], head[2], n[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int x = 2 * w.unit + u;
-    tile[u] = x < total ? nt - 1 - x / p.group : -1;
-    head[u] = kvh * p.group + x % p.group;
-    n[u] = tile[u] + 1;
-  }
-  if (w.nothing) {
-    for (int u = 0; u < 2; ++u)
-      if (n[u]) zero_out(p.o, w.start + tile[u] * TILE, min(TILE, w.len - tile[u] * TILE), p.heads, head[u], p.D);
-    if (warp == 17) tmem_free(tmem, 512);
-    return;
-  }
-  const bool ragged = n[0] * TILE > w.len;      // the last tile of keys reaches past the sequence
   if (warp == 0) {
     if (lane == 31) {
       fault.raised = 0;
       fault.status = p.status;
     }
-    const int tiles = n[1] ? 2 : 1, kind = lane >> 1;      // (two of each, a lane a barrier)
-    const int count = kind == 2 ? tiles : kind == 4 ? tiles + ragged : kind == 6 || kind == 8 ? 256 : 1;
-    if (kind < 10) bar_init(bar0 + 8 * lane, count);
+    const int kind = lane >> 1;      // (a lane a barrier)
+    if (kind < 11) bar_init(bar0 + 8 * lane, kind == 3 ? 2 : kind == 5 ? 3 : kind == 7 || kind == 9 ? 256 : 1);
     bar_init_done();
   }
+  fence_before();
   __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_;
+  dependent_launch();
+  const int total = *(volatile const int*)p.listed * p.kv_heads;
   const uint32_t sq = smem, sk = smem + 2 * TB, sv = smem + 4 * TB;
+  char* const stage = smem_p + 6 * TB;      // 2 KB a softmax warp
 
   if (warp == 16) {
     const bool one = elect();
@@ -228,63 +275,96 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       }
       __syncwarp();
     };
-    load_tile(sq, &mq, w.start + tile[0] * TILE, head[0], qfull);
-    for (int i = 0; i < n[0]; ++i) {
-      const int s = i & 1;
-      const unsigned ph = ((i >> 1) & 1) ^ 1u;
-      if (!bar_wait_warp(kempty + 8 * s, ph, &fault)) break;
-      load_tile(sk + s * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s);
-      if (i == 0 && n[1]) load_tile(sq + TB, &mq, w.start + tile[1] * TILE, head[1], qfull + 8);
-      if (!bar_wait_warp(vempty + 8 * s, ph, &fault)) break;
-      load_tile(sv + s * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s);
+    bool ok = true;
+    int g = 0, qn0 = 0, qn1 = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int kvh = it.head(p.kv_heads);
+      if (w.nothing) continue;
+      const Pair x(w, kvh, p.group);
+      const int n0 = x.n(0), n1 = x.n(1);
+      if (!(ok = bar_wait_warp(qempty, (qn0++ & 1) ^ 1, &fault))) break;
+      load_tile(sq, &mq, w.start + (n0 - 1) * TILE, x.head(0), qfull);
+      for (int i = 0; i < n0; ++i, ++g) {
+        const int s = g & 1;
+        const unsigned ph = ((g >> 1) & 1) ^ 1u;
+        if (!(ok = bar_wait_warp(kempty + 8 * s, ph, &fault))) break;
+        load_tile(sk + s * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s);
+        if (i == 0 && n1) {
+          if (!(ok = bar_wait_warp(qempty + 8, (qn1++ & 1) ^ 1, &fault))) break;
+          load_tile(sq + TB, &mq, w.start + (n1 - 1) * TILE, x.head(1), qfull + 8);
+        }
+        if (!(ok = bar_wait_warp(vempty + 8 * s, ph, &fault))) break;
+        load_tile(sv + s * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s);
+      }
     }
   } else if (warp == 19) {
-    // where the last tile is ragged every tile of values goes through this warp's hands (it keeps its place in the ring so)
-    for (int i = 0; i < n[0] && ragged; ++i) {
-      const int s = i & 1;
-      if (!bar_wait_warp(vfull + 8 * s, (i >> 1) & 1, &fault)) break;
-      if (i == n[0] - 1) zero_rows(smem_p + 4 * TB + s * TB, ATOMS, w.len - i * TILE);
-      if (lane == 0) {
-        bar_arrive(vready + 8 * s);
-        bar_arrive(vempty + 8 * s);
+    // every tile of values goes through this warp's hands, which overwrites the rows behind the sequence (it keeps its place in
+    // the ring so); only pieces with such rows wait for it
+    bool ok = true;
+    int g = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int kvh = it.head(p.kv_heads);
+      if (w.nothing) continue;
+      const Pair x(w, kvh, p.group);
+      const int n0 = x.n(0);
+      const bool ragged = x.ragged();
+      for (int i = 0; i < n0; ++i, ++g) {
+        const int s = g & 1;
+        if (!(ok = bar_wait_warp(vfull + 8 * s, (g >> 1) & 1, &fault))) break;
+        if (ragged && i == n0 - 1) zero_rows(smem_p + 4 * TB + s * TB, ATOMS, w.len - i * TILE);
+        if (lane == 0) {
+          bar_arrive(vready + 8 * s);
+          bar_arrive(vempty + 8 * s);
+        }
       }
     }
   } else if (warp >= 17) {
-    const int u = warp - 17, nu = n[u];
-    if (nu) {
-      const bool one = elect();
-      const int ksteps = (p.D + 15) / 16;
-      const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
-      const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
-      const uint32_t ts = tmem + u * TILE, to = tmem + 2 * TILE + u * DP, tp = kApart ? tmem + 3 * TILE + u * 64 : ts,
-                     values = ragged ? vready : vfull;
-      constexpr int kHalf = kApart ? 32 : 64;      // columns from one half of P to the other
-      const uint64_t a = operand(sq + u * TB), k0 = operand(sk), v0 = operand(sv, kAtom);
-      const auto scores = [&](int s) {
-        const uint64_t b = k0 + (uint64_t)(s * (TB >> 4));
-        if (one) {
+    const int u = warp - 17, ksteps = (p.D + 15) / 16;
+    const bool one = elect();
+    const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
+    const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
+    const uint32_t ts = tmem + u * TILE, to = tmem + 2 * TILE + u * DP, tp = kApart ? tmem + 3 * TILE + u * 64 : ts;
+    constexpr int kHalf = kApart ? 32 : 64;      // columns from one half of P to the other
+    const uint64_t a = operand(sq + u * TB), k0 = operand(sk), v0 = operand(sv, kAtom);
+    const auto scores = [&](int s, bool last) {
+      const uint64_t b = k0 + (uint64_t)(s * (TB >> 4));
+      if (one) {
 #pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            if (k < ksteps) mma_ss(ts, along(a, k), along(b, k), dscore, k > 0);
-          commit(sfull + 8 * u);
-          commit(kempty + 8 * s);
-        }
-        __syncwarp();
-      };
-      bool ok = bar_wait_warp(qfull + 8 * u, 0, &fault) && bar_wait_warp(kfull, 0, &fault);
-      if (ok) scores(0);
+        for (int k = 0; k < DP / 16; ++k)
+          if (k < ksteps) mma_ss(ts, along(a, k), along(b, k), dscore, k > 0);
+        commit(sfull + 8 * u);
+        commit(kempty + 8 * s);
+        if (last) commit(qempty + 8 * u);
+      }
+      __syncwarp();
+    };
+    bool ok = true;
+    int g = 0, t = 0, qn = 0;      // tiles of keys, own turns, own pieces
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int kvh = it.head(p.kv_heads);
+      if (w.nothing) continue;
+      const Pair x(w, kvh, p.group);
+      const int n0 = x.n(0), nu = x.n(u);
+      const uint32_t values = x.ragged() ? vready : vfull;
+      if (nu) {
+        if (!(ok = bar_wait_warp(qfull + 8 * u, qn++ & 1, &fault) && bar_wait_warp(kfull + 8 * (g & 1), (g >> 1) & 1, &fault))) break;
+        scores(g & 1, nu == 1);
+      }
 #pragma unroll 1
-      for (int i = 0; i < nu && ok; ++i) {
-        const int s = i & 1;
+      for (int i = 0; i < nu; ++i, ++g, ++t) {
+        const int s = g & 1;
         const uint64_t b = v0 + (uint64_t)(s * (TB >> 4));
-        if (i + 1 < nu && !(ok = bar_wait_warp(kfull + 8 * (s ^ 1), ((i + 1) >> 1) & 1, &fault))) break;
+        if (i + 1 < nu && !(ok = bar_wait_warp(kfull + 8 * (s ^ 1), ((g + 1) >> 1) & 1, &fault))) break;
         if (kApart && i + 1 < nu) {
-          if (!(ok = bar_wait_warp(sread + 8 * u, i & 1, &fault))) break;
+          if (!(ok = bar_wait_warp(sread + 8 * u, t & 1, &fault))) break;
           fence_after();
-          scores(s ^ 1);
+          scores(s ^ 1, i + 2 == nu);
         }
-        if (!(ok = bar_wait_warp(values + 8 * s, (i >> 1) & 1, &fault))) break;
-        if (!(ok = bar_wait_warp(pfull + 8 * u, i & 1, &fault))) break;
+        if (!(ok = bar_wait_warp(values + 8 * s, (g >> 1) & 1, &fault))) break;
+        if (!(ok = bar_wait_warp(pfull + 8 * u, t & 1, &fault))) break;
         fence_after();
         if (one) {
 #pragma unroll
@@ -293,109 +373,128 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
         }
         __syncwarp();
         // the next scores go over P, behind the products that read it
-        if (!kApart && i + 1 < nu) scores(s ^ 1);
+        if (!kApart && i + 1 < nu) scores(s ^ 1, i + 2 == nu);
         if (one) commit(vempty + 8 * s);
         __syncwarp();
       }
-      if (ok && nu < n[0] && bar_wait_warp(kfull + 8 * (nu & 1), (nu >> 1) & 1, &fault)) {
-        // tile 1 ends one turn before tile 0: its last arrivals
-        if (one) bar_arrive(kempty + 8 * (nu & 1));
-        if (bar_wait_warp(vfull + 8 * (nu & 1), (nu >> 1) & 1, &fault) && one) bar_arrive(vempty + 8 * (nu & 1));
+      // tiles that only tile 0 sees: this one's arrivals
+      for (int i = nu; i < n0 && ok; ++i, ++g) {
+        const int s = g & 1;
+        if (!(ok = bar_wait_warp(kfull + 8 * s, (g >> 1) & 1, &fault))) break;
+        if (one) bar_arrive(kempty + 8 * s);
+        if (!(ok = bar_wait_warp(vfull + 8 * s, (g >> 1) & 1, &fault))) break;
+        if (one) bar_arrive(vempty + 8 * s);
+        __syncwarp();
       }
     }
   } else {
-    const int u = warp >> 3, half = (warp >> 2) & 1, nu = n[u], r0 = (warp & 3) * 32 + lane;
+    const int u = warp >> 3, half = (warp >> 2) & 1, r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + u * TILE + half * 64 + lanes, tp = kApart ? tmem + 3 * TILE + u * 64 + half * 32 + lanes : ts,
                    to = tmem + 2 * TILE + u * DP + half * (DP / 2) + lanes;
-    const int row = tile[u] * TILE + r0;
+    float* const joint = reinterpret_cast<float*>(stage + u * 8 * 2048);      // [half][row]; the outputs' way later
     const float sl = p.scale_log2;
     const uint64_t sl2 = pair(sl, sl);
-    float ref = 0.f;                       // the maximum that the sums are relative to, times scale log2 e
-    uint64_t sum2[2] = {0ull, 0ull};       // (two zeros each)
-    // The warps of a tile meet at barriers that cannot give up, so none of them leaves the loop: once a wait ran out all waits
-    // end at once, and the turns that are left go over whatever the scores hold.
-#pragma unroll 1
-    for (int i = 0; i < nu; ++i) {
-      bar_wait_warp(sfull + 8 * u, i & 1, &fault);
-      fence_after();
-      uint32_t r[64];
-      ld32(ts, r);
-      ld32(ts + 32, r + 32);
-      wait_ld(r);
-      if (kApart) {
-        fence_before();
-        bar_arrive(sread + 8 * u);
+    unsigned turn = 0, piece = 0;      // parities of the turns and of the pieces so far
+    for (Walk it; it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const Pair x(w, it.head(p.kv_heads), p.group);
+      if (w.nothing) {
+        for (int v = 0; v < 2; ++v)
+          if (x.n(v)) zero_out(p.o, w.start + (x.n(v) - 1) * TILE, min(TILE, w.len - (x.n(v) - 1) * TILE), p.heads, x.head(v), p.D, 512);
+        continue;
       }
-      if (i == nu - 1) {
-        const int last = r0 - half * 64;
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > last) r[c] = __float_as_uint(-INFINITY);
-      }
-      float m4[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-#pragma unroll
-      for (int c = 4; c < 32; ++c) m4[c & 3] = max3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-      const float top = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * sl;
-      const bool grows = any_of_tile(u, i == 0 || top > ref + 8.f);
-      if (kApart && i > 0) bar_wait_warp(odone + 8 * u, (i - 1) & 1, &fault);
-      if (grows) {
-        joint[u][half][r0] = top;
-        sync_tile(u);
-        const float both = fmaxf(top, joint[u][half ^ 1][r0]);
-        sync_tile(u);
-        if (i == 0) {
-          ref = both == -INFINITY ? 0.f : both;
-        } else {
-          // (the output rests: the products of the tile before are done, as the scores' commit came behind them or odone says so)
-          fence_after();
-          const float next = fmaxf(ref, both), f = ex2(ref - next);
-          const uint64_t f2 = pair(f, f);
-          ref = next;
-          sum2[0] = mul2(sum2[0], f2);
-          sum2[1] = mul2(sum2[1], f2);
+      const int nu = x.n(u);
+      if (!nu) continue;
+      float ref = 0.f;                       // the maximum that the sums are relative to, times scale log2 e
+      uint64_t sum2[2] = {0ull, 0ull};       // (two zeros each)
+      // The warps of a tile meet at barriers that cannot give up, so none of them leaves the loops: once a wait ran out all
+      // waits end at once, and the turns that are left go over whatever the scores hold.
 #pragma unroll 1
-          for (int c = 0; c < DP / 2; c += 16) {
-            uint32_t o[16];
-            ld16(to + c, o);
-            wait_ld(o);
+      for (int left = nu; left > 0; --left) {
+        bar_wait_warp(sfull + 8 * u, turn, &fault);
+        fence_after();
+        uint32_t r[64];
+        ld32(ts, r);
+        ld32(ts + 32, r + 32);
+        wait_ld(r);
+        if (kApart) {
+          fence_before();
+          bar_arrive(sread + 8 * u);
+        }
+        if (left == 1) {
+          const int last = r0 - half * 64;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            st16(to + c, o);
+          for (int c = 0; c < 64; ++c)
+            if (c > last) r[c] = __float_as_uint(-INFINITY);
+        }
+        float m4[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+#pragma unroll
+        for (int c = 4; c < 32; ++c) m4[c & 3] = max3(m4[c & 3], __uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+        const float top = max3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * sl;
+        const bool grows = any_of_tile(u, left == nu || top > ref + 8.f);
+        if (kApart && left < nu) bar_wait_warp(odone + 8 * u, turn ^ 1, &fault);
+        if (grows) {
+          joint[half * TILE + r0] = top;
+          sync_tile(u);
+          const float both = fmaxf(top, joint[(half ^ 1) * TILE + r0]);
+          sync_tile(u);
+          if (left == nu) {
+            ref = both == -INFINITY ? 0.f : both;
+          } else {
+            // (the output rests: the products of the tile before are done, as the scores' commit came behind them or odone says so)
+            fence_after();
+            const float next = fmaxf(ref, both), f = ex2(ref - next);
+            const uint64_t f2 = pair(f, f);
+            ref = next;
+            sum2[0] = mul2(sum2[0], f2);
+            sum2[1] = mul2(sum2[1], f2);
+#pragma unroll 1
+            for (int c = 0; c < DP / 2; c += 16) {
+              uint32_t o[16];
+              ld16(to + c, o);
+              wait_ld(o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              st16(to + c, o);
+            }
+            wait_st();
           }
-          wait_st();
         }
-      }
-      const uint64_t nref2 = pair(-ref, -ref);
+        const uint64_t nref2 = pair(-ref, -ref);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t pk[16];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[16];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float2 e = ex2_pair(fma2(pair(r[32 * h + 2 * c], r[32 * h + 2 * c + 1]), sl2, nref2));
-          sum2[c & 1] = add2(sum2[c & 1], pair(e.x, e.y));
-          pk[c] = pack2<T>(e.x, e.y);
+          for (int c = 0; c < 16; ++c) {
+            const float2 e = ex2_pair(fma2(pair(r[32 * h + 2 * c], r[32 * h + 2 * c + 1]), sl2, nref2));
+            sum2[c & 1] = add2(sum2[c & 1], pair(e.x, e.y));
+            pk[c] = pack2<T>(e.x, e.y);
+          }
+          st16(tp + 16 * h, pk);
         }
-        st16(tp + 16 * h, pk);
+        wait_st();
+        fence_before();
+        bar_arrive(pfull + 8 * u);
+        turn ^= 1;
       }
-      wait_st();
-      fence_before();
-      bar_arrive(pfull + 8 * u);
-    }
-    if (nu) {
-      bar_wait_warp(odone + 8 * u, kApart ? (nu - 1) & 1 : 0, &fault);
-      fence_after();
       const float2 a = unpair(add2(sum2[0], sum2[1]));
-      joint[u][half][r0] = a.x + a.y;
+      joint[half * TILE + r0] = a.x + a.y;
       sync_tile(u);
-      const float sum = joint[u][0][r0] + joint[u][1][r0], f = 1.f / sum;
-      const bool in = row < w.len;
-      if (in && half == 0) p.lse[(long long)head[u] * p.T + w.start + row] = ref + log2f(sum);
-      const int first = tile[u] * TILE + (warp & 3) * 32;      // the warp's first row
-      store_rows<T, DP>(to, f, smem_p + u * TB + (warp & 7) * 32 * DP, p.o + ((long long)(w.start + first) * p.heads + head[u]) * p.D * 2,
-                        (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
+      const float sum = joint[r0] + joint[TILE + r0], f = 1.f / sum;
+      sync_tile(u);
+      bar_wait_warp(odone + 8 * u, kApart ? turn ^ 1 : piece, &fault);
+      fence_after();
+      piece ^= 1;
+      const Work w2 = it.work(p, p.kv_heads);
+      const Pair x2(w2, it.head(p.kv_heads), p.group);
+      const int head = x2.head(u), first = (nu - 1) * TILE + (warp & 3) * 32;      // the warp's first row
+      if (half == 0 && first + lane < w2.len) p.lse[(long long)head * p.T + w2.start + first + lane] = ref + log2f(sum);
+      store_rows<T>(to, DP / 2, f, stage + warp * 2048, p.o + ((long long)(w2.start + first) * p.heads + head) * p.D * 2,
+                    (long long)p.heads * p.D * 2, w2.len - first, half * (DP / 2), p.D);
+      fence_before();      // (the accumulators are read: the next piece's products come behind its first P)
     }
   }
   fence_before();
@@ -429,55 +528,45 @@ __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_
   }
 }
 
+// At DP = 64 there is room for the outputs' way out beside the tiles; else it leads through the own tiles, whose next loads wait.
+template <int DP> constexpr bool kRoom = DP == 64;
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
         const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[18];
+  __shared__ __align__(8) unsigned long long bars[19];
   __shared__ float part[2][TILE];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
-  __shared__ Work work;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t qfull = bar0, kfull = bar0 + 8, kempty = bar0 + 32, vfull = bar0 + 56, vempty = bar0 + 72, sfull = bar0 + 88,
-                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128;
+                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, qempty = bar0 + 144;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
-  dependent_launch();
-  if (warp == 0) find_work(p, blockIdx.x / p.heads, 0, &work);
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const Work w = work;
-  const uint32_t tmem = tmem_;
-  if (w.len == 0) {
-    if (warp == 9) tmem_free(tmem, 512);
-    return;
-  }
-  const int head = blockIdx.x % p.heads, kvh = head / p.group, nt = (w.len + TILE - 1) / TILE;
-  const int tile = nt - 1 - w.unit, n = tile + 1;
-  if (w.nothing) {
-    zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D);
-    if (warp == 9) tmem_free(tmem, 512);
-    return;
-  }
-  const bool ragged = n * TILE > w.len;
   if (warp == 0) {
     if (lane == 31) {
       fault.raised = 0;
       fault.status = p.status;
     }
-    // (a lane a barrier: Q and dO arrive at one; the slots of K and V are freed by the zeros' warp too where that has them)
-    const int count = lane == 0 ? 2 : (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 1 + ragged : lane == 14 ? 256 : 1;
-    if (lane < 18) bar_init(bar0 + 8 * lane, count);
+    // (a lane a barrier: Q and dO arrive at one; the slots of K and V are freed by the products and by the zeros' warp)
+    const int count = lane == 0 || (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 2 : lane == 14 ? 256 : lane == 18 && !kRoom<DP> ? 8 : 1;
+    if (lane < 19) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
+  fence_before();
   __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_;
+  dependent_launch();
+  const int total = *(volatile const int*)p.listed * p.heads;
   const uint32_t sq = smem, sdo = smem + TB, sk = smem + 2 * TB, sv = smem + 5 * TB;
   const uint32_t tdp = tmem + 2 * TILE, tdq = tmem + 3 * TILE;
+  // tile of queries, and tiles of keys, of a piece
+  const auto tiles_of = [](const Work& w) { return (w.len + TILE - 1) / TILE - w.unit; };
 
   if (warp == 8) {
     const bool one = elect();
@@ -489,28 +578,49 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       }
       __syncwarp();
     };
-    load_tile(sq, &mq, w.start + tile * TILE, head, qfull);
-    load_tile(sdo, &mdo, w.start + tile * TILE, head, qfull);
-    for (int i = 0, s3 = 0, ph3 = 1; i < n; ++i) {
-      const int s2 = i & 1;
-      if (!bar_wait_warp(kempty + 8 * s3, ph3, &fault)) break;
-      load_tile(sk + s3 * TB, &mk, w.start + i * TILE, kvh, kfull + 8 * s3);
-      if (!bar_wait_warp(vempty + 8 * s2, ((i >> 1) & 1) ^ 1, &fault)) break;
-      load_tile(sv + s2 * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * s2);
-      if (++s3 == 3) { s3 = 0; ph3 ^= 1; }
+    bool ok = true;
+    int g = 0, pieces = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.heads);
+      const int head = it.head(p.heads), kvh = head / p.group, n = tiles_of(w);
+      if (w.nothing) continue;
+      // (the first keys before the queries, whose place may be taken by the last piece's way out)
+      for (int i = -1; i < n; ++i) {
+        if (i >= 0) {
+          if (!(ok = bar_wait_warp(vempty + 8 * (g & 1), ((g >> 1) & 1) ^ 1, &fault))) break;
+          load_tile(sv + (g & 1) * TB, &mv, w.start + i * TILE, kvh, vfull + 8 * (g & 1));
+          ++g;
+        }
+        if (i + 1 < n) {
+          if (!(ok = bar_wait_warp(kempty + 8 * (g % 3), ((g / 3) & 1) ^ 1, &fault))) break;
+          load_tile(sk + g % 3 * TB, &mk, w.start + (i + 1) * TILE, kvh, kfull + 8 * (g % 3));
+        }
+        if (i < 0) {
+          if (!(ok = bar_wait_warp(qempty, (pieces++ & 1) ^ 1, &fault))) break;
+          load_tile(sq, &mq, w.start + (n - 1) * TILE, head, qfull);
+          load_tile(sdo, &mdo, w.start + (n - 1) * TILE, head, qfull);
+        }
+      }
     }
   } else if (warp == 10) {
-    for (int i = 0; i < n && ragged; ++i) {
-      const int s3 = i % 3, s2 = i & 1;
-      if (!bar_wait_warp(kfull + 8 * s3, (i / 3) & 1, &fault) || !bar_wait_warp(vfull + 8 * s2, (i >> 1) & 1, &fault)) break;
-      if (i == n - 1) {
-        zero_rows(smem_p + 2 * TB + s3 * TB, ATOMS, w.len - i * TILE);
-        zero_rows(smem_p + 5 * TB + s2 * TB, ATOMS, w.len - i * TILE);
-      }
-      if (lane == 0) {
-        bar_arrive(ready + 8 * s2);
-        bar_arrive(kempty + 8 * s3);
-        bar_arrive(vempty + 8 * s2);
+    bool ok = true;
+    int g = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.heads);
+      const int n = tiles_of(w);
+      if (w.nothing) continue;
+      for (int i = 0; i < n; ++i, ++g) {
+        const int s3 = g % 3, s2 = g & 1;
+        if (!(ok = bar_wait_warp(kfull + 8 * s3, (g / 3) & 1, &fault) && bar_wait_warp(vfull + 8 * s2, (g >> 1) & 1, &fault))) break;
+        if (i == n - 1 && n * TILE > w.len) {
+          zero_rows(smem_p + 2 * TB + s3 * TB, ATOMS, w.len - i * TILE);
+          zero_rows(smem_p + 5 * TB + s2 * TB, ATOMS, w.len - i * TILE);
+        }
+        if (lane == 0) {
+          bar_arrive(ready + 8 * s2);
+          bar_arrive(kempty + 8 * s3);
+          bar_arrive(vempty + 8 * s2);
+        }
       }
     }
   } else if (warp == 9) {
@@ -519,13 +629,13 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
     const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
     const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
     const uint64_t aq = operand(sq), ado = operand(sdo), k0 = operand(sk), v0 = operand(sv), kt0 = operand(sk, kAtom);
-    const uint32_t values = ragged ? ready : vfull;
     const auto product = [&](uint32_t acc, uint64_t a, uint64_t b) {
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
         if (k < ksteps) mma_ss(acc, along(a, k), along(b, k), dscore, k > 0);
     };
-    // scores of tile i, over the dS of tile i - 2
+    bool ragged = false;
+    // scores of the tile that comes as number i, over the dS of number i - 2
     const auto scores = [&](int i) {
       const int s3 = i % 3;
       const uint32_t bar = ragged ? ready + 8 * (i & 1) : kfull + 8 * s3;
@@ -538,7 +648,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       return true;
     };
     const auto dprobs = [&](int i) {
-      if (!bar_wait_warp(values + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (!bar_wait_warp((ragged ? ready : vfull) + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
       if (one) {
         product(tdp, ado, v0 + (uint64_t)((i & 1) * (TB >> 4)));
         commit(dpfull);
@@ -547,92 +657,121 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       __syncwarp();
       return true;
     };
-    bool ok = bar_wait_warp(qfull, 0, &fault) && scores(0) && dprobs(0) && (n < 2 || scores(1));
+    bool ok = true;
+    int g = 0, pieces = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.heads);
+      const int n = tiles_of(w);
+      if (w.nothing) continue;
+      ragged = n * TILE > w.len;
+      if (!(ok = bar_wait_warp(qfull, pieces++ & 1, &fault) && scores(g) && dprobs(g) && (n < 2 || scores(g + 1)))) break;
 #pragma unroll 1
-    for (int i = 0; i < n && ok; ++i) {
-      if (!(ok = bar_wait_warp(dsfull, i & 1, &fault))) break;
-      fence_after();
-      if (i + 1 < n && !(ok = dprobs(i + 1))) break;
-      const uint64_t b = kt0 + (uint64_t)((i % 3) * (TB >> 4));
-      if (one) {
+      for (int i = 0; i < n; ++i, ++g) {
+        if (!(ok = bar_wait_warp(dsfull, g & 1, &fault))) break;
+        fence_after();
+        if (i + 1 < n && !(ok = dprobs(g + 1))) break;
+        const uint64_t b = kt0 + (uint64_t)((g % 3) * (TB >> 4));
+        if (one) {
 #pragma unroll
-        for (int k = 0; k < TILE / 16; ++k)
-          mma_ts(tdq, tmem + (i & 1) * TILE + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, i > 0 || k > 0);
-        commit(i + 1 < n ? kempty + 8 * (i % 3) : done);
+          for (int k = 0; k < TILE / 16; ++k)
+            mma_ts(tdq, tmem + (g & 1) * TILE + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, i > 0 || k > 0);
+          commit(kempty + 8 * (g % 3));
+          if (i + 1 == n) {
+            commit(done);
+            if (kRoom<DP>) commit(qempty);
+          }
+        }
+        __syncwarp();
+        if (i + 2 < n && !(ok = scores(g + 2))) break;
       }
-      __syncwarp();
-      if (i + 2 < n) ok = scores(i + 2);
     }
   } else {
-    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane, row = tile * TILE + r0;
+    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const bool in = row < w.len;
-    const long long at = (long long)head * p.T + w.start + row;
-    float d = 0.f;
-    if (in) {
-      const uint4* o = reinterpret_cast<const uint4*>(p.o + ((long long)(w.start + row) * p.heads + head) * p.D * 2);
-      const uint4* g = reinterpret_cast<const uint4*>(p.dout + ((w.start + row) * p.dout_t + head * p.dout_h) * 2);
+    const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
+    char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
+    int g = 0, pieces = 0;
+    // (as in the forward pass: the warps meet at a barrier for every piece, so none of them leaves)
+    for (Walk it; it.next(total);) {
+      const Work w = it.work(p, p.heads);
+      const int head = it.head(p.heads), n = tiles_of(w), tile = n - 1, row = tile * TILE + r0;
+      if (w.nothing) {
+        zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D, 256);
+        continue;
+      }
+      const bool in = row < w.len;
+      const long long at = (long long)head * p.T + w.start + row;
+      float d = 0.f;
+      if (in) {
+        const uint4* o = reinterpret_cast<const uint4*>(p.o + ((long long)(w.start + row) * p.heads + head) * p.D * 2);
+        const uint4* gr = reinterpret_cast<const uint4*>(p.dout + ((w.start + row) * p.dout_t + head * p.dout_h) * 2);
 #pragma unroll 4
-      for (int c = half * (DP / 16); c < (half + 1) * (DP / 16); ++c) {
-        if (c * 8 >= p.D) break;
-        const uint4 a = __ldcg(o + c), b = __ldcg(g + c);
-        const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+        for (int c = half * (DP / 16); c < (half + 1) * (DP / 16); ++c) {
+          if (c * 8 >= p.D) break;
+          const uint4 a = __ldcg(o + c), b = __ldcg(gr + c);
+          const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 x = unpack2<T>(av[j]), y = unpack2<T>(bv[j]);
-          d = fmaf(x.x, y.x, fmaf(x.y, y.y, d));
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = unpack2<T>(av[j]), y = unpack2<T>(bv[j]);
+            d = fmaf(x.x, y.x, fmaf(x.y, y.y, d));
+          }
         }
       }
-    }
-    part[half][r0] = d;
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float delta = part[0][r0] + part[1][r0];
-    const float lse = in ? __ldcg(p.lse + at) : 0.f;
-    if (in && half == 0) p.delta[at] = delta;
-    const uint64_t sl2 = pair(p.scale_log2, p.scale_log2), nlse2 = pair(-lse, -lse), ndelta2 = pair(-delta, -delta);
-    bool ok = true;
+      const float lse = in ? __ldcg(p.lse + at) : 0.f;
+      part[half][r0] = d;
+      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+      const float delta = part[0][r0] + part[1][r0];
+      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+      if (in && half == 0) p.delta[at] = delta;
+      const uint64_t nlse2 = pair(-lse, -lse), ndelta2 = pair(-delta, -delta);
 #pragma unroll 1
-    for (int i = 0; i < n; ++i) {
-      if (!(ok = bar_wait_warp(sfull + 8 * (i & 1), (i >> 1) & 1, &fault))) break;
-      fence_after();
-      const uint32_t ts = tmem + (i & 1) * TILE + half * 64 + lanes;
-      uint32_t r[64];
-      ld32(ts, r);
-      ld32(ts + 32, r + 32);
-      wait_ld(r);
-      probabilities(r, sl2, nlse2);
-      if (!(ok = bar_wait_warp(dpfull, i & 1, &fault))) break;
-      fence_after();
-      uint32_t g[64];
-      ld32(tdp + half * 64 + lanes, g);
-      ld32(tdp + half * 64 + 32 + lanes, g + 32);
-      wait_ld(g);
+      for (int i = 0; i < n; ++i, ++g) {
+        bar_wait_warp(sfull + 8 * (g & 1), (g >> 1) & 1, &fault);
+        fence_after();
+        const uint32_t ts = tmem + (g & 1) * TILE + half * 64 + lanes;
+        uint32_t r[64];
+        ld32(ts, r);
+        ld32(ts + 32, r + 32);
+        wait_ld(r);
+        probabilities(r, sl2, nlse2);
+        bar_wait_warp(dpfull, g & 1, &fault);
+        fence_after();
+        uint32_t v[64];
+        ld32(tdp + half * 64 + lanes, v);
+        ld32(tdp + half * 64 + 32 + lanes, v + 32);
+        wait_ld(v);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), add2(pair(g[2 * c], g[2 * c + 1]), ndelta2)));
-        g[2 * c] = __float_as_uint(t.x);
-        g[2 * c + 1] = __float_as_uint(t.y);
+        for (int c = 0; c < 32; ++c) {
+          const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), add2(pair(v[2 * c], v[2 * c + 1]), ndelta2)));
+          v[2 * c] = __float_as_uint(t.x);
+          v[2 * c + 1] = __float_as_uint(t.y);
+        }
+        if (i == n - 1) {
+          // the last column that the row sees (selected: above the diagonal anything may stand); a row that sees one key has a
+          // probability of 1, whatever its score
+          const int last = row == 0 ? -1 : r0 - half * 64;
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c > last) v[c] = 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = pack2<T>(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
+        st32(ts, v);
+        wait_st();
+        fence_before();
+        bar_arrive(dsfull);
       }
-      if (i == n - 1) {
-        // the last column that the row sees (selected: above the diagonal anything may stand); a row that sees one key has a
-        // probability of 1, whatever its score
-        const int last = row == 0 ? -1 : r0 - half * 64;
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > last) g[c] = 0u;
-      }
-#pragma unroll
-      for (int c = 0; c < 32; ++c) g[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
-      st32(ts, g);
-      wait_st();
-      fence_before();
-      bar_arrive(dsfull);
-    }
-    if (ok && bar_wait_warp(done, 0, &fault)) {
+      bar_wait_warp(done, pieces++ & 1, &fault);
       fence_after();
       const int first = tile * TILE + (warp & 3) * 32;
-      store_rows<T, DP>(tdq + half * (DP / 2) + lanes, p.scale, smem_p + warp * 32 * DP,
-                        p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2, (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
+      store_rows<T>(tdq + half * (DP / 2) + lanes, DP / 2, p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
+                    (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
+      fence_before();
+      if (!kRoom<DP>) {
+        fence_async_proxy();      // (the next load comes over what was written there)
+        __syncwarp();
+        if (lane == 0) bar_arrive(qempty);
+      }
     }
   }
   fence_before();
@@ -648,50 +787,33 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
          const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[18];
+  __shared__ __align__(8) unsigned long long bars[19];
   __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
-  __shared__ Work work;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
-                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128;
+                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, free_own = bar0 + 144;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
-  dependent_launch();
-  if (warp == 0) find_work(p, blockIdx.x / p.kv_heads, 0, &work);
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const Work w = work;
-  const uint32_t tmem = tmem_;
-  if (w.len == 0) {
-    if (warp == 9) tmem_free(tmem, 512);
-    return;
-  }
-  const int kvh = blockIdx.x % p.kv_heads, nt = (w.len + TILE - 1) / TILE;
-  const int tile = w.unit, per_head = nt - tile, n = per_head * p.group;
-  if (w.nothing) {
-    const int rows_here = min(TILE, w.len - tile * TILE);
-    zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
-    zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D);
-    if (warp == 9) tmem_free(tmem, 512);
-    return;
-  }
-  const bool ragged = nt * TILE > w.len;      // every head's last tile of queries reaches past the sequence
   if (warp == 0) {
     if (lane == 31) {
-      fault.raised = !fits(smem_p + 7 * TB, smem_raw);
+      fault.raised = !fits(smem_p + 7 * TB + (kRoom<DP> ? 8 * 2048 : 0), smem_raw);
       fault.status = p.status;
       if (fault.raised) atomicExch(p.status, 1u);
     }
-    // (a lane a barrier: K and V arrive at one, dO with lse and D at another; slots are freed by the zeros' warp too where that has them)
-    const int count = lane == 0 || lane == 7 || lane == 8 ? 2 : (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 1 + ragged : lane == 13 || lane == 14 ? 256 : 1;
-    if (lane < 18) bar_init(bar0 + 8 * lane, count);
+    // (a lane a barrier: K and V arrive at one, dO with lse and D at another; slots are freed by the products and by the zeros' warp)
+    const int count = lane == 0 || (lane >= 4 && lane < 11) ? 2 : lane == 13 || lane == 14 ? 256 : lane == 18 && !kRoom<DP> ? 8 : 1;
+    if (lane < 19) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
+  fence_before();
   __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_;
+  dependent_launch();
+  const int total = *(volatile const int*)p.listed * p.kv_heads;
   if (fault.raised) {
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
@@ -699,6 +821,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   }
   const uint32_t sk = smem, sv = smem + TB, sq = smem + 2 * TB, sg = smem + 5 * TB;
   const uint32_t tdp = tmem + TILE, tdv = tmem + 2 * TILE, tdk = tmem + 3 * TILE;
+  const auto tiles_in = [](const Work& w) { return (w.len + TILE - 1) / TILE; };      // tiles of the sequence; the piece's is number `unit`
 
   if (warp == 8) {
     const bool one = elect();
@@ -710,43 +833,63 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       }
       __syncwarp();
     };
-    load_tile(sk, &mk, w.start + tile * TILE, kvh, own);
-    load_tile(sv, &mv, w.start + tile * TILE, kvh, own);
-    for (int i = 0, head = kvh * p.group, q = tile; i < n; ++i) {
-      const int s3 = i % 3, s2 = i & 1, q0 = q * TILE;
-      if (!bar_wait_warp(qempty + 8 * s3, ((i / 3) & 1) ^ 1, &fault)) break;
-      load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
-      if (!bar_wait_warp(gempty + 8 * s2, ((i >> 1) & 1) ^ 1, &fault)) break;
-      load_tile(sg + s2 * TB, &mdo, w.start + q0, head, gfull + 8 * s2);
-      // behind the sequence's end P becomes 0
+    bool ok = true;
+    int g = 0, pieces = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int kvh = it.head(p.kv_heads), nt = tiles_in(w), n = (nt - w.unit) * p.group;
+      if (w.nothing) continue;
+      for (int i = 0, head = kvh * p.group, q = w.unit; i < n; ++i, ++g) {
+        const int s3 = g % 3, s2 = g & 1, q0 = q * TILE;
+        if (!(ok = bar_wait_warp(qempty + 8 * s3, ((g / 3) & 1) ^ 1, &fault))) break;
+        load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
+        if (!(ok = bar_wait_warp(gempty + 8 * s2, ((g >> 1) & 1) ^ 1, &fault))) break;
+        load_tile(sg + s2 * TB, &mdo, w.start + q0, head, gfull + 8 * s2);
+        // behind the sequence's end P becomes 0
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = lane + 32 * j;
-        const long long at = (long long)head * p.T + w.start + q0 + r;
-        const bool in = q0 + r < w.len;
-        nlse[s2][r] = in ? -__ldcg(p.lse + at) : -INFINITY;
-        ndelta[s2][r] = in ? -__ldcg(p.delta + at) : 0.f;
-      }
-      __syncwarp();
-      if (one) bar_arrive(gfull + 8 * s2);
-      if (++q == nt) {
-        q = tile;
-        ++head;
+        for (int j = 0; j < 4; ++j) {
+          const int r = lane + 32 * j;
+          const long long at = (long long)head * p.T + w.start + q0 + r;
+          const bool in = q0 + r < w.len;
+          nlse[s2][r] = in ? -__ldcg(p.lse + at) : -INFINITY;
+          ndelta[s2][r] = in ? -__ldcg(p.delta + at) : 0.f;
+        }
+        __syncwarp();
+        if (one) bar_arrive(gfull + 8 * s2);
+        if (i == 0) {
+          // (behind the first queries, as their place may be taken by the last piece's way out)
+          if (!(ok = bar_wait_warp(free_own, (pieces++ & 1) ^ 1, &fault))) break;
+          load_tile(sk, &mk, w.start + w.unit * TILE, kvh, own);
+          load_tile(sv, &mv, w.start + w.unit * TILE, kvh, own);
+        }
+        if (++q == nt) {
+          q = w.unit;
+          ++head;
+        }
       }
     }
   } else if (warp == 10) {
-    for (int i = 0, q = tile; i < n && ragged; ++i) {
-      const int s3 = i % 3, s2 = i & 1;
-      if (!bar_wait_warp(qfull + 8 * s3, (i / 3) & 1, &fault) || !bar_wait_warp(gfull + 8 * s2, (i >> 1) & 1, &fault)) break;
-      if (++q == nt) {
-        q = tile;
-        zero_rows(smem_p + 2 * TB + s3 * TB, ATOMS, w.len - (nt - 1) * TILE);
-        zero_rows(smem_p + 5 * TB + s2 * TB, ATOMS, w.len - (nt - 1) * TILE);
-      }
-      if (lane == 0) {
-        bar_arrive(ready + 8 * s2);
-        bar_arrive(qempty + 8 * s3);
-        bar_arrive(gempty + 8 * s2);
+    bool ok = true;
+    int g = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int nt = tiles_in(w), n = (nt - w.unit) * p.group;
+      if (w.nothing) continue;
+      for (int i = 0, q = w.unit; i < n; ++i, ++g) {
+        const int s3 = g % 3, s2 = g & 1;
+        if (!(ok = bar_wait_warp(qfull + 8 * s3, (g / 3) & 1, &fault) && bar_wait_warp(gfull + 8 * s2, (g >> 1) & 1, &fault))) break;
+        if (++q == nt) {
+          q = w.unit;
+          if (nt * TILE > w.len) {
+            zero_rows(smem_p + 2 * TB + s3 * TB, ATOMS, w.len - (nt - 1) * TILE);
+            zero_rows(smem_p + 5 * TB + s2 * TB, ATOMS, w.len - (nt - 1) * TILE);
+          }
+        }
+        if (lane == 0) {
+          bar_arrive(ready + 8 * s2);
+          bar_arrive(qempty + 8 * s3);
+          bar_arrive(gempty + 8 * s2);
+        }
       }
     }
   } else if (warp == 9) {
@@ -755,12 +898,12 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
     const uint32_t dout = product_desc<T>(TILE, ksteps * 16, false, true);
     const uint64_t ak = operand(sk), av = operand(sv), q0 = operand(sq), g0 = operand(sg), qt0 = operand(sq, kAtom), gt0 = operand(sg, kAtom);
-    const uint32_t douts = ragged ? ready : gfull;
     const auto product = [&](uint32_t acc, uint64_t a, uint64_t b) {
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
         if (k < ksteps) mma_ss(acc, along(a, k), along(b, k), dscore, k > 0);
     };
+    bool ragged = false;
     const auto scores = [&](int i) {
       const int s3 = i % 3;
       const uint32_t bar = ragged ? ready + 8 * (i & 1) : qfull + 8 * s3;
@@ -773,7 +916,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       return true;
     };
     const auto dprobs = [&](int i) {
-      if (!bar_wait_warp(douts + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (!bar_wait_warp((ragged ? ready : gfull) + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
       if (one) {
         product(tdp, av, g0 + (uint64_t)((i & 1) * (TB >> 4)));
         commit(dpfull);
@@ -785,25 +928,34 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
       for (int k = 0; k < TILE / 16; ++k) mma_ts(acc, a + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, add || k > 0);
     };
-    bool ok = bar_wait_warp(own, 0, &fault) && scores(0) && dprobs(0);
+    bool ok = true;
+    int g = 0, pieces = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int nt = tiles_in(w), n = (nt - w.unit) * p.group;
+      if (w.nothing) continue;
+      ragged = nt * TILE > w.len;      // every head's last tile of queries reaches past the sequence
+      if (!(ok = bar_wait_warp(own, pieces++ & 1, &fault) && scores(g) && dprobs(g))) break;
 #pragma unroll 1
-    for (int i = 0; i < n && ok; ++i) {
-      if (!(ok = bar_wait_warp(pfull, i & 1, &fault))) break;
-      fence_after();
-      if (one) outputs(tdv, tmem, gt0 + (uint64_t)((i & 1) * (TB >> 4)), i > 0);
-      __syncwarp();
-      if (i + 1 < n && !(ok = scores(i + 1))) break;
-      if (!(ok = bar_wait_warp(dsfull, i & 1, &fault))) break;
-      fence_after();
-      if (one) {
-        commit(gempty + 8 * (i & 1));      // dO, lse and D of tile i are no longer read
-        outputs(tdk, tdp, qt0 + (uint64_t)((i % 3) * (TB >> 4)), i > 0);
-        if (i + 1 == n) commit(done);
-      }
-      __syncwarp();
-      if (i + 1 < n) {
-        if (!(ok = dprobs(i + 1))) break;
-        if (one) commit(qempty + 8 * (i % 3));
+      for (int i = 0; i < n; ++i, ++g) {
+        if (!(ok = bar_wait_warp(pfull, g & 1, &fault))) break;
+        fence_after();
+        if (one) outputs(tdv, tmem, gt0 + (uint64_t)((g & 1) * (TB >> 4)), i > 0);
+        __syncwarp();
+        if (i + 1 < n && !(ok = scores(g + 1))) break;
+        if (!(ok = bar_wait_warp(dsfull, g & 1, &fault))) break;
+        fence_after();
+        if (one) {
+          commit(gempty + 8 * (g & 1));      // dO, lse and D of the tile are no longer read
+          outputs(tdk, tdp, qt0 + (uint64_t)((g % 3) * (TB >> 4)), i > 0);
+          if (i + 1 == n) {
+            commit(done);
+            if (kRoom<DP>) commit(free_own);
+          }
+        }
+        __syncwarp();
+        if (i + 1 < n && !(ok = dprobs(g + 1))) break;
+        if (one) commit(qempty + 8 * (g % 3));
         __syncwarp();
       }
     }
@@ -813,76 +965,93 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     const uint32_t ts = tmem + half * 64 + lanes, tp = tdp + half * 64 + lanes;
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
     const int first = r0 - half * 64;      // on the diagonal: the first column (query) of this half that sees the row (key)
+    char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
     bool ok = true;
+    int g = 0, pieces = 0;
+    for (Walk it; ok && it.next(total);) {
+      const Work w = it.work(p, p.kv_heads);
+      const int kvh = it.head(p.kv_heads), nt = tiles_in(w), tile = w.unit, n = (nt - tile) * p.group;
+      if (w.nothing) {
+        const int rows_here = min(TILE, w.len - tile * TILE);
+        zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, 256);
+        zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, 256);
+        continue;
+      }
 #pragma unroll 1
-    for (int i = 0, q = tile; i < n; ++i) {
-      const float4* l4 = reinterpret_cast<const float4*>(nlse[i & 1] + half * 64);
-      const float4* d4 = reinterpret_cast<const float4*>(ndelta[i & 1] + half * 64);
-      const bool diagonal = q == tile;
-      if (++q == nt) q = tile;
-      if (!(ok = bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault) && bar_wait_warp(sfull, i & 1, &fault))) break;
+      for (int i = 0, q = tile; i < n; ++i, ++g) {
+        const float4* l4 = reinterpret_cast<const float4*>(nlse[g & 1] + half * 64);
+        const float4* d4 = reinterpret_cast<const float4*>(ndelta[g & 1] + half * 64);
+        const bool diagonal = q == tile;
+        if (++q == nt) q = tile;
+        if (!(ok = bar_wait_warp(gfull + 8 * (g & 1), (g >> 1) & 1, &fault) && bar_wait_warp(sfull, g & 1, &fault))) break;
+        fence_after();
+        uint32_t r[64];
+        ld32(ts, r);
+        ld32(ts + 32, r + 32);
+        wait_ld(r);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float4 l = l4[c];
+          const float2 a = ex2_pair(fma2(pair(r[4 * c], r[4 * c + 1]), sl2, pair(l.x, l.y)));
+          const float2 b = ex2_pair(fma2(pair(r[4 * c + 2], r[4 * c + 3]), sl2, pair(l.z, l.w)));
+          r[4 * c] = __float_as_uint(a.x);
+          r[4 * c + 1] = __float_as_uint(a.y);
+          r[4 * c + 2] = __float_as_uint(b.x);
+          r[4 * c + 3] = __float_as_uint(b.y);
+        }
+        if (diagonal) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c < first) r[c] = 0u;
+        }
+        uint32_t o[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+        st32(ts, o);
+        wait_st();
+        fence_before();
+        bar_arrive(pfull);
+        if (!(ok = bar_wait_warp(dpfull, g & 1, &fault))) break;
+        fence_after();
+        uint32_t v[64];
+        ld32(tp, v);
+        ld32(tp + 32, v + 32);
+        wait_ld(v);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float4 l = d4[c];
+          const float2 a = unpair(mul2(pair(r[4 * c], r[4 * c + 1]), add2(pair(v[4 * c], v[4 * c + 1]), pair(l.x, l.y))));
+          const float2 b = unpair(mul2(pair(r[4 * c + 2], r[4 * c + 3]), add2(pair(v[4 * c + 2], v[4 * c + 3]), pair(l.z, l.w))));
+          v[4 * c] = __float_as_uint(a.x);
+          v[4 * c + 1] = __float_as_uint(a.y);
+          v[4 * c + 2] = __float_as_uint(b.x);
+          v[4 * c + 3] = __float_as_uint(b.y);
+        }
+        if (diagonal) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c < first) v[c] = 0u;
+          if (tile == 0 && half == 0) v[0] = 0u;      // (the first query sees one key: its probability is 1)
+        }
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
+        st32(tp, o);
+        wait_st();
+        fence_before();
+        bar_arrive(dsfull);
+      }
+      if (!ok || !(ok = bar_wait_warp(done, pieces++ & 1, &fault))) break;
       fence_after();
-      uint32_t r[64];
-      ld32(ts, r);
-      ld32(ts + 32, r + 32);
-      wait_ld(r);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 l = l4[c];
-        const float2 a = ex2_pair(fma2(pair(r[4 * c], r[4 * c + 1]), sl2, pair(l.x, l.y)));
-        const float2 b = ex2_pair(fma2(pair(r[4 * c + 2], r[4 * c + 3]), sl2, pair(l.z, l.w)));
-        r[4 * c] = __float_as_uint(a.x);
-        r[4 * c + 1] = __float_as_uint(a.y);
-        r[4 * c + 2] = __float_as_uint(b.x);
-        r[4 * c + 3] = __float_as_uint(b.y);
-      }
-      if (diagonal) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < first) r[c] = 0u;
-      }
-      uint32_t o[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-      st32(ts, o);
-      wait_st();
+      const int first_row = tile * TILE + (warp & 3) * 32;
+      const long long at = ((long long)(w.start + first_row) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
+      store_rows<T>(tdv + half * (DP / 2) + lanes, DP / 2, 1.f, stage, p.dv + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+      store_rows<T>(tdk + half * (DP / 2) + lanes, DP / 2, p.scale, stage, p.dk + at, pitch, w.len - first_row, half * (DP / 2), p.D);
       fence_before();
-      bar_arrive(pfull);
-      if (!(ok = bar_wait_warp(dpfull, i & 1, &fault))) break;
-      fence_after();
-      uint32_t g[64];
-      ld32(tp, g);
-      ld32(tp + 32, g + 32);
-      wait_ld(g);
-#pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 l = d4[c];
-        const float2 a = unpair(mul2(pair(r[4 * c], r[4 * c + 1]), add2(pair(g[4 * c], g[4 * c + 1]), pair(l.x, l.y))));
-        const float2 b = unpair(mul2(pair(r[4 * c + 2], r[4 * c + 3]), add2(pair(g[4 * c + 2], g[4 * c + 3]), pair(l.z, l.w))));
-        g[4 * c] = __float_as_uint(a.x);
-        g[4 * c + 1] = __float_as_uint(a.y);
-        g[4 * c + 2] = __float_as_uint(b.x);
-        g[4 * c + 3] = __float_as_uint(b.y);
+      if (!kRoom<DP>) {
+        fence_async_proxy();      // (the next load comes over what was written there)
+        __syncwarp();
+        if (lane == 0) bar_arrive(free_own);
       }
-      if (diagonal) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c < first) g[c] = 0u;
-        if (tile == 0 && half == 0) g[0] = 0u;      // (the first query sees one key: its probability is 1)
-      }
-#pragma unroll
-      for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(g[2 * c]), __uint_as_float(g[2 * c + 1]));
-      st32(tp, o);
-      wait_st();
-      fence_before();
-      bar_arrive(dsfull);
-    }
-    if (ok && bar_wait_warp(done, 0, &fault)) {
-      fence_after();
-      const int first = tile * TILE + (warp & 3) * 32;
-      const long long at = ((long long)(w.start + first) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
-      store_rows<T, DP>(tdv + half * (DP / 2) + lanes, 1.f, smem_p + warp * 32 * DP, p.dv + at, pitch, w.len - first, half * (DP / 2), p.D);
-      store_rows<T, DP>(tdk + half * (DP / 2) + lanes, p.scale, smem_p + TB + warp * 32 * DP, p.dk + at, pitch, w.len - first, half * (DP / 2), p.D);
     }
   }
   fence_before();
@@ -910,13 +1079,11 @@ long long most_units(long long T, int seqs, bool bounds, int group) {
 
 bool args_ok(int dtype, long long T, int heads, int kv_heads, int D, int seqs, float scale) {
   return (dtype == CHB_BF16 || dtype == CHB_F16) && T >= 1 && T < (1ll << 31) - 2 * TILE && heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 &&
-         heads <= 65535 && D >= 8 && D % 8 == 0 && D <= 128 && seqs >= 0 && scale > 0.f && scale < INFINITY;
+         D >= 8 && D % 8 == 0 && D <= 128 && seqs >= 0 && scale > 0.f && scale < INFINITY;
 }
 
-AttnArgs common_args(long long T, int heads, int kv_heads, int D, const int* cu, int seqs, float scale) {
+AttnArgs common_args(long long T, int heads, int kv_heads, int D, float scale) {
   AttnArgs p{};
-  p.cu = cu;
-  p.seqs = seqs;
   p.T = (int)T;
   p.heads = heads;
   p.kv_heads = kv_heads;
@@ -928,15 +1095,17 @@ AttnArgs common_args(long long T, int heads, int kv_heads, int D, const int* cu,
   return p;
 }
 
+unsigned ctas(long long pieces, int sms) { return (unsigned)(pieces < sms ? pieces : sms); }
+
 template <typename T, int DP>
-int run_forward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaStream_t s) {
+int run_forward(const CUtensorMap* m, const AttnArgs& p, long long pieces, int sms, cudaStream_t s) {
   static std::atomic<unsigned long long> done{0};
-  return launch_big(attn_forward<T, DP>, 6 * DP / 64 * kAtom + 1024, (unsigned)(p.kv_heads * units), kFwdThreads, s, done, m[0], m[1], m[2], p) ==
-                 cudaSuccess ? CHB_SUCCESS : CHB_ERR_CUDA;
+  return launch_big(attn_forward<T, DP>, 6 * DP / 64 * kAtom + 16 * 2048 + 1024, ctas(pieces, sms), kFwdThreads, s, done, m[0], m[1], m[2], p) == cudaSuccess
+             ? CHB_SUCCESS : CHB_ERR_CUDA;
 }
 template <typename T, int DP>
-int run_backward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaStream_t s) {
-  constexpr int kMost = 227 * 1024, kNeed = 7 * DP / 64 * kAtom + 1024;      // (of a CTA, static and dynamic)
+int run_backward(const CUtensorMap* m, const AttnArgs& p, long long tiles, int sms, cudaStream_t s) {
+  constexpr int kMost = 227 * 1024, kNeed = 7 * DP / 64 * kAtom + (kRoom<DP> ? 8 * 2048 : 0) + 1024;      // (of a CTA, static and dynamic)
   static std::atomic<unsigned long long> done_q{0}, done_kv{0};
   static std::atomic<int> own{0};      // static shared memory of attn_dkv
   if (!own.load(std::memory_order_relaxed)) {
@@ -945,8 +1114,8 @@ int run_backward(const CUtensorMap* m, const AttnArgs& p, long long units, cudaS
     own.store((int)f.sharedSizeBytes, std::memory_order_relaxed);
   }
   const int left = kMost - own.load(std::memory_order_relaxed);
-  if (launch_big(attn_dq<T, DP>, kNeed, (unsigned)(p.heads * units), kBwdThreads, s, done_q, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
-      launch_big(attn_dkv<T, DP>, kNeed < left ? kNeed : left, (unsigned)(p.kv_heads * units), kBwdThreads, s, done_kv, m[0], m[1], m[2], m[3], p) != cudaSuccess)
+  if (launch_big(attn_dq<T, DP>, kNeed, ctas(tiles * p.heads, sms), kBwdThreads, s, done_q, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
+      launch_big(attn_dkv<T, DP>, kNeed < left ? kNeed : left, ctas(tiles * p.kv_heads, sms), kBwdThreads, s, done_kv, m[0], m[1], m[2], m[3], p) != cudaSuccess)
     return CHB_ERR_CUDA;
   return CHB_SUCCESS;
 }
@@ -958,31 +1127,49 @@ using namespace chb;
 
 extern "C" {
 
+// Bytes of the list of work that the forward pass makes and the backward pass reads.
+int chb_attention_plan_bytes(long long T, int group, int seqs, int bounds, long long* out) {
+  if (!out || T < 1 || T >= (1ll << 31) - 2 * TILE || group < 1 || seqs < 0) return CHB_ERR_ARG;
+  *out = 16 * (kPlanHead + most_units(T, seqs, bounds != 0, group) + most_units(T, seqs, bounds != 0, 0));
+  return CHB_SUCCESS;
+}
+
 // q [T, heads, D], k and v [T, kv_heads, D] with strides[6] (token and head of each, in elements, multiples of 8; 16-byte aligned);
-// cu: seqs + 1 bounds on the device, or null: one sequence.  o [T, heads, D] contiguous, lse [heads, T].
+// cu: seqs + 1 bounds on the device, or null: one sequence.  o [T, heads, D] contiguous, lse [heads, T]; plan: see above.
 int chb_attention_forward(int dtype, const void* q, const void* k, const void* v, const long long* strides, long long T, int heads,
-                          int kv_heads, int D, const int* cu, int seqs, float scale, void* o, float* lse, cudaStream_t stream) {
-  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !strides || !o || !lse) return CHB_ERR_ARG;
-  const long long units = most_units(T, seqs, cu != nullptr, heads / kv_heads);
-  if (units * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;      // (CTAs of a launch)
-  AttnArgs p = common_args(T, heads, kv_heads, D, cu, seqs, scale);
+                          int kv_heads, int D, const int* cu, int seqs, float scale, void* o, float* lse, void* plan, cudaStream_t stream) {
+  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !strides || !o || !lse || !plan) return CHB_ERR_ARG;
+  const int group = heads / kv_heads, sms = sm_count();
+  const long long pairs = most_units(T, seqs, cu != nullptr, group), tiles = most_units(T, seqs, cu != nullptr, 0);
+  if (tiles * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;      // (pieces of work)
+  if (!sms) return CHB_ERR_CUDA;
+  AttnArgs p = common_args(T, heads, kv_heads, D, scale);
+  int4* const list = static_cast<int4*>(plan);
+  p.listed = static_cast<const int*>(plan);
+  p.list = list + kPlanHead;
   p.o = static_cast<char*>(o);
   p.lse = lse;
   CUtensorMap m[3];
   if (!p.status || !map3(&m[0], dtype, q, T, heads, D, strides[0], strides[1]) || !map3(&m[1], dtype, k, T, kv_heads, D, strides[2], strides[3]) ||
       !map3(&m[2], dtype, v, T, kv_heads, D, strides[4], strides[5])) return CHB_ERR_CUDA;
-  if (dtype == CHB_F16) return D <= 64 ? run_forward<__half, 64>(m, p, units, stream) : run_forward<__half, 128>(m, p, units, stream);
-  return D <= 64 ? run_forward<__nv_bfloat16, 64>(m, p, units, stream) : run_forward<__nv_bfloat16, 128>(m, p, units, stream);
+  if (launch_overlapped(attn_plan, dim3(1), dim3(1024), stream, cu, seqs, (int)T, group, (int)pairs, (int)tiles, list) != cudaSuccess) return CHB_ERR_CUDA;
+  const long long n = pairs * kv_heads;
+  if (dtype == CHB_F16) return D <= 64 ? run_forward<__half, 64>(m, p, n, sms, stream) : run_forward<__half, 128>(m, p, n, sms, stream);
+  return D <= 64 ? run_forward<__nv_bfloat16, 64>(m, p, n, sms, stream) : run_forward<__nv_bfloat16, 128>(m, p, n, sms, stream);
 }
 
-// strides[8]: also of dout.  delta: heads * T floats of workspace; dq, dk, dv contiguous.
+// strides[8]: also of dout.  plan: as the forward pass left it.  delta: heads * T floats of workspace; dq, dk, dv contiguous.
 int chb_attention_backward(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout, const long long* strides,
-                           const float* lse, long long T, int heads, int kv_heads, int D, const int* cu, int seqs, float scale, float* delta,
-                           void* dq, void* dk, void* dv, cudaStream_t stream) {
-  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !o || !dout || !strides || !lse || !delta || !dq || !dk || !dv) return CHB_ERR_ARG;
-  const long long units = most_units(T, seqs, cu != nullptr, 0);
-  if (units * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;      // (CTAs of a launch)
-  AttnArgs p = common_args(T, heads, kv_heads, D, cu, seqs, scale);
+                           const float* lse, const void* plan, long long T, int heads, int kv_heads, int D, int bounds, int seqs, float scale,
+                           float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
+  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !o || !dout || !strides || !lse || !plan || !delta || !dq || !dk || !dv) return CHB_ERR_ARG;
+  const int sms = sm_count();
+  const long long pairs = most_units(T, seqs, bounds != 0, heads / kv_heads), tiles = most_units(T, seqs, bounds != 0, 0);
+  if (tiles * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;
+  if (!sms) return CHB_ERR_CUDA;
+  AttnArgs p = common_args(T, heads, kv_heads, D, scale);
+  p.listed = static_cast<const int*>(plan) + 1;
+  p.list = static_cast<const int4*>(plan) + kPlanHead + pairs;
   p.o = static_cast<char*>(const_cast<void*>(o));
   p.lse = const_cast<float*>(lse);
   p.delta = delta;
@@ -995,8 +1182,8 @@ int chb_attention_backward(int dtype, const void* q, const void* k, const void* 
   CUtensorMap m[4];
   if (!p.status || !map3(&m[0], dtype, q, T, heads, D, strides[0], strides[1]) || !map3(&m[1], dtype, k, T, kv_heads, D, strides[2], strides[3]) ||
       !map3(&m[2], dtype, v, T, kv_heads, D, strides[4], strides[5]) || !map3(&m[3], dtype, dout, T, heads, D, strides[6], strides[7])) return CHB_ERR_CUDA;
-  if (dtype == CHB_F16) return D <= 64 ? run_backward<__half, 64>(m, p, units, stream) : run_backward<__half, 128>(m, p, units, stream);
-  return D <= 64 ? run_backward<__nv_bfloat16, 64>(m, p, units, stream) : run_backward<__nv_bfloat16, 128>(m, p, units, stream);
+  if (dtype == CHB_F16) return D <= 64 ? run_backward<__half, 64>(m, p, tiles, sms, stream) : run_backward<__half, 128>(m, p, tiles, sms, stream);
+  return D <= 64 ? run_backward<__nv_bfloat16, 64>(m, p, tiles, sms, stream) : run_backward<__nv_bfloat16, 128>(m, p, tiles, sms, stream);
 }
 
 }  // extern "C"

@@ -52,25 +52,24 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, unsigned parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-static __device__ __noinline__ bool bar_wait_slow(uint32_t bar, unsigned parity, Fault* fault) {
-  const unsigned long long t0 = now_ns();
+// Waits for the phase of the given parity to complete; false: given up (the caller leaves its loops, or goes on without
+// waiting).  No function call: one would have to save what a softmax holds in registers.  The timer is read every 256 tries,
+// as that takes most of a microsecond.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, Fault* fault) {
+  unsigned since = 0;      // (in 2^20 ns; wraps after 52 days)
+#pragma unroll 1
   for (unsigned n = 1;; ++n) {
     if (bar_try(bar, parity)) return true;
-    if ((n & 15u) == 0) {
+    if ((n & 255u) == 0) {
+      const unsigned now = (unsigned)(now_ns() >> 20);
+      if (n == 256) since = now;
       if (fault->raised) return false;
-      if (now_ns() - t0 > kWaitLimitNs || n > (1u << 30)) break;
+      if (now - since > (unsigned)(kWaitLimitNs >> 20) || n > (1u << 30)) break;
     }
   }
   fault->raised = 1;
   atomicExch(fault->status, 1u);
   return false;
-}
-// Waits for the phase of the given parity to complete; false: given up (the caller leaves its loops).
-__device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, Fault* fault) {
-#pragma unroll 1
-  for (int i = 0; i < 256; ++i)      // (the slow way begins by reading the global timer, which takes most of a microsecond)
-    if (bar_try(bar, parity)) return true;
-  return bar_wait_slow(bar, parity, fault);
 }
 // The same by a whole warp, with one answer for all its lanes (what follows is often a warp-wide instruction).
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, unsigned parity, Fault* fault) {

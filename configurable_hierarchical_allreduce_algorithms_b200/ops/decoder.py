@@ -27,8 +27,9 @@ N.optional("chb_linear_ce_backward", i32, [i32, vp, vp, i64, i32, i32, i32, vp, 
 
 N.optional("chb_head_rope_rows", i32, [i32, i32, C.POINTER(i32)])
 N.optional("chb_head_rope", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, vp, i32, f32, C.c_double, i32, vp, vp, vp])
-N.optional("chb_attention_forward", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp])
-N.optional("chb_attention_backward", i32, [i32, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp, vp, vp])
+N.optional("chb_attention_plan_bytes", i32, [i64, i32, i32, i32, C.POINTER(i64)])
+N.optional("chb_attention_forward", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp, vp])
+N.optional("chb_attention_backward", i32, [i32, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp])
 
 _HALF = (torch.bfloat16, torch.float16)
 _ROPE_TYPES = (*_HALF, torch.float32)
@@ -222,30 +223,42 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
 
 # ------------------------------------------------------------------------------------------------------ causal attention
 
+@lru_cache(maxsize=1024)
+def _plan_bytes(T: int, group: int, seqs: int, bounds: bool) -> int:
+    n = i64(0)
+    rc = N.lib().chb_attention_plan_bytes(T, group, seqs, bounds, C.byref(n))
+    if rc:
+        raise OperatorError(f"chb_attention_plan_bytes failed: {N.ERR_NAMES.get(rc, rc)}")
+    return n.value
+
+
 def _attention_forward(q, k, v, cu, scale):
     shape, dev = q.shape, q.device
     T, h, d = shape
+    hk, seqs = k.shape[1], 0 if cu is None else cu.shape[0] - 1
     o = torch.empty(shape, dtype=q.dtype, device=dev)
     lse = torch.empty((h, T), dtype=torch.float32, device=dev)
+    plan = torch.empty(_plan_bytes(T, h // hk, seqs, cu is not None) if T else 0, dtype=torch.uint8, device=dev)
     if T:
         q, k, v = _heads(q), _heads(k), _heads(v)
         (a, b, _), (c, e, _), (f, g, _) = q.stride(), k.stride(), v.stride()
-        _call("chb_attention_forward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), _eight(a, b, c, e, f, g, 0, 0), T, h,
-              k.shape[1], d, None if cu is None else cu.data_ptr(), 0 if cu is None else cu.shape[0] - 1, scale, o.data_ptr(), lse.data_ptr())
-    return o, lse
+        _call("chb_attention_forward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), _eight(a, b, c, e, f, g, 0, 0), T, h, hk, d,
+              None if cu is None else cu.data_ptr(), seqs, scale, o.data_ptr(), lse.data_ptr(), plan.data_ptr())
+    return o, lse, plan, -1 if cu is None else seqs
 
 
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, scale):
-        o, lse = _attention_forward(q, k, v, cu, scale)
-        ctx.save_for_backward(q, k, v, o, lse, cu)
-        ctx.scale = scale
+        o, lse, plan, seqs = _attention_forward(q, k, v, cu, scale)
+        ctx.save_for_backward(q, k, v, o, lse, plan)      # (the bounds are in the plan)
+        ctx.args = seqs, scale
         return o
 
     @_first_order
     def backward(ctx, grad):
-        q, k, v, o, lse, cu = ctx.saved_tensors
+        q, k, v, o, lse, plan = ctx.saved_tensors
+        seqs, scale = ctx.args
         dev = q.device
         T, h, d = q.shape
         kv = k.shape
@@ -257,8 +270,8 @@ class _CausalAttention(torch.autograd.Function):
             (a, b, _), (c, e, _), (f, g, _), (m, n, _) = q.stride(), k.stride(), v.stride(), grad.stride()
             delta = torch.empty((h, T), dtype=torch.float32, device=dev)
             _call("chb_attention_backward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), grad.data_ptr(),
-                  _eight(a, b, c, e, f, g, m, n), lse.data_ptr(), T, h, kv[1], d, None if cu is None else cu.data_ptr(),
-                  0 if cu is None else cu.shape[0] - 1, ctx.scale, delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+                  _eight(a, b, c, e, f, g, m, n), lse.data_ptr(), plan.data_ptr(), T, h, kv[1], d, seqs >= 0, max(seqs, 0), scale,
+                  delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         return dq, dk, dv, None, None
 
 
