@@ -701,24 +701,36 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       }
       const bool in = row < w.len;
       const long long at = (long long)head * p.T + w.start + row;
-      float d = 0.f;
-      if (in) {
-        const uint4* o = reinterpret_cast<const uint4*>(p.o + ((long long)(w.start + row) * p.heads + head) * p.D * 2);
-        const uint4* gr = reinterpret_cast<const uint4*>(p.dout + ((w.start + row) * p.dout_t + head * p.dout_h) * 2);
-#pragma unroll 4
-        for (int c = half * (DP / 16); c < (half + 1) * (DP / 16); ++c) {
-          if (c * 8 >= p.D) break;
-          const uint4 a = __ldcg(o + c), b = __ldcg(gr + c);
-          const uint32_t av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w};
+      // D of the warp's rows, a row's half to kLanes lanes, so that a load takes whole rows
+      constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
+      const int col = half * (DP / 2) + lane % kLanes * 8;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 x = unpack2<T>(av[j]), y = unpack2<T>(bv[j]);
+      for (int i = 0; i < kLanes; i += 4) {
+        uint4 ov[4], gv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = (warp & 3) * 32 + (i + j) * kAtOnce + lane / kLanes, tr = tile * TILE + r;
+          ov[j] = gv[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (tr < w.len && col < p.D) {
+            ov[j] = __ldcg(reinterpret_cast<const uint4*>(p.o + (((long long)(w.start + tr) * p.heads + head) * p.D + col) * 2));
+            gv[j] = __ldcg(reinterpret_cast<const uint4*>(p.dout + ((w.start + tr) * p.dout_t + head * p.dout_h + col) * 2));
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t av[4] = {ov[j].x, ov[j].y, ov[j].z, ov[j].w}, bv[4] = {gv[j].x, gv[j].y, gv[j].z, gv[j].w};
+          float d = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 x = unpack2<T>(av[k]), y = unpack2<T>(bv[k]);
             d = fmaf(x.x, y.x, fmaf(x.y, y.y, d));
           }
+#pragma unroll
+          for (int o = kLanes / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          if (lane % kLanes == 0) part[half][(warp & 3) * 32 + (i + j) * kAtOnce + lane / kLanes] = d;
         }
       }
       const float lse = in ? __ldcg(p.lse + at) : 0.f;
-      part[half][r0] = d;
       asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
       const float delta = part[0][r0] + part[1][r0];
       asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
