@@ -11,7 +11,7 @@
 //   forward  a CTA has two tiles of queries at a time (neighbouring in (tile, head of the group) order, so that two heads share
 //            the keys and values where there are groups): the products of one run while the other's exponentials are taken.
 //            One pass with a running maximum; the sums are rescaled only when a maximum grows by more than 2^8.
-//   dq       a CTA has a tile of queries and walks its keys; also writes D.
+//   dq       a CTA has a tile of queries and walks its keys; also finds D.
 //   dkv      a CTA has a tile of keys of one key head and walks the queries of all heads of the group that see it, so
 //            gradients of shared heads are summed in the accumulators, in one order: no atomics on results anywhere.
 //
@@ -701,11 +701,13 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       }
       const bool in = row < w.len;
       const long long at = (long long)head * p.T + w.start + row;
-      // D of the warp's rows, a row's half to kLanes lanes, so that a load takes whole rows
+      // D.  A piece with one tile of keys has all of P and dP at once and sums them (below): with few keys the rounding of O
+      // would weigh (sequences of two tokens, bf16: dQ off by 0.0036 of its norm, 0.0026 like this).  Else D = dO . O of the
+      // warp's rows, a row's half to kLanes lanes, so that a load takes whole rows.
       constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
       const int col = half * (DP / 2) + lane % kLanes * 8;
 #pragma unroll
-      for (int i = 0; i < kLanes; i += 4) {
+      for (int i = 0; i < kLanes && n > 1; i += 4) {
         uint4 ov[4], gv[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -731,11 +733,16 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         }
       }
       const float lse = in ? __ldcg(p.lse + at) : 0.f;
-      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-      const float delta = part[0][r0] + part[1][r0];
-      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-      if (in && half == 0) p.delta[at] = delta;
-      const uint64_t nlse2 = pair(-lse, -lse), ndelta2 = pair(-delta, -delta);
+      float delta = 0.f;
+      // the halves' sums of a row are added; the second barrier is for the next use
+      const auto join = [&] {
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        delta = part[0][r0] + part[1][r0];
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        if (in && half == 0) p.delta[at] = delta;
+      };
+      if (n > 1) join();
+      const uint64_t nlse2 = pair(-lse, -lse);
 #pragma unroll 1
       for (int i = 0; i < n; ++i, ++g) {
         bar_wait_warp(sfull + 8 * (g & 1), (g >> 1) & 1, &fault);
@@ -752,6 +759,15 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         ld32(tdp + half * 64 + lanes, v);
         ld32(tdp + half * 64 + 32 + lanes, v + 32);
         wait_ld(v);
+        if (n == 1) {
+          const int last = r0 - half * 64;
+          float d[2] = {0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 64; ++c) d[c & 1] += c > last ? 0.f : __uint_as_float(r[c]) * __uint_as_float(v[c]);
+          part[half][r0] = d[0] + d[1];
+          join();
+        }
+        const uint64_t ndelta2 = pair(-delta, -delta);
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), add2(pair(v[2 * c], v[2 * c + 1]), ndelta2)));
