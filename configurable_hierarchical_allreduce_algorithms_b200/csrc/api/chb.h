@@ -180,6 +180,32 @@ int chb_rs_adam(struct chb_comm* c, const void* const* grad, void* const* master
 int chb_adam_flat(const void* grad, void* master, void* m, void* v, void* param_bf16, long long n,
                   const float* hyper, chb_stream_t stream);
 
+/* --------------------------------------------------- operators of a decoder
+ * Device pointers throughout; 16-bit operands CHB_BF16 or CHB_F16; strides in elements, multiples of 16 bytes.  All
+ * launches go to `stream`; workspaces belong to the call, saved / plan buffers go from forward to backward. */
+/* causal attention: q [T, heads, D], k and v [T, kv_heads, D], D <= 128, a multiple of 8; cu: seqs + 1 bounds (device) or
+ * null.  strides: token and head of q, k, v (and dout).  lse, delta: heads * T floats */
+int chb_attention_plan_bytes(long long T, int group, int seqs, int bounds, long long* out);
+int chb_attention_forward(int dtype, const void* q, const void* k, const void* v, const long long* strides, long long T, int heads,
+                          int kv_heads, int D, const int* cu, int seqs, float scale, void* o, float* lse, void* plan, chb_stream_t stream);
+int chb_attention_backward(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
+                           const long long* strides, const float* lse, const void* plan, long long T, int heads, int kv_heads, int D,
+                           int bounds, int seqs, float scale, float* delta, void* dq, void* dk, void* dv, chb_stream_t stream);
+/* norm of the heads (w null: none) and rotation by position; dy null: forward, else gradients; part: chb_head_rope_rows() * D
+ * floats where dw is wanted.  Arrays of two: queries, keys; strides: token and head of x[0], x[1], dy[0], dy[1] */
+int chb_head_rope_rows(int heads_q, int heads_k, int* out);
+int chb_head_rope(int dtype, const void* const* x, const void* const* dy, void* const* y, const long long* strides, long long T,
+                  int heads_q, int heads_k, int D, const void* const* w, int w_dtype, const void* pos, int pos64, float eps,
+                  double base, int interleaved, float* part, void* const* dw, chb_stream_t stream);
+/* cross entropy of x [N, D] w [V, D]^T; reduction 0 none, 1 mean, 2 sum; dx, dw may be null */
+int chb_linear_ce_bytes(long long N, int D, int V, long long* saved, long long* forward, long long* backward);
+int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w, const long long* targets, long long N, int D, int V,
+                          long long ignore_index, int reduction, float* loss, void* saved, void* work, chb_stream_t stream);
+int chb_linear_ce_backward(int dtype, const void* w, const float* grad, long long N, int D, int V, int reduction, const void* saved,
+                           void* work, void* dx, void* dw, chb_stream_t stream);
+/* synchronises the stream; 0, or 1 after a bounded wait inside one of these kernels ran out; cleared by the call */
+int chb_matrix_status(unsigned* out, chb_stream_t stream);
+
 int chb_dtype_size(int dtype);
 const char* chb_version(void);
 

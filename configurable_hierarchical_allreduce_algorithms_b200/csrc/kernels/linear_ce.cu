@@ -40,7 +40,7 @@ struct Saved {
 
 struct GemmArgs {
   const int* count;
-  int N, V, v0, vn;          // rows of x at most; vocabulary, first column and width of the piece
+  int V, v0, vn;             // vocabulary, first column and width of the piece
   int D;
   int a_rows;                // LSE and GRAD: rows of x that a tile loads (all 128, or all there are: the others' results go nowhere)
   int bn;                    // columns of a tile: a multiple of 32 (GRAD and BOTH: of 64)
@@ -737,7 +737,7 @@ int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, con
       !map2(&mg, dtype, b.g, q.width, pad, q.width)) return CHB_ERR_CUDA;
   GemmArgs p{};
   p.count = sv.head;
-  p.N = N; p.V = V; p.D = D;
+  p.V = V; p.D = D;
   p.tgt = sv.tgt; p.lse2 = sv.lse2; p.gs = b.gs; p.g = b.g; p.ldg = q.width;
   p.slab_x = b.slab_x; p.slab_w = b.slab_w; p.split_x = q.split_x; p.split_w = q.split_w;
   p.rows_pad = (int)pad;
@@ -807,7 +807,7 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
   }
   GemmArgs p{};
   p.count = sv.head;
-  p.N = n; p.V = V; p.D = D; p.vn = V; p.bn = bn; p.a_rows = rows_loaded(n);
+  p.V = V; p.D = D; p.vn = V; p.bn = bn; p.a_rows = rows_loaded(n);
   p.part = f.part; p.tlogit = f.tlogit; p.tgt = sv.tgt; p.rows_pad = (int)pad;
   p.status = status_word();
   if (!p.status) return CHB_ERR_CUDA;

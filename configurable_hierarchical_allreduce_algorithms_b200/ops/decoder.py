@@ -4,7 +4,8 @@ grouped heads (``csrc/kernels/attention.cu``), and softmax cross entropy of a li
 (``csrc/kernels/linear_ce.cu``).
 
 They take CUDA tensors, run on the current stream of the tensors' device, and get their workspaces from torch's allocator,
-so they can be captured into CUDA graphs.  The reference stops at the collectives
+so they can be captured into CUDA graphs (a backward pass, as of every torch operation, only while no eager graph of the
+same leaves is alive).  Results and gradients do not depend on the order in which CTAs run: repeated calls agree bit for bit.  The reference stops at the collectives
 (testing/custom_implementations/work_dir/all_reduce/all_reduce_radix_batch.cpp:202); these are the operators of the
 models whose gradients this package's data-parallel paths move."""
 from __future__ import annotations
@@ -375,8 +376,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     _need(reduction in _REDUCTIONS, f"linear_cross_entropy: unknown reduction {reduction!r}")
     _need(x.is_cuda and weight.device == x.device and targets.device == x.device, "linear_cross_entropy: tensors of one CUDA device expected")
     if targets.numel() == 0:
-        zero = x.float().sum() + 0.0 * weight[:1].float().sum()
-        return x.float().sum(-1) if reduction == "none" else zero / 0.0 if reduction == "mean" else zero
+        nothing = weight[:0].float().sum()      # (zero, and zero gradients, whatever the weight holds)
+        rows = x.float().sum(-1) + nothing
+        return rows if reduction == "none" else rows.sum() + nothing + (float("nan") if reduction == "mean" else 0.0)
     args = x.reshape(-1, d), weight, targets.reshape(-1), int(ignore_index), _REDUCTIONS[reduction]
     loss = _LinearCrossEntropy.apply(*args) if _wants_grad(x, weight) else _loss_forward(*args)[0]
     return loss.view(targets.shape) if reduction == "none" else loss

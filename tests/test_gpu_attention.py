@@ -246,3 +246,44 @@ def test_captured_and_replayed_on_new_inputs(cuda):
     graph.replay()
     for a, b in zip(outs, run(q, k, v, do, cu)):
         assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(cuda):
+    inputs = [make(900, 4, 2, 64, torch.bfloat16, seed=i) for i in range(2)]
+    cus = [on_device([0, 100, 900]), on_device([0, 33, 700, 890])]
+    alone = [run(*inputs[i], cus[i]) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                o = chb.causal_attention(*inputs[i][:3], cus[i])
+                got[i].append((o.detach(), *torch.autograd.grad(o, inputs[i][:3], inputs[i][3])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))
+    chb.check_operators()
+
+
+@pytest.mark.parametrize("n", [3000, 70])
+def test_many_sequences_of_mixed_length(cuda, n):
+    """More sequences than a warp, or a block, has threads; the first rows of a long sequence among them."""
+    lens = [(i * 7919) % 11 for i in range(n)] + [777]
+    q, k, v, do = make(sum(lens), 2, 1, 32, torch.float16)
+    got = run(q, k, v, do, on_device(bounds(lens)))
+    alone = run(*(t[-777:].detach().requires_grad_() for t in (q, k, v)), do[-777:])
+    for a, b in zip(got, alone):
+        assert torch.equal(a[-777:], b)
+    check(q, k, v, do, bounds(lens))
+
+
+def test_gradients_of_some_inputs(cuda):
+    q, k, v, do = make(200, 4, 2, 64, torch.bfloat16)
+    _, dq, dk, dv = run(q, k, v, do)
+    o = chb.causal_attention(q.detach(), k, v.detach())
+    assert torch.equal(torch.autograd.grad(o, k, do)[0], dk)
+    with pytest.raises(RuntimeError):                          # (not differentiable twice)
+        g, = torch.autograd.grad(chb.causal_attention(q, k, v), q, do, create_graph=True)
+        g.sum().backward()

@@ -157,3 +157,51 @@ def test_differences(cuda):
         # third order: 2^-24 of the sum of sizes, and the outputs' own error of (D + 32) e twice
         size = sum((a.double() * b.double()).abs().sum() for a, b in zip(out, (gq, gk)))
         assert abs(f[0] - f[1] - slope) <= 160 * E * size
+
+
+def test_offsets_beyond_32_bits(cuda):
+    T, h, d, last = 66000, 128, 256, 9                         # 2.16e9 elements of q
+    g = torch.Generator(device="cuda").manual_seed(3)
+    small = [torch.randn(last, n, d, generator=g, device="cuda").bfloat16() for n in (h, 1, h, 1)]
+    big = [torch.zeros(T, t.shape[1], d, dtype=t.dtype, device="cuda") for t in small]
+    for b, t in zip(big, small):
+        b[-last:] = t
+    w = torch.ones(d, device="cuda")
+    pos = torch.arange(T, device="cuda", dtype=torch.int32)
+
+    def run(q, k, gq, gk, pos):
+        q.requires_grad_(), k.requires_grad_()
+        out = chb.head_norm_rope(q, k, w, w, pos)
+        return (*(t.detach() for t in out), *torch.autograd.grad(out, (q, k), (gq, gk)))
+
+    for a, b in zip(run(*big, pos), run(*small, pos[-last:])):
+        assert torch.equal(a[-last:], b)
+
+
+def test_captured_and_replayed_on_new_inputs(cuda):
+    q, k, wq, wk, gq, gk = make(300, 4, 2, 64, torch.bfloat16, torch.float32)
+    pos = torch.arange(300, device="cuda")
+
+    def step():
+        out = chb.head_norm_rope(q, k, wq, wk, pos)
+        return (*(t.detach() for t in out), *torch.autograd.grad(out, (q, k, wq, wk), (gq, gk)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]        # (two graphs of the same call share no workspace)
+    outs = []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step())
+    with torch.no_grad():
+        for a, b in zip((q, k, wq, wk, gq, gk), make(300, 4, 2, 64, torch.bfloat16, torch.float32, seed=4)):
+            a.copy_(b)
+        pos.add_(1000)
+    for graph in graphs:
+        graph.replay()
+    want = step()
+    for out in outs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -177,6 +177,7 @@ def test_no_rows(cuda):
     t = torch.zeros(0, dtype=torch.int64, device="cuda")
     assert chb.linear_cross_entropy(x, w, t).isnan()
     assert chb.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
+    w.data[0, 0] = float("inf")
     s = chb.linear_cross_entropy(x, w, t, reduction="sum")
     dx, dw = torch.autograd.grad(s, (x, w))
     assert s == 0 and dx.shape == x.shape and not dw.any()
@@ -220,3 +221,47 @@ def test_captured_and_replayed_on_new_inputs(cuda):
     graph.replay()
     for a, b in zip(outs, step()):
         assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits(cuda):
+    n, d, v, last = 66000, 32768, 96, 40                       # 2.16e9 elements of x
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.zeros(n, d, dtype=torch.bfloat16, device="cuda")
+    x[-last:] = torch.randn(last, d, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(v, d, generator=g, device="cuda") * (1.6 / d ** 0.5)).bfloat16().requires_grad_()
+    t = torch.randint(0, v, (n,), generator=g, device="cuda")
+    grad = torch.zeros(n, device="cuda")
+    grad[-last:] = torch.randn(last, generator=g, device="cuda")
+    x.requires_grad_()
+    loss = chb.linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad(loss, (x, w), grad)
+    want = formula(x[-last:], w, t[-last:], grad[-last:], -100, "none")
+    for got, ref, tol in zip((loss[-last:], dx[-last:], dw), want[:3], want[3:]):
+        # (dw is summed over all rows: 66000 more terms of zero add nothing)
+        assert ((got.double() - ref).abs() <= tol).all(), ((got.double() - ref).abs() - tol).max()
+    assert not dx[:-last].any()
+
+
+def test_two_streams_at_once(cuda):
+    """Calls that overlap share nothing: each stream's results are those of the call alone."""
+    inputs = [make(700, 256, 3000, torch.bfloat16, 0.3, seed=i) for i in range(2)]
+    grad = torch.ones((), device="cuda")
+
+    def step(i):
+        x, w, t = inputs[i]
+        loss = chb.linear_cross_entropy(x, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w), grad))
+
+    alone = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))
+    chb.check_operators()
