@@ -184,13 +184,14 @@ int chb_adam_flat(const void* grad, void* master, void* m, void* v, void* param_
  * Device pointers throughout; 16-bit operands CHB_BF16 or CHB_F16; strides in elements, multiples of 16 bytes.  All
  * launches go to `stream`; workspaces belong to the call, saved / plan buffers go from forward to backward. */
 /* causal attention: q [T, heads, D], k and v [T, kv_heads, D], D <= 128, a multiple of 8; cu: seqs + 1 bounds (device) or
- * null.  strides: token and head of q, k, v (and dout).  lse, delta: heads * T floats */
+ * null.  strides: token and head of q, k, v (and dout).  lse: heads * T floats */
 int chb_attention_plan_bytes(long long T, int group, int seqs, int bounds, long long* out);
 int chb_attention_forward(int dtype, const void* q, const void* k, const void* v, const long long* strides, long long T, int heads,
                           int kv_heads, int D, const int* cu, int seqs, float scale, void* o, float* lse, void* plan, chb_stream_t stream);
+int chb_attention_backward_bytes(long long T, int heads, int kv_heads, int D, int bounds, int seqs, long long* out);      /* of work */
 int chb_attention_backward(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout,
                            const long long* strides, const float* lse, const void* plan, long long T, int heads, int kv_heads, int D,
-                           int bounds, int seqs, float scale, float* delta, void* dq, void* dk, void* dv, chb_stream_t stream);
+                           int bounds, int seqs, float scale, void* work, void* dq, void* dk, void* dv, chb_stream_t stream);
 /* norm of the heads (w null: none) and rotation by position; dy null: forward, else gradients; part: chb_head_rope_rows() * D
  * floats where dw is wanted.  Arrays of two: queries, keys; strides: token and head of x[0], x[1], dy[0], dy[1] */
 int chb_head_rope_rows(int heads_q, int heads_k, int* out);

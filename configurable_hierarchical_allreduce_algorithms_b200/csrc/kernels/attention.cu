@@ -13,7 +13,8 @@
 //            One pass with a running maximum; the sums are rescaled only when a maximum grows by more than 2^8.
 //   dq       a CTA has a tile of queries and walks its keys; also finds D.
 //   dkv      a CTA has a tile of keys of one key head and walks the queries of all heads of the group that see it, so
-//            gradients of shared heads are summed in the accumulators, in one order: no atomics on results anywhere.
+//            gradients of shared heads are summed in the accumulators, in one order: no atomics on results anywhere.  Where
+//            there are few tiles for the SMs the group's heads are shared out; the last share to end adds all, in their order.
 //
 // Each has one CTA an SM that takes one piece of work after the other: the loads and first products of the next run under the
 // end of this one (8 x 1024 tokens, 16 heads of 64, forward: a CTA for each piece 53 us).  A first small kernel lists the
@@ -47,6 +48,10 @@ struct AttnArgs {
   const char* dout;       // strides in elements
   long long dout_t, dout_h;
   char *dq, *dk, *dv;     // contiguous
+  int split;              // dkv: shares of a group's heads, each a piece of its own
+  float* sums;            // split > 1: [piece][share][dV, dK][column][row]
+  int* arrived;           // shares of a piece that are there (dq clears them)
+  int pieces;
   unsigned* status;
 };
 
@@ -164,15 +169,15 @@ __device__ __forceinline__ uint64_t across(uint64_t tile, int k) { return tile +
 // A warp's 32 rows of `cols` columns of an accumulator, times a factor, to 16-bit rows in global memory: by way of 2 KB of shared
 // memory of the warp's own, so that a store covers 64 bytes of eight rows and not one 16-byte word of 32 (an epilogue at D = 128:
 // 5000 -> 1400 clocks).  `rows`: how many of the 32 exist, `pitch`: bytes between rows.
-template <typename T>
-__device__ __forceinline__ void store_rows(uint32_t acc, int cols, float f, char* stage, char* out, long long pitch, int rows, int col0, int D) {
+// fetch(c, r): the lane's row of columns c to c + 31.
+template <typename T, typename F>
+__device__ __forceinline__ void store_rows(F&& fetch, int cols, float f, char* stage, char* out, long long pitch, int rows, int col0, int D) {
   const int lane = threadIdx.x & 31;
 #pragma unroll 1
   for (int c = 0; c < cols; c += 32) {
     uint32_t r[32];
     __syncwarp();
-    ld32(acc + c, r);
-    wait_ld(r);
+    fetch(c, r);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       uint4 o;
@@ -193,6 +198,14 @@ __device__ __forceinline__ void store_rows(uint32_t acc, int cols, float f, char
   }
   __syncwarp();
 }
+// (from an accumulator)
+struct FromTmem {
+  uint32_t acc;
+  __device__ __forceinline__ void operator()(int c, uint32_t (&r)[32]) const {
+    ld32(acc + c, r);
+    wait_ld(r);
+  }
+};
 
 // (by the first `threads` threads of the CTA)
 __device__ __forceinline__ void zero_out(char* base, long long first, int rows, int heads, int head, int D, int threads) {
@@ -492,7 +505,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       const Pair x2(w2, it.head(p.kv_heads), p.group);
       const int head = x2.head(u), first = (nu - 1) * TILE + (warp & 3) * 32;      // the warp's first row
       if (half == 0 && first + lane < w2.len) p.lse[(long long)head * p.T + w2.start + first + lane] = ref + log2f(sum);
-      store_rows<T>(to, DP / 2, f, stage + warp * 2048, p.o + ((long long)(w2.start + first) * p.heads + head) * p.D * 2,
+      store_rows<T>(FromTmem{to}, DP / 2, f, stage + warp * 2048, p.o + ((long long)(w2.start + first) * p.heads + head) * p.D * 2,
                     (long long)p.heads * p.D * 2, w2.len - first, half * (DP / 2), p.D);
       fence_before();      // (the accumulators are read: the next piece's products come behind its first P)
     }
@@ -563,6 +576,8 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   const uint32_t tmem = tmem_;
   dependent_launch();
   const int total = *(volatile const int*)p.listed * p.heads;
+  if (p.split > 1)
+    for (int i = blockIdx.x * kBwdThreads + threadIdx.x; i < p.pieces; i += gridDim.x * kBwdThreads) p.arrived[i] = 0;
   const uint32_t sq = smem, sdo = smem + TB, sk = smem + 2 * TB, sv = smem + 5 * TB;
   const uint32_t tdp = tmem + 2 * TILE, tdq = tmem + 3 * TILE;
   // tile of queries, and tiles of keys, of a piece
@@ -792,7 +807,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       bar_wait_warp(done, pieces++ & 1, &fault);
       fence_after();
       const int first = tile * TILE + (warp & 3) * 32;
-      store_rows<T>(tdq + half * (DP / 2) + lanes, DP / 2, p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
+      store_rows<T>(FromTmem{tdq + half * (DP / 2) + lanes}, DP / 2, p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
                     (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
       fence_before();
       if (!kRoom<DP>) {
@@ -819,6 +834,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
+  __shared__ int last_share;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
@@ -841,7 +857,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   fence_after();
   const uint32_t tmem = tmem_;
   dependent_launch();
-  const int total = *(volatile const int*)p.listed * p.kv_heads;
+  const int shares = p.kv_heads * p.split, each = p.group / p.split;      // heads of a share
+  const int total = *(volatile const int*)p.listed * shares;
   if (fault.raised) {
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
@@ -864,10 +881,10 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     bool ok = true;
     int g = 0, pieces = 0;
     for (Walk it; ok && it.next(total);) {
-      const Work w = it.work(p, p.kv_heads);
-      const int kvh = it.head(p.kv_heads), nt = tiles_in(w), n = (nt - w.unit) * p.group;
+      const Work w = it.work(p, shares);
+      const int share = it.head(shares), kvh = share / p.split, nt = tiles_in(w), n = (nt - w.unit) * each;
       if (w.nothing) continue;
-      for (int i = 0, head = kvh * p.group, q = w.unit; i < n; ++i, ++g) {
+      for (int i = 0, head = share * each, q = w.unit; i < n; ++i, ++g) {
         const int s3 = g % 3, s2 = g & 1, q0 = q * TILE;
         if (!(ok = bar_wait_warp(qempty + 8 * s3, ((g / 3) & 1) ^ 1, &fault))) break;
         load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
@@ -900,8 +917,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     bool ok = true;
     int g = 0;
     for (Walk it; ok && it.next(total);) {
-      const Work w = it.work(p, p.kv_heads);
-      const int nt = tiles_in(w), n = (nt - w.unit) * p.group;
+      const Work w = it.work(p, shares);
+      const int nt = tiles_in(w), n = (nt - w.unit) * each;
       if (w.nothing) continue;
       for (int i = 0, q = w.unit; i < n; ++i, ++g) {
         const int s3 = g % 3, s2 = g & 1;
@@ -959,8 +976,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     bool ok = true;
     int g = 0, pieces = 0;
     for (Walk it; ok && it.next(total);) {
-      const Work w = it.work(p, p.kv_heads);
-      const int nt = tiles_in(w), n = (nt - w.unit) * p.group;
+      const Work w = it.work(p, shares);
+      const int nt = tiles_in(w), n = (nt - w.unit) * each;
       if (w.nothing) continue;
       ragged = nt * TILE > w.len;      // every head's last tile of queries reaches past the sequence
       if (!(ok = bar_wait_warp(own, pieces++ & 1, &fault) && scores(g) && dprobs(g))) break;
@@ -994,12 +1011,13 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
     const int first = r0 - half * 64;      // on the diagonal: the first column (query) of this half that sees the row (key)
     char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
-    bool ok = true;
     int g = 0, pieces = 0;
-    for (Walk it; ok && it.next(total);) {
-      const Work w = it.work(p, p.kv_heads);
-      const int kvh = it.head(p.kv_heads), nt = tiles_in(w), tile = w.unit, n = (nt - tile) * p.group;
+    // (as in the forward pass: the warps may meet at barriers, so none of them leaves)
+    for (Walk it; it.next(total);) {
+      const Work w = it.work(p, shares);
+      const int share = it.head(shares), kvh = share / p.split, nt = tiles_in(w), tile = w.unit, n = (nt - tile) * each;
       if (w.nothing) {
+        if (share % p.split) continue;
         const int rows_here = min(TILE, w.len - tile * TILE);
         zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, 256);
         zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, 256);
@@ -1011,7 +1029,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         const float4* d4 = reinterpret_cast<const float4*>(ndelta[g & 1] + half * 64);
         const bool diagonal = q == tile;
         if (++q == nt) q = tile;
-        if (!(ok = bar_wait_warp(gfull + 8 * (g & 1), (g >> 1) & 1, &fault) && bar_wait_warp(sfull, g & 1, &fault))) break;
+        bar_wait_warp(gfull + 8 * (g & 1), (g >> 1) & 1, &fault);
+        bar_wait_warp(sfull, g & 1, &fault);
         fence_after();
         uint32_t r[64];
         ld32(ts, r);
@@ -1039,7 +1058,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         wait_st();
         fence_before();
         bar_arrive(pfull);
-        if (!(ok = bar_wait_warp(dpfull, g & 1, &fault))) break;
+        bar_wait_warp(dpfull, g & 1, &fault);
         fence_after();
         uint32_t v[64];
         ld32(tp, v);
@@ -1068,12 +1087,55 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         fence_before();
         bar_arrive(dsfull);
       }
-      if (!ok || !(ok = bar_wait_warp(done, pieces++ & 1, &fault))) break;
+      bar_wait_warp(done, pieces++ & 1, &fault);
       fence_after();
       const int first_row = tile * TILE + (warp & 3) * 32;
       const long long at = ((long long)(w.start + first_row) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
-      store_rows<T>(tdv + half * (DP / 2) + lanes, DP / 2, 1.f, stage, p.dv + at, pitch, w.len - first_row, half * (DP / 2), p.D);
-      store_rows<T>(tdk + half * (DP / 2) + lanes, DP / 2, p.scale, stage, p.dk + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+      const FromTmem dv{tdv + half * (DP / 2) + lanes}, dk{tdk + half * (DP / 2) + lanes};
+      if (p.split == 1) {
+        store_rows<T>(dv, DP / 2, 1.f, stage, p.dv + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+        store_rows<T>(dk, DP / 2, p.scale, stage, p.dk + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+      } else {
+        const int piece = (int)(it.at() / p.split);
+        float* const mine = p.sums + ((long long)piece * p.split + share % p.split) * 2 * DP * TILE + half * (DP / 2) * TILE + r0;
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {      // (dV's columns, then dK's)
+          uint32_t r[32];
+          __syncwarp();
+          if (c < DP / 2) dv(c, r);
+          else dk(c - DP / 2, r);
+          float* const to = mine + (c < DP / 2 ? c : DP + c - DP / 2) * TILE;
+#pragma unroll
+          for (int i2 = 0; i2 < 32; ++i2) __stcg(to + i2 * TILE, __uint_as_float(r[i2]));
+        }
+        // all of the CTA's sums are written before it says so; the last to say so reads all
+        __threadfence();
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        if (threadIdx.x == 0) last_share = atomicAdd(p.arrived + piece, 1) == p.split - 1;
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        if (last_share) {
+          __threadfence();
+          const float* const all = p.sums + (long long)piece * p.split * 2 * DP * TILE + half * (DP / 2) * TILE + r0;
+          const auto summed = [&](int tensor) {
+            return [&, tensor](int c, uint32_t (&r)[32]) {
+              float f[32];
+#pragma unroll
+              for (int i2 = 0; i2 < 32; ++i2) f[i2] = 0.f;
+#pragma unroll 1
+              for (int k = 0; k < p.split; ++k) {
+                const float* from = all + ((long long)k * 2 + tensor) * DP * TILE + c * TILE;
+#pragma unroll
+                for (int i2 = 0; i2 < 32; ++i2) f[i2] += __ldcg(from + i2 * TILE);
+              }
+#pragma unroll
+              for (int i2 = 0; i2 < 32; ++i2) r[i2] = __float_as_uint(f[i2]);
+            };
+          };
+          store_rows<T>(summed(0), DP / 2, 1.f, stage, p.dv + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+          store_rows<T>(summed(1), DP / 2, p.scale, stage, p.dk + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+        }
+        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");      // (last_share is read)
+      }
       fence_before();
       if (!kRoom<DP>) {
         fence_async_proxy();      // (the next load comes over what was written there)
@@ -1131,6 +1193,31 @@ int run_forward(const CUtensorMap* m, const AttnArgs& p, long long pieces, int s
   return launch_big(attn_forward<T, DP>, 6 * DP / 64 * kAtom + 16 * 2048 + 1024, ctas(pieces, sms), kFwdThreads, s, done, m[0], m[1], m[2], p) == cudaSuccess
              ? CHB_SUCCESS : CHB_ERR_CUDA;
 }
+// Shares of a group's heads in dkv: as many as give every SM four pieces, where there are less than three for two SMs.  Beyond
+// that the sums' way through memory costs more than it gives (8191 tokens in 12 sequences, 16 / 4 heads of 128, 248 pieces: 121 us,
+// with two shares 134 us; 6000 tokens, 16 / 2 heads, 94 pieces: one share about 560 us by the longest piece, two 334 us, four 305 us).
+int head_shares(long long tiles, int kv_heads, int group, int sms) {
+  const long long pieces = tiles * kv_heads, want = 2 * pieces >= 3ll * sms ? 1 : (4ll * sms + pieces - 1) / pieces;
+  int n = 1;
+  for (int d = 2; d <= group && d <= want; ++d)
+    if (group % d == 0) n = d;
+  return n;
+}
+
+struct BackwardWork { float* delta; int* arrived; float* sums; };
+long long backward_layout(char* base, long long T, int heads, int kv_heads, int D, long long tiles, int split, BackwardWork* w) {
+  long long at = 0;
+  const auto take = [&](long long bytes) {
+    char* const r = base ? base + at : nullptr;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  w->delta = reinterpret_cast<float*>(take(4 * heads * T));
+  w->arrived = reinterpret_cast<int*>(take(split > 1 ? 4 * tiles * kv_heads : 0));
+  w->sums = reinterpret_cast<float*>(take(split > 1 ? tiles * kv_heads * split * 2 * (D <= 64 ? 64 : 128) * TILE * 4 : 0));
+  return at;
+}
+
 template <typename T, int DP>
 int run_backward(const CUtensorMap* m, const AttnArgs& p, long long tiles, int sms, cudaStream_t s) {
   constexpr int kMost = 227 * 1024, kNeed = 7 * DP / 64 * kAtom + (kRoom<DP> ? 8 * 2048 : 0) + 1024;      // (of a CTA, static and dynamic)
@@ -1143,7 +1230,7 @@ int run_backward(const CUtensorMap* m, const AttnArgs& p, long long tiles, int s
   }
   const int left = kMost - own.load(std::memory_order_relaxed);
   if (launch_big(attn_dq<T, DP>, kNeed, ctas(tiles * p.heads, sms), kBwdThreads, s, done_q, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
-      launch_big(attn_dkv<T, DP>, kNeed < left ? kNeed : left, ctas(tiles * p.kv_heads, sms), kBwdThreads, s, done_kv, m[0], m[1], m[2], m[3], p) != cudaSuccess)
+      launch_big(attn_dkv<T, DP>, kNeed < left ? kNeed : left, ctas(tiles * p.kv_heads * p.split, sms), kBwdThreads, s, done_kv, m[0], m[1], m[2], m[3], p) != cudaSuccess)
     return CHB_ERR_CUDA;
   return CHB_SUCCESS;
 }
@@ -1186,11 +1273,21 @@ int chb_attention_forward(int dtype, const void* q, const void* k, const void* v
   return D <= 64 ? run_forward<__nv_bfloat16, 64>(m, p, n, sms, stream) : run_forward<__nv_bfloat16, 128>(m, p, n, sms, stream);
 }
 
-// strides[8]: also of dout.  plan: as the forward pass left it.  delta: heads * T floats of workspace; dq, dk, dv contiguous.
+int chb_attention_backward_bytes(long long T, int heads, int kv_heads, int D, int bounds, int seqs, long long* out) {
+  const int sms = sm_count();
+  if (!out || !args_ok(CHB_BF16, T, heads, kv_heads, D, seqs, 1.f)) return CHB_ERR_ARG;
+  if (!sms) return CHB_ERR_CUDA;
+  const long long tiles = most_units(T, seqs, bounds != 0, 0);
+  BackwardWork w;
+  *out = backward_layout(nullptr, T, heads, kv_heads, D, tiles, head_shares(tiles, kv_heads, heads / kv_heads, sms), &w);
+  return CHB_SUCCESS;
+}
+
+// strides[8]: also of dout.  plan: as the forward pass left it.  work: see above; dq, dk, dv contiguous.
 int chb_attention_backward(int dtype, const void* q, const void* k, const void* v, const void* o, const void* dout, const long long* strides,
                            const float* lse, const void* plan, long long T, int heads, int kv_heads, int D, int bounds, int seqs, float scale,
-                           float* delta, void* dq, void* dk, void* dv, cudaStream_t stream) {
-  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !o || !dout || !strides || !lse || !plan || !delta || !dq || !dk || !dv) return CHB_ERR_ARG;
+                           void* work, void* dq, void* dk, void* dv, cudaStream_t stream) {
+  if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !o || !dout || !strides || !lse || !plan || !work || !dq || !dk || !dv) return CHB_ERR_ARG;
   const int sms = sm_count();
   const long long pairs = most_units(T, seqs, bounds != 0, heads / kv_heads), tiles = most_units(T, seqs, bounds != 0, 0);
   if (tiles * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;
@@ -1200,7 +1297,13 @@ int chb_attention_backward(int dtype, const void* q, const void* k, const void* 
   p.list = static_cast<const int4*>(plan) + kPlanHead + pairs;
   p.o = static_cast<char*>(const_cast<void*>(o));
   p.lse = const_cast<float*>(lse);
-  p.delta = delta;
+  BackwardWork bw;
+  p.split = head_shares(tiles, kv_heads, heads / kv_heads, sms);
+  backward_layout(static_cast<char*>(work), T, heads, kv_heads, D, tiles, p.split, &bw);
+  p.delta = bw.delta;
+  p.arrived = bw.arrived;
+  p.sums = bw.sums;
+  p.pieces = (int)(tiles * kv_heads);
   p.dout = static_cast<const char*>(dout);
   p.dout_t = strides[6];
   p.dout_h = strides[7];

@@ -29,6 +29,7 @@ N.optional("chb_linear_ce_backward", i32, [i32, vp, vp, i64, i32, i32, i32, vp, 
 N.optional("chb_head_rope_rows", i32, [i32, i32, C.POINTER(i32)])
 N.optional("chb_head_rope", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, vp, i32, f32, C.c_double, i32, vp, vp, vp])
 N.optional("chb_attention_plan_bytes", i32, [i64, i32, i32, i32, C.POINTER(i64)])
+N.optional("chb_attention_backward_bytes", i32, [i64, i32, i32, i32, i32, i32, C.POINTER(i64)])
 N.optional("chb_attention_forward", i32, [i32, vp, vp, vp, vp, i64, i32, i32, i32, vp, i32, f32, vp, vp, vp, vp])
 N.optional("chb_attention_backward", i32, [i32, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp])
 
@@ -233,6 +234,16 @@ def _plan_bytes(T: int, group: int, seqs: int, bounds: bool) -> int:
     return n.value
 
 
+@lru_cache(maxsize=1024)
+def _backward_bytes(device: torch.device, T: int, h: int, hk: int, d: int, bounds: bool, seqs: int) -> int:
+    n = i64(0)
+    with torch.cuda.device(device):
+        rc = N.lib().chb_attention_backward_bytes(T, h, hk, d, bounds, seqs, C.byref(n))
+    if rc:
+        raise OperatorError(f"chb_attention_backward_bytes failed: {N.ERR_NAMES.get(rc, rc)}")
+    return n.value
+
+
 def _attention_forward(q, k, v, cu, scale):
     shape, dev = q.shape, q.device
     T, h, d = shape
@@ -269,10 +280,11 @@ class _CausalAttention(torch.autograd.Function):
         if T:
             q, k, v, grad = _heads(q), _heads(k), _heads(v), _heads(grad)
             (a, b, _), (c, e, _), (f, g, _), (m, n, _) = q.stride(), k.stride(), v.stride(), grad.stride()
-            delta = torch.empty((h, T), dtype=torch.float32, device=dev)
+            bounds, seqs = seqs >= 0, max(seqs, 0)
+            work = torch.empty(_backward_bytes(dev, T, h, kv[1], d, bounds, seqs), dtype=torch.uint8, device=dev)
             _call("chb_attention_backward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), grad.data_ptr(),
-                  _eight(a, b, c, e, f, g, m, n), lse.data_ptr(), plan.data_ptr(), T, h, kv[1], d, seqs >= 0, max(seqs, 0), scale,
-                  delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+                  _eight(a, b, c, e, f, g, m, n), lse.data_ptr(), plan.data_ptr(), T, h, kv[1], d, bounds, seqs, scale,
+                  work.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         return dq, dk, dv, None, None
 
 

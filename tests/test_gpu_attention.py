@@ -201,8 +201,12 @@ def test_offsets_beyond_32_bits(cuda):
         t.requires_grad_()
     cu = on_device(list(range(0, T + 1, n)))
     got = run(*big, cu)
-    for a, b in zip(got, run(*last)):
-        assert torch.equal(a[-n:], b) and not a[:-n].any()
+    alone = run(*last)
+    assert all(torch.equal(a[-n:], b) for a, b in zip(got[:2], alone))
+    # (how many CTAs share the heads that dk and dv sum over depends on the number of tokens: another order, no other bound)
+    want, tol = formula(*last, [0, n], d ** -0.5)
+    for a, b, t in zip(got, want, tol):
+        assert ((a[-n:].double() - b).abs() <= t).all() and not a[:-n].any()
 
 
 def test_differences(cuda):
@@ -274,8 +278,7 @@ def test_many_sequences_of_mixed_length(cuda, n):
     q, k, v, do = make(sum(lens), 2, 1, 32, torch.float16)
     got = run(q, k, v, do, on_device(bounds(lens)))
     alone = run(*(t[-777:].detach().requires_grad_() for t in (q, k, v)), do[-777:])
-    for a, b in zip(got, alone):
-        assert torch.equal(a[-777:], b)
+    assert all(torch.equal(a[-777:], b) for a, b in zip(got[:2], alone))      # (dk and dv: summed in another order, see above)
     check(q, k, v, do, bounds(lens))
 
 
