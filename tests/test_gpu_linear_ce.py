@@ -82,7 +82,11 @@ def test_matches_the_formula(cuda, dtype, reduction, n, d, v, ignored):
 
 
 def test_several_pieces_of_the_vocabulary(cuda):
-    check(*make(8192, 64, 7001, torch.bfloat16, 0.2), "mean")      # 114 MB of G: several pieces
+    check(*make(8192, 64, 7001, torch.bfloat16, 0.2), "mean")      # 114 MB of G
+
+
+def test_more_pieces_of_the_vocabulary(cuda):
+    check(*make(9000, 72, 25001, torch.float16, 0.05), "mean")     # more than 400 MB of G: three pieces of 192 MiB
 
 
 def test_negative_and_zero_gradients(cuda):
