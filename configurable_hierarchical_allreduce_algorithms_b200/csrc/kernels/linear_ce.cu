@@ -490,24 +490,39 @@ ce_gather_few(const long long* targets, const char* x, long long ldx, int N, int
   }
 }
 
-// Joins the column tiles of 32 rows (lane = row, the eight warps take every eighth tile) and, in the last CTA to come, the
-// sum over the rows: CTA sums in the order of the rows, whichever CTA is last.
-__global__ void __launch_bounds__(256)
+// Joins the column tiles of 32 rows (lane = row, the 32 warps take every 32nd tile, eight loads at a time: the kernel is a
+// chain of latencies, JOINFIG) and, in the last CTA to come, the sum over
+// the rows: CTA sums in the order of the rows, whichever CTA is last.
+constexpr int kJoinWarps = 32, kJoinLoads = 8;
+
+__global__ void __launch_bounds__(kJoinWarps * 32)
 ce_join(const float2* part, const float* tlogit, int nt, int rows_pad, int reduction, Saved sv, double* sums, float* loss) {
-  __shared__ float sm[8][32], ss[8][32];
+  __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32];
   __shared__ int is_last;
   dependent_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int count = *(volatile const int*)sv.head;
   const int row = blockIdx.x * 32 + lane;
   const bool in = row < count;
+  int label = -1;
+  float target = 0.f;
+  if (in && warp == 0) label = sv.tgt[row], target = tlogit[row];
   float m = -INFINITY, s = 0.f;
   if (in) {
-#pragma unroll 4
-    for (int t = warp; t < nt; t += 8) {
-      const float2 v = part[(long long)t * rows_pad + row];
-      const float nm = fmaxf(m, v.x), ref = nm == -INFINITY ? 0.f : nm;
-      s = s * ex2((m - ref) * kLog2e) + v.y * ex2((v.x - ref) * kLog2e);
+    for (int t0 = warp; t0 < nt; t0 += kJoinWarps * kJoinLoads) {
+      float2 v[kJoinLoads];
+#pragma unroll
+      for (int i = 0; i < kJoinLoads; ++i) {
+        const int t = t0 + i * kJoinWarps;
+        v[i] = t < nt ? part[(long long)t * rows_pad + row] : make_float2(-INFINITY, 0.f);
+      }
+      float nm = m;
+#pragma unroll
+      for (int i = 0; i < kJoinLoads; ++i) nm = fmaxf(nm, v[i].x);
+      const float ref = nm == -INFINITY ? 0.f : nm;
+      s *= ex2((m - ref) * kLog2e);
+#pragma unroll
+      for (int i = 0; i < kJoinLoads; ++i) s += v[i].y * ex2((v[i].x - ref) * kLog2e);
       m = nm;
     }
   }
@@ -519,13 +534,13 @@ ce_join(const float2* part, const float* tlogit, int nt, int rows_pad, int reduc
     if (in) {
       float M = m;
 #pragma unroll
-      for (int w = 1; w < 8; ++w) M = fmaxf(M, sm[w][lane]);
+      for (int w = 1; w < kJoinWarps; ++w) M = fmaxf(M, sm[w][lane]);
       const float ref = M == -INFINITY ? 0.f : M;
       float S = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) S += ss[w][lane] * ex2((sm[w][lane] - ref) * kLog2e);
-      const bool known = sv.tgt[row] >= 0;
-      loss_r = known ? logf(S) + (M - tlogit[row]) : __int_as_float(0x7fffffff);      // (no such label: NaN)
+      for (int w = 0; w < kJoinWarps; ++w) S += ss[w][lane] * ex2((sm[w][lane] - ref) * kLog2e);
+      const bool known = label >= 0;
+      loss_r = known ? logf(S) + (M - target) : __int_as_float(0x7fffffff);      // (no such label: NaN)
       sv.lse2[row] = known ? fmaf(M, kLog2e, log2f(S)) : __int_as_float(0x7fffffff);
       if (reduction == 0) loss[sv.idx[row]] = loss_r;
     }
@@ -816,7 +831,7 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
   const cudaError_t e = dtype == CHB_F16 ? gemm<__half, LSE>(mx, mw, mw, p, tiles, sms, stream)
                                          : gemm<__nv_bfloat16, LSE>(mx, mw, mw, p, tiles, sms, stream);
   if (e != cudaSuccess) return CHB_ERR_CUDA;
-  if (launch_overlapped(ce_join, dim3((unsigned)(pad / 32)), dim3(256), stream, (const float2*)f.part, (const float*)f.tlogit, nt, (int)pad,
+  if (launch_overlapped(ce_join, dim3((unsigned)(pad / 32)), dim3(kJoinWarps * 32), stream, (const float2*)f.part, (const float*)f.tlogit, nt, (int)pad,
                         reduction, sv, f.sums, loss) != cudaSuccess) return CHB_ERR_CUDA;
   return CHB_SUCCESS;
 }

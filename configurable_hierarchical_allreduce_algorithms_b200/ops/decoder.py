@@ -44,6 +44,7 @@ class OperatorError(RuntimeError):
 
 _current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _functions: dict = {}
+_empty_like, _contiguous = torch.empty_like, torch.contiguous_format
 
 
 def _call(name: str, device: torch.device, *args) -> None:
@@ -70,6 +71,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous, on a 16-byte boundary (copied if it is not)."""
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """Uninitialised and contiguous, otherwise like ``t`` (half the time of torch.empty with a shape, type and device)."""
+    return _empty_like(t, memory_format=_contiguous)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -130,8 +136,7 @@ def _head_rope(x, dy, y, heads, w, pos, eps, base, interleaved, part=None, dw=No
 
 
 def _rope_forward(q, k, wq, wk, pos, eps, base, interleaved):
-    # (not empty_like: the outputs are contiguous whatever q and k are)
-    y = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    y = _new(q), _new(k)
     if q.shape[0]:
         _head_rope((_heads(q), _heads(k)), None, y, (q.shape[1], k.shape[1]), None if wq is None else (_aligned(wq), _aligned(wk)), pos, eps,
                    base, interleaved)
@@ -152,7 +157,7 @@ class _HeadNormRope(torch.autograd.Function):
     def backward(ctx, gq, gk):
         saved = ctx.saved_tensors
         pos = saved[0]
-        dx = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device), torch.empty(gk.shape, dtype=gk.dtype, device=gk.device)
+        dx = _new(gq), _new(gk)
         heads = gq.shape[1], gk.shape[1]
         x = w = part = dw = None
         if len(saved) > 1:
@@ -248,7 +253,7 @@ def _attention_forward(q, k, v, cu, scale):
     shape, dev = q.shape, q.device
     T, h, d = shape
     hk, seqs = k.shape[1], 0 if cu is None else cu.shape[0] - 1
-    o = torch.empty(shape, dtype=q.dtype, device=dev)
+    o = _new(q)
     lse = torch.empty((h, T), dtype=torch.float32, device=dev)
     plan = torch.empty(_plan_bytes(T, h // hk, seqs, cu is not None) if T else 0, dtype=torch.uint8, device=dev)
     if T:
@@ -274,9 +279,7 @@ class _CausalAttention(torch.autograd.Function):
         dev = q.device
         T, h, d = q.shape
         kv = k.shape
-        dq = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        dk = torch.empty(kv, dtype=q.dtype, device=dev)
-        dv = torch.empty(kv, dtype=q.dtype, device=dev)
+        dq, dk, dv = _new(q), _new(k), _new(v)
         if T:
             q, k, v, grad = _heads(q), _heads(k), _heads(v), _heads(grad)
             (a, b, _), (c, e, _), (f, g, _), (m, n, _) = q.stride(), k.stride(), v.stride(), grad.stride()
