@@ -220,7 +220,8 @@ __device__ __forceinline__ void zero_out(char* base, long long first, int rows, 
 // What bounds the kernel is the chain scores -> softmax -> product of one tile (per tile of 128 x 128: 1024 clocks of products
 // at D = 128, 1024 of the special function unit, and latencies between them), so each tile has a warp of its own for its
 // products, and four warps a scheduler hide the latencies in a softmax (16384 tokens, 16 / 4 heads of 128: 858 us; with two
-// warps a scheduler 1066 us, or 917 us with tile 1 held back by half a turn).
+// warps a scheduler 1066 us, or 917 us with tile 1 held back by half a turn).  That case runs at 1.28 PFLOP/s.  Short
+// sequences pay for the ends of their pieces: 4 x 2048 tokens, 16 heads of 128, 85 us, 0.81 PFLOP/s; 8 x 1024, 16 of 64, 47 us.
 constexpr int kFwdThreads = 640;
 
 // Whether any of a tile's 256 threads wants it; barrier 1 + tile
@@ -528,7 +529,10 @@ __device__ __forceinline__ bool fits(const char* end, const char* dynamic) {
 // Both kernels: warps 0-7 hold the tile's rows twice, each half of the 128 columns (P and dS of a half go over the first half
 // of its scores' columns, so no thread writes where another reads); warp 8 loads, a thread of warp 9 issues the products,
 // warp 10 writes the zeros.  Shared memory: the CTA's own two tiles, three slots of the operand that is used by two products
-// and two of the other.
+// and two of the other.  P is made in both (seven products for five): one kernel for all three gradients would add dq with
+// atomics, in an order that changes from run to run.  What bounds them is the chain of two products, exponentials and a third
+// product, and the ends of the pieces (4 x 2048 tokens, 16 heads of 128: dq 119 us, 0.87 PFLOP/s; dkv 135 us, 1.02 PFLOP/s; the
+// tensor pipe is busy 53 and 57 % of the time).
 constexpr int kBwdThreads = 352;
 
 // 64 scores of a row: P = exp2(scale S - lse)
@@ -544,6 +548,7 @@ __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_
 // At DP = 64 there is room for the outputs' way out beside the tiles; else it leads through the own tiles, whose next loads wait.
 template <int DP> constexpr bool kRoom = DP == 64;
 
+// A tile of queries against its keys: S = Q K^T, dP = dO V^T, dQ += dS K.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -824,6 +829,8 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   if (warp == 9) tmem_free(tmem, 512);
 }
 
+// A tile of keys against the queries that see it, of all heads of the group (or of a share of them): the transposes
+// S^T = K Q^T and dP^T = V dO^T, so that dV += P^T dO and dK += dS^T Q have their left operands in tensor memory.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,

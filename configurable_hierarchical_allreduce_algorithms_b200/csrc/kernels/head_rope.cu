@@ -6,6 +6,8 @@
 // Bound by HBM: every element is read once and written once.  A group of lanes holds one head, each lane two vectors
 // of its pairs, so norm, rotation and both sums stay in registers; a warp keeps the sines of its token for all its heads and
 // has the next heads' loads in flight while it works on these (the compiler may not move them ahead of the stores itself).
+// 8192 tokens, 16 + 16 heads of 128, bf16: forward 33 us (134 MB, 4.1 TB/s), backward with dw 47 us (201 MB, 4.3 TB/s); latency
+// and the registers that the loads ahead take are what is between that and a copy's 6.5 TB/s.
 // A CTA has queries or keys only, so that a thread sums one weight's gradient.
 // Angles: base^(-2i/D) / 2 pi is a 64-bit fraction of a turn, and position times fraction wraps modulo one turn exactly,
 // so far positions are as exact as near ones; only the angle within the turn is rounded to fp32.
