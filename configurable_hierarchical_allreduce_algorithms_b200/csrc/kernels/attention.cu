@@ -526,19 +526,19 @@ __device__ __forceinline__ bool fits(const char* end, const char* dynamic) {
 }
 
 // ------------------------------------------------------------------ backward
-// Both kernels: warps 0-7 hold the tile's rows twice, each half of the 128 columns (P and dS of a half go over the first half
-// of its scores' columns, so no thread writes where another reads); warp 8 loads, a thread of warp 9 issues the products,
-// warp 10 writes the zeros.  Shared memory: the CTA's own two tiles, three slots of the operand that is used by two products
+// Both kernels: warps 0-15 hold the tile's rows four times, each a quarter of the 128 columns (P and dS of a quarter go over the
+// first half of its scores' columns, so no thread writes where another reads); warp 16 loads, warp 17 issues the products,
+// warp 18 writes the zeros.  Shared memory: the CTA's own two tiles, three slots of the operand that is used by two products
 // and two of the other.  P is made in both (seven products for five): one kernel for all three gradients would add dq with
 // atomics, in an order that changes from run to run.  What bounds them is the chain of two products, exponentials and a third
 // product, and the ends of the pieces (4 x 2048 tokens, 16 heads of 128: dq 119 us, 0.87 PFLOP/s; dkv 135 us, 1.02 PFLOP/s; the
 // tensor pipe is busy 53 and 57 % of the time).
-constexpr int kBwdThreads = 352;
+constexpr int kRowWarps = 16, kRowThreads = kRowWarps * 32, kBwdThreads = kRowThreads + 96;
 
-// 64 scores of a row: P = exp2(scale S - lse)
+// 32 scores of a row: P = exp2(scale S - lse)
 __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_t nlse2) {
 #pragma unroll
-  for (int c = 0; c < 32; ++c) {
+  for (int c = 0; c < 16; ++c) {
     const float2 e = ex2_pair(fma2(pair(r[2 * c], r[2 * c + 1]), sl2, nlse2));
     r[2 * c] = __float_as_uint(e.x);
     r[2 * c + 1] = __float_as_uint(e.y);
@@ -564,14 +564,14 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   const uint32_t qfull = bar0, kfull = bar0 + 8, kempty = bar0 + 32, vfull = bar0 + 56, vempty = bar0 + 72, sfull = bar0 + 88,
                  dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, qempty = bar0 + 144;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
+  if (warp == kRowWarps + 1) tmem_alloc(smem_u32(&tmem_), 512);
   if (warp == 0) {
     if (lane == 31) {
       fault.raised = 0;
       fault.status = p.status;
     }
     // (a lane a barrier: Q and dO arrive at one; the slots of K and V are freed by the products and by the zeros' warp)
-    const int count = lane == 0 || (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 2 : lane == 14 ? 256 : lane == 18 && !kRoom<DP> ? 8 : 1;
+    const int count = lane == 0 || (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 2 : lane == 14 ? kRowThreads : lane == 18 && !kRoom<DP> ? kRowWarps : 1;
     if (lane < 19) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
@@ -588,7 +588,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   // tile of queries, and tiles of keys, of a piece
   const auto tiles_of = [](const Work& w) { return (w.len + TILE - 1) / TILE - w.unit; };
 
-  if (warp == 8) {
+  if (warp == kRowWarps) {
     const bool one = elect();
     const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
       if (one) {
@@ -622,7 +622,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         }
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == kRowWarps + 2) {
     bool ok = true;
     int g = 0;
     for (Walk it; ok && it.next(total);) {
@@ -643,7 +643,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         }
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kRowWarps + 1) {
     const bool one = elect();
     const int ksteps = (p.D + 15) / 16;
     const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
@@ -694,7 +694,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         if (one) {
 #pragma unroll
           for (int k = 0; k < TILE / 16; ++k)
-            mma_ts(tdq, tmem + (g & 1) * TILE + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, i > 0 || k > 0);
+            mma_ts(tdq, tmem + (g & 1) * TILE + (k >> 1) * 32 + (k & 1) * 8, across(b, k), dout, i > 0 || k > 0);
           commit(kempty + 8 * (g % 3));
           if (i + 1 == n) {
             commit(done);
@@ -706,7 +706,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       }
     }
   } else {
-    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane;
+    const int quarter = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
     char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
@@ -716,22 +716,21 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       const Work w = it.work(p, p.heads);
       const int head = it.head(p.heads), n = tiles_of(w), tile = n - 1, row = tile * TILE + r0;
       if (w.nothing) {
-        zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D, 256);
+        zero_out(p.dq, w.start + tile * TILE, min(TILE, w.len - tile * TILE), p.heads, head, p.D, kRowThreads);
         continue;
       }
       const bool in = row < w.len;
       const long long at = (long long)head * p.T + w.start + row;
       // D.  A piece with one tile of keys has all of P and dP at once and sums them (below): with few keys the rounding of O
-      // would weigh (sequences of two tokens, bf16: dQ off by 0.0036 of its norm, 0.0026 like this).  Else D = dO . O of the
-      // warp's rows, a row's half to kLanes lanes, so that a load takes whole rows.
-      constexpr int kLanes = DP / 16, kAtOnce = 32 / kLanes;
-      const int col = half * (DP / 2) + lane % kLanes * 8;
+      // would weigh (sequences of two tokens, bf16: dQ off by 0.0036 of its norm, 0.0026 like this).  Else D = dO . O, eight rows
+      // a warp, a row to kLanes lanes, so that a load takes whole rows.
+      constexpr int kLanes = DP / 8, kAtOnce = 32 / kLanes, kSteps = TILE / kRowWarps / kAtOnce;
+      if (n > 1) {
+        const int col = lane % kLanes * 8;
+        uint4 ov[kSteps], gv[kSteps];
 #pragma unroll
-      for (int i = 0; i < kLanes && n > 1; i += 4) {
-        uint4 ov[4], gv[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = (warp & 3) * 32 + (i + j) * kAtOnce + lane / kLanes, tr = tile * TILE + r;
+        for (int j = 0; j < kSteps; ++j) {
+          const int tr = tile * TILE + warp * (TILE / kRowWarps) + j * kAtOnce + lane / kLanes;
           ov[j] = gv[j] = make_uint4(0u, 0u, 0u, 0u);
           if (tr < w.len && col < p.D) {
             ov[j] = __ldcg(reinterpret_cast<const uint4*>(p.o + (((long long)(w.start + tr) * p.heads + head) * p.D + col) * 2));
@@ -739,7 +738,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kSteps; ++j) {
           const uint32_t av[4] = {ov[j].x, ov[j].y, ov[j].z, ov[j].w}, bv[4] = {gv[j].x, gv[j].y, gv[j].z, gv[j].w};
           float d = 0.f;
 #pragma unroll
@@ -749,47 +748,53 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
           }
 #pragma unroll
           for (int o = kLanes / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-          if (lane % kLanes == 0) part[half][(warp & 3) * 32 + (i + j) * kAtOnce + lane / kLanes] = d;
+          if (lane % kLanes == 0) part[0][warp * (TILE / kRowWarps) + j * kAtOnce + lane / kLanes] = d;
         }
       }
       const float lse = in ? __ldcg(p.lse + at) : 0.f;
       float delta = 0.f;
-      // the halves' sums of a row are added; the second barrier is for the next use
-      const auto join = [&] {
-        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-        delta = part[0][r0] + part[1][r0];
-        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-        if (in && half == 0) p.delta[at] = delta;
-      };
-      if (n > 1) join();
+      const auto meet = [] { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kRowThreads) : "memory"); };
+      if (n > 1) {
+        meet();
+        delta = part[0][r0];
+        meet();      // (for the next use)
+        if (in && quarter == 0) p.delta[at] = delta;
+      }
       const uint64_t nlse2 = pair(-lse, -lse);
 #pragma unroll 1
       for (int i = 0; i < n; ++i, ++g) {
         bar_wait_warp(sfull + 8 * (g & 1), (g >> 1) & 1, &fault);
         fence_after();
-        const uint32_t ts = tmem + (g & 1) * TILE + half * 64 + lanes;
-        uint32_t r[64];
+        const uint32_t ts = tmem + (g & 1) * TILE + quarter * 32 + lanes;
+        uint32_t r[32];
         ld32(ts, r);
-        ld32(ts + 32, r + 32);
         wait_ld(r);
         probabilities(r, sl2, nlse2);
         bar_wait_warp(dpfull, g & 1, &fault);
         fence_after();
-        uint32_t v[64];
-        ld32(tdp + half * 64 + lanes, v);
-        ld32(tdp + half * 64 + 32 + lanes, v + 32);
+        uint32_t v[32];
+        ld32(tdp + quarter * 32 + lanes, v);
         wait_ld(v);
         if (n == 1) {
-          const int last = r0 - half * 64;
+          const int last = r0 - quarter * 32;
           float d[2] = {0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 64; ++c) d[c & 1] += c > last ? 0.f : __uint_as_float(r[c]) * __uint_as_float(v[c]);
-          part[half][r0] = d[0] + d[1];
-          join();
+          for (int c = 0; c < 32; ++c) d[c & 1] += c > last ? 0.f : __uint_as_float(r[c]) * __uint_as_float(v[c]);
+          // (the quarters' sums: two and two, as shared memory has no room for four)
+          d[0] += d[1];
+          if (quarter >= 2) part[quarter - 2][r0] = d[0];
+          meet();
+          if (quarter < 2) d[0] += part[quarter][r0];
+          meet();
+          if (quarter < 2) part[quarter][r0] = d[0];
+          meet();
+          delta = part[0][r0] + part[1][r0];
+          meet();
+          if (in && quarter == 0) p.delta[at] = delta;
         }
         const uint64_t ndelta2 = pair(-delta, -delta);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = 0; c < 16; ++c) {
           const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), add2(pair(v[2 * c], v[2 * c + 1]), ndelta2)));
           v[2 * c] = __float_as_uint(t.x);
           v[2 * c + 1] = __float_as_uint(t.y);
@@ -797,14 +802,14 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         if (i == n - 1) {
           // the last column that the row sees (selected: above the diagonal anything may stand); a row that sees one key has a
           // probability of 1, whatever its score
-          const int last = row == 0 ? -1 : r0 - half * 64;
+          const int last = row == 0 ? -1 : r0 - quarter * 32;
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
+          for (int c = 0; c < 32; ++c)
             if (c > last) v[c] = 0u;
         }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = pack2<T>(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
-        st32(ts, v);
+        for (int c = 0; c < 16; ++c) v[c] = pack2<T>(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
+        st16(ts, v);
         wait_st();
         fence_before();
         bar_arrive(dsfull);
@@ -812,8 +817,9 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       bar_wait_warp(done, pieces++ & 1, &fault);
       fence_after();
       const int first = tile * TILE + (warp & 3) * 32;
-      store_rows<T>(FromTmem{tdq + half * (DP / 2) + lanes}, DP / 2, p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
-                    (long long)p.heads * p.D * 2, w.len - first, half * (DP / 2), p.D);
+      if (quarter * 32 < DP)
+        store_rows<T>(FromTmem{tdq + quarter * 32 + lanes}, 32, p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
+                      (long long)p.heads * p.D * 2, w.len - first, quarter * 32, p.D);
       fence_before();
       if (!kRoom<DP>) {
         fence_async_proxy();      // (the next load comes over what was written there)
@@ -826,7 +832,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
   __syncthreads();
   fence_after();
   if (fault.raised) drain_after_abort();
-  if (warp == 9) tmem_free(tmem, 512);
+  if (warp == kRowWarps + 1) tmem_free(tmem, 512);
 }
 
 // A tile of keys against the queries that see it, of all heads of the group (or of a share of them): the transposes
@@ -847,15 +853,15 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
                  dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, free_own = bar0 + 144;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 9) tmem_alloc(smem_u32(&tmem_), 512);
+  if (warp == kRowWarps + 1) tmem_alloc(smem_u32(&tmem_), 512);
   if (warp == 0) {
     if (lane == 31) {
-      fault.raised = !fits(smem_p + 7 * TB + (kRoom<DP> ? 8 * 2048 : 0), smem_raw);
+      fault.raised = !fits(smem_p + 7 * TB + (kRoom<DP> ? kRowWarps * 2048 : 0), smem_raw);
       fault.status = p.status;
       if (fault.raised) atomicExch(p.status, 1u);
     }
     // (a lane a barrier: K and V arrive at one, dO with lse and D at another; slots are freed by the products and by the zeros' warp)
-    const int count = lane == 0 || (lane >= 4 && lane < 11) ? 2 : lane == 13 || lane == 14 ? 256 : lane == 18 && !kRoom<DP> ? 8 : 1;
+    const int count = lane == 0 || (lane >= 4 && lane < 11) ? 2 : lane == 13 || lane == 14 ? kRowThreads : lane == 18 && !kRoom<DP> ? kRowWarps : 1;
     if (lane < 19) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
@@ -868,14 +874,14 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   const int total = *(volatile const int*)p.listed * shares;
   if (fault.raised) {
     __syncthreads();
-    if (warp == 9) tmem_free(tmem, 512);
+    if (warp == kRowWarps + 1) tmem_free(tmem, 512);
     return;
   }
   const uint32_t sk = smem, sv = smem + TB, sq = smem + 2 * TB, sg = smem + 5 * TB;
   const uint32_t tdp = tmem + TILE, tdv = tmem + 2 * TILE, tdk = tmem + 3 * TILE;
   const auto tiles_in = [](const Work& w) { return (w.len + TILE - 1) / TILE; };      // tiles of the sequence; the piece's is number `unit`
 
-  if (warp == 8) {
+  if (warp == kRowWarps) {
     const bool one = elect();
     const auto load_tile = [&](uint32_t dst, const CUtensorMap* m, int row, int h, uint32_t bar) {
       if (one) {
@@ -920,7 +926,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         }
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == kRowWarps + 2) {
     bool ok = true;
     int g = 0;
     for (Walk it; ok && it.next(total);) {
@@ -944,7 +950,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         }
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == kRowWarps + 1) {
     const bool one = elect();
     const int ksteps = (p.D + 15) / 16;
     const uint32_t dscore = product_desc<T>(TILE, TILE, false, false);
@@ -978,7 +984,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     };
     const auto outputs = [&](uint32_t acc, uint32_t a, uint64_t b, bool add) {
 #pragma unroll
-      for (int k = 0; k < TILE / 16; ++k) mma_ts(acc, a + (k >> 2) * 64 + (k & 3) * 8, across(b, k), dout, add || k > 0);
+      for (int k = 0; k < TILE / 16; ++k) mma_ts(acc, a + (k >> 1) * 32 + (k & 1) * 8, across(b, k), dout, add || k > 0);
     };
     bool ok = true;
     int g = 0, pieces = 0;
@@ -1012,13 +1018,14 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       }
     }
   } else {
-    const int half = warp >> 2, r0 = (warp & 3) * 32 + lane;
+    const int quarter = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + half * 64 + lanes, tp = tdp + half * 64 + lanes;
+    const uint32_t ts = tmem + quarter * 32 + lanes, tp = tdp + quarter * 32 + lanes;
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
-    const int first = r0 - half * 64;      // on the diagonal: the first column (query) of this half that sees the row (key)
+    const int first = r0 - quarter * 32;      // on the diagonal: the first column (query) of this quarter that sees the row (key)
     char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
     int g = 0, pieces = 0;
+    const auto meet = [] { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kRowThreads) : "memory"); };
     // (as in the forward pass: the warps may meet at barriers, so none of them leaves)
     for (Walk it; it.next(total);) {
       const Work w = it.work(p, shares);
@@ -1026,25 +1033,24 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       if (w.nothing) {
         if (share % p.split) continue;
         const int rows_here = min(TILE, w.len - tile * TILE);
-        zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, 256);
-        zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, 256);
+        zero_out(p.dk, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, kRowThreads);
+        zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, kRowThreads);
         continue;
       }
 #pragma unroll 1
       for (int i = 0, q = tile; i < n; ++i, ++g) {
-        const float4* l4 = reinterpret_cast<const float4*>(nlse[g & 1] + half * 64);
-        const float4* d4 = reinterpret_cast<const float4*>(ndelta[g & 1] + half * 64);
+        const float4* l4 = reinterpret_cast<const float4*>(nlse[g & 1] + quarter * 32);
+        const float4* d4 = reinterpret_cast<const float4*>(ndelta[g & 1] + quarter * 32);
         const bool diagonal = q == tile;
         if (++q == nt) q = tile;
         bar_wait_warp(gfull + 8 * (g & 1), (g >> 1) & 1, &fault);
         bar_wait_warp(sfull, g & 1, &fault);
         fence_after();
-        uint32_t r[64];
+        uint32_t r[32];
         ld32(ts, r);
-        ld32(ts + 32, r + 32);
         wait_ld(r);
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
+        for (int c = 0; c < 8; ++c) {
           const float4 l = l4[c];
           const float2 a = ex2_pair(fma2(pair(r[4 * c], r[4 * c + 1]), sl2, pair(l.x, l.y)));
           const float2 b = ex2_pair(fma2(pair(r[4 * c + 2], r[4 * c + 3]), sl2, pair(l.z, l.w)));
@@ -1055,24 +1061,23 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         }
         if (diagonal) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
+          for (int c = 0; c < 32; ++c)
             if (c < first) r[c] = 0u;
         }
-        uint32_t o[32];
+        uint32_t o[16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
-        st32(ts, o);
+        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(r[2 * c]), __uint_as_float(r[2 * c + 1]));
+        st16(ts, o);
         wait_st();
         fence_before();
         bar_arrive(pfull);
         bar_wait_warp(dpfull, g & 1, &fault);
         fence_after();
-        uint32_t v[64];
+        uint32_t v[32];
         ld32(tp, v);
-        ld32(tp + 32, v + 32);
         wait_ld(v);
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
+        for (int c = 0; c < 8; ++c) {
           const float4 l = d4[c];
           const float2 a = unpair(mul2(pair(r[4 * c], r[4 * c + 1]), add2(pair(v[4 * c], v[4 * c + 1]), pair(l.x, l.y))));
           const float2 b = unpair(mul2(pair(r[4 * c + 2], r[4 * c + 3]), add2(pair(v[4 * c + 2], v[4 * c + 3]), pair(l.z, l.w))));
@@ -1083,13 +1088,13 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         }
         if (diagonal) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
+          for (int c = 0; c < 32; ++c)
             if (c < first) v[c] = 0u;
-          if (tile == 0 && half == 0) v[0] = 0u;      // (the first query sees one key: its probability is 1)
+          if (tile == 0 && quarter == 0) v[0] = 0u;      // (the first query sees one key: its probability is 1)
         }
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = pack2<T>(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
-        st32(tp, o);
+        for (int c = 0; c < 16; ++c) o[c] = pack2<T>(__uint_as_float(v[2 * c]), __uint_as_float(v[2 * c + 1]));
+        st16(tp, o);
         wait_st();
         fence_before();
         bar_arrive(dsfull);
@@ -1098,50 +1103,55 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       fence_after();
       const int first_row = tile * TILE + (warp & 3) * 32;
       const long long at = ((long long)(w.start + first_row) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
-      const FromTmem dv{tdv + half * (DP / 2) + lanes}, dk{tdk + half * (DP / 2) + lanes};
+      // 32 columns of dV and of dK a warp, at DP = 64 of one of them
+      constexpr int kOutputs = DP / 64;
+      const auto tensor = [&](int k) { return DP == 64 ? quarter >> 1 : k; };
+      const int col = DP == 64 ? (quarter & 1) * 32 : quarter * 32;
       if (p.split == 1) {
-        store_rows<T>(dv, DP / 2, 1.f, stage, p.dv + at, pitch, w.len - first_row, half * (DP / 2), p.D);
-        store_rows<T>(dk, DP / 2, p.scale, stage, p.dk + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+#pragma unroll
+        for (int k = 0; k < kOutputs; ++k) {
+          const bool of_k = tensor(k);
+          store_rows<T>(FromTmem{(of_k ? tdk : tdv) + col + lanes}, 32, of_k ? p.scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
+        }
       } else {
         const int piece = (int)(it.at() / p.split);
-        float* const mine = p.sums + ((long long)piece * p.split + share % p.split) * 2 * DP * TILE + half * (DP / 2) * TILE + r0;
+        float* const sums = p.sums + (long long)piece * p.split * 2 * DP * TILE + col * TILE + r0;
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {      // (dV's columns, then dK's)
+        for (int k = 0; k < kOutputs; ++k) {
           uint32_t r[32];
           __syncwarp();
-          if (c < DP / 2) dv(c, r);
-          else dk(c - DP / 2, r);
-          float* const to = mine + (c < DP / 2 ? c : DP + c - DP / 2) * TILE;
+          FromTmem{(tensor(k) ? tdk : tdv) + col + lanes}(0, r);
+          float* const to = sums + (share % p.split * 2 + tensor(k)) * DP * TILE;
 #pragma unroll
-          for (int i2 = 0; i2 < 32; ++i2) __stcg(to + i2 * TILE, __uint_as_float(r[i2]));
+          for (int c = 0; c < 32; ++c) __stcg(to + c * TILE, __uint_as_float(r[c]));
         }
         // all of the CTA's sums are written before it says so; the last to say so reads all
         __threadfence();
-        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        meet();
         if (threadIdx.x == 0) last_share = atomicAdd(p.arrived + piece, 1) == p.split - 1;
-        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+        meet();
         if (last_share) {
           __threadfence();
-          const float* const all = p.sums + (long long)piece * p.split * 2 * DP * TILE + half * (DP / 2) * TILE + r0;
-          const auto summed = [&](int tensor) {
-            return [&, tensor](int c, uint32_t (&r)[32]) {
+#pragma unroll 1
+          for (int k = 0; k < kOutputs; ++k) {
+            const bool of_k = tensor(k);
+            const auto summed = [&](int, uint32_t (&r)[32]) {
               float f[32];
 #pragma unroll
-              for (int i2 = 0; i2 < 32; ++i2) f[i2] = 0.f;
+              for (int c = 0; c < 32; ++c) f[c] = 0.f;
 #pragma unroll 1
-              for (int k = 0; k < p.split; ++k) {
-                const float* from = all + ((long long)k * 2 + tensor) * DP * TILE + c * TILE;
+              for (int j = 0; j < p.split; ++j) {
+                const float* from = sums + (j * 2 + of_k) * DP * TILE;
 #pragma unroll
-                for (int i2 = 0; i2 < 32; ++i2) f[i2] += __ldcg(from + i2 * TILE);
+                for (int c = 0; c < 32; ++c) f[c] += __ldcg(from + c * TILE);
               }
 #pragma unroll
-              for (int i2 = 0; i2 < 32; ++i2) r[i2] = __float_as_uint(f[i2]);
+              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(f[c]);
             };
-          };
-          store_rows<T>(summed(0), DP / 2, 1.f, stage, p.dv + at, pitch, w.len - first_row, half * (DP / 2), p.D);
-          store_rows<T>(summed(1), DP / 2, p.scale, stage, p.dk + at, pitch, w.len - first_row, half * (DP / 2), p.D);
+            store_rows<T>(summed, 32, of_k ? p.scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
+          }
         }
-        asm volatile("barrier.cta.sync 1, 256;" ::: "memory");      // (last_share is read)
+        meet();      // (last_share is read)
       }
       fence_before();
       if (!kRoom<DP>) {
@@ -1155,7 +1165,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   __syncthreads();
   fence_after();
   if (fault.raised) drain_after_abort();
-  if (warp == 9) tmem_free(tmem, 512);
+  if (warp == kRowWarps + 1) tmem_free(tmem, 512);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1227,7 +1237,7 @@ long long backward_layout(char* base, long long T, int heads, int kv_heads, int 
 
 template <typename T, int DP>
 int run_backward(const CUtensorMap* m, const AttnArgs& p, long long tiles, int sms, cudaStream_t s) {
-  constexpr int kMost = 227 * 1024, kNeed = 7 * DP / 64 * kAtom + (kRoom<DP> ? 8 * 2048 : 0) + 1024;      // (of a CTA, static and dynamic)
+  constexpr int kMost = 227 * 1024, kNeed = 7 * DP / 64 * kAtom + (kRoom<DP> ? kRowWarps * 2048 : 0) + 1024;      // (of a CTA, static and dynamic)
   static std::atomic<unsigned long long> done_q{0}, done_kv{0};
   static std::atomic<int> own{0};      // static shared memory of attn_dkv
   if (!own.load(std::memory_order_relaxed)) {
