@@ -545,7 +545,8 @@ __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_
   }
 }
 
-// At DP = 64 there is room for the outputs' way out beside the tiles; else it leads through the own tiles, whose next loads wait.
+// At DP = 64 there is room for the outputs' way out beside the tiles; else it leads through the second own tile (dO or V), whose
+// next load waits; the first one's (Q or K) does not.
 template <int DP> constexpr bool kRoom = DP == 64;
 
 // A tile of queries against its keys: S = Q K^T, dP = dO V^T, dQ += dS K.
@@ -555,14 +556,14 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[19];
+  __shared__ __align__(8) unsigned long long bars[21];
   __shared__ float part[2][TILE];
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t qfull = bar0, kfull = bar0 + 8, kempty = bar0 + 32, vfull = bar0 + 56, vempty = bar0 + 72, sfull = bar0 + 88,
-                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, qempty = bar0 + 144;
+                 dpfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, qempty = bar0 + 144, gfull = bar0 + 152, gempty = bar0 + 160;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kRowWarps + 1) tmem_alloc(smem_u32(&tmem_), 512);
   if (warp == 0) {
@@ -570,9 +571,9 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       fault.raised = 0;
       fault.status = p.status;
     }
-    // (a lane a barrier: Q and dO arrive at one; the slots of K and V are freed by the products and by the zeros' warp)
-    const int count = lane == 0 || (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 2 : lane == 14 ? kRowThreads : lane == 18 && !kRoom<DP> ? kRowWarps : 1;
-    if (lane < 19) bar_init(bar0 + 8 * lane, count);
+    // (a lane a barrier; the slots of K and V are freed by the products and by the zeros' warp)
+    const int count = (lane >= 4 && lane < 7) || lane == 9 || lane == 10 ? 2 : lane == 14 ? kRowThreads : lane == 20 && !kRoom<DP> ? kRowWarps : 1;
+    if (lane < 21) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
   fence_before();
@@ -604,7 +605,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       const Work w = it.work(p, p.heads);
       const int head = it.head(p.heads), kvh = head / p.group, n = tiles_of(w);
       if (w.nothing) continue;
-      // (the first keys before the queries, whose place may be taken by the last piece's way out)
+      // (dO comes last: its place may be taken by the last piece's way out)
       for (int i = -1; i < n; ++i) {
         if (i >= 0) {
           if (!(ok = bar_wait_warp(vempty + 8 * (g & 1), ((g >> 1) & 1) ^ 1, &fault))) break;
@@ -616,9 +617,11 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
           load_tile(sk + g % 3 * TB, &mk, w.start + (i + 1) * TILE, kvh, kfull + 8 * (g % 3));
         }
         if (i < 0) {
-          if (!(ok = bar_wait_warp(qempty, (pieces++ & 1) ^ 1, &fault))) break;
+          if (!(ok = bar_wait_warp(qempty, (pieces & 1) ^ 1, &fault))) break;
           load_tile(sq, &mq, w.start + (n - 1) * TILE, head, qfull);
-          load_tile(sdo, &mdo, w.start + (n - 1) * TILE, head, qfull);
+        } else if (i == 0) {
+          if (!(ok = bar_wait_warp(gempty, (pieces++ & 1) ^ 1, &fault))) break;
+          load_tile(sdo, &mdo, w.start + (n - 1) * TILE, head, gfull);
         }
       }
     }
@@ -684,7 +687,8 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       const int n = tiles_of(w);
       if (w.nothing) continue;
       ragged = n * TILE > w.len;
-      if (!(ok = bar_wait_warp(qfull, pieces++ & 1, &fault) && scores(g) && dprobs(g) && (n < 2 || scores(g + 1)))) break;
+      if (!(ok = bar_wait_warp(qfull, pieces & 1, &fault) && scores(g) && bar_wait_warp(gfull, pieces & 1, &fault) && dprobs(g) && (n < 2 || scores(g + 1)))) break;
+      ++pieces;
 #pragma unroll 1
       for (int i = 0; i < n; ++i, ++g) {
         if (!(ok = bar_wait_warp(dsfull, g & 1, &fault))) break;
@@ -698,7 +702,8 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
           commit(kempty + 8 * (g % 3));
           if (i + 1 == n) {
             commit(done);
-            if (kRoom<DP>) commit(qempty);
+            commit(qempty);
+            if (kRoom<DP>) commit(gempty);
           }
         }
         __syncwarp();
@@ -709,7 +714,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
     const int quarter = warp >> 2, r0 = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
-    char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
+    char* const stage = smem_p + (kRoom<DP> ? 7 : 1) * TB + warp * 2048;
     int g = 0, pieces = 0;
     // (as in the forward pass: the warps meet at a barrier for every piece, so none of them leaves)
     for (Walk it; it.next(total);) {
@@ -824,7 +829,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       if (!kRoom<DP>) {
         fence_async_proxy();      // (the next load comes over what was written there)
         __syncwarp();
-        if (lane == 0) bar_arrive(qempty);
+        if (lane == 0) bar_arrive(gempty);
       }
     }
   }
@@ -843,7 +848,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
          const __grid_constant__ CUtensorMap mdo, const AttnArgs p) {
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
-  __shared__ __align__(8) unsigned long long bars[19];
+  __shared__ __align__(8) unsigned long long bars[21];
   __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
@@ -851,7 +856,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   char* const smem_p = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t smem = smem_u32(smem_p), bar0 = smem_u32(bars);
   const uint32_t own = bar0, qfull = bar0 + 8, qempty = bar0 + 32, gfull = bar0 + 56, gempty = bar0 + 72, sfull = bar0 + 88,
-                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, free_own = bar0 + 144;
+                 dpfull = bar0 + 96, pfull = bar0 + 104, dsfull = bar0 + 112, done = bar0 + 120, ready = bar0 + 128, free_own = bar0 + 144, vown = bar0 + 152, free_v = bar0 + 160;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kRowWarps + 1) tmem_alloc(smem_u32(&tmem_), 512);
   if (warp == 0) {
@@ -860,9 +865,9 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       fault.status = p.status;
       if (fault.raised) atomicExch(p.status, 1u);
     }
-    // (a lane a barrier: K and V arrive at one, dO with lse and D at another; slots are freed by the products and by the zeros' warp)
-    const int count = lane == 0 || (lane >= 4 && lane < 11) ? 2 : lane == 13 || lane == 14 ? kRowThreads : lane == 18 && !kRoom<DP> ? kRowWarps : 1;
-    if (lane < 19) bar_init(bar0 + 8 * lane, count);
+    // (a lane a barrier: dO arrives with lse and D; slots are freed by the products and by the zeros' warp)
+    const int count = lane >= 4 && lane < 11 ? 2 : lane == 13 || lane == 14 ? kRowThreads : lane == 20 && !kRoom<DP> ? kRowWarps : 1;
+    if (lane < 21) bar_init(bar0 + 8 * lane, count);
     bar_init_done();
   }
   fence_before();
@@ -903,6 +908,10 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         load_tile(sq + s3 * TB, &mq, w.start + q0, head, qfull + 8 * s3);
         if (!(ok = bar_wait_warp(gempty + 8 * s2, ((g >> 1) & 1) ^ 1, &fault))) break;
         load_tile(sg + s2 * TB, &mdo, w.start + q0, head, gfull + 8 * s2);
+        if (i == 0) {
+          if (!(ok = bar_wait_warp(free_own, (pieces & 1) ^ 1, &fault))) break;
+          load_tile(sk, &mk, w.start + w.unit * TILE, kvh, own);
+        }
         // behind the sequence's end P becomes 0
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -915,10 +924,9 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         __syncwarp();
         if (one) bar_arrive(gfull + 8 * s2);
         if (i == 0) {
-          // (behind the first queries, as their place may be taken by the last piece's way out)
-          if (!(ok = bar_wait_warp(free_own, (pieces++ & 1) ^ 1, &fault))) break;
-          load_tile(sk, &mk, w.start + w.unit * TILE, kvh, own);
-          load_tile(sv, &mv, w.start + w.unit * TILE, kvh, own);
+          // (V last: its place may be taken by the last piece's way out)
+          if (!(ok = bar_wait_warp(free_v, (pieces++ & 1) ^ 1, &fault))) break;
+          load_tile(sv, &mv, w.start + w.unit * TILE, kvh, vown);
         }
         if (++q == nt) {
           q = w.unit;
@@ -993,7 +1001,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       const int nt = tiles_in(w), n = (nt - w.unit) * each;
       if (w.nothing) continue;
       ragged = nt * TILE > w.len;      // every head's last tile of queries reaches past the sequence
-      if (!(ok = bar_wait_warp(own, pieces++ & 1, &fault) && scores(g) && dprobs(g))) break;
+      if (!(ok = bar_wait_warp(own, pieces & 1, &fault) && scores(g) && bar_wait_warp(vown, pieces & 1, &fault) && dprobs(g))) break;
+      ++pieces;
 #pragma unroll 1
       for (int i = 0; i < n; ++i, ++g) {
         if (!(ok = bar_wait_warp(pfull, g & 1, &fault))) break;
@@ -1008,7 +1017,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           outputs(tdk, tdp, qt0 + (uint64_t)((g % 3) * (TB >> 4)), i > 0);
           if (i + 1 == n) {
             commit(done);
-            if (kRoom<DP>) commit(free_own);
+            commit(free_own);
+            if (kRoom<DP>) commit(free_v);
           }
         }
         __syncwarp();
@@ -1023,7 +1033,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     const uint32_t ts = tmem + quarter * 32 + lanes, tp = tdp + quarter * 32 + lanes;
     const uint64_t sl2 = pair(p.scale_log2, p.scale_log2);
     const int first = r0 - quarter * 32;      // on the diagonal: the first column (query) of this quarter that sees the row (key)
-    char* const stage = smem_p + (kRoom<DP> ? 7 * TB : 0) + warp * 2048;
+    char* const stage = smem_p + (kRoom<DP> ? 7 : 1) * TB + warp * 2048;
     int g = 0, pieces = 0;
     const auto meet = [] { asm volatile("barrier.cta.sync 1, %0;" ::"n"(kRowThreads) : "memory"); };
     // (as in the forward pass: the warps may meet at barriers, so none of them leaves)
@@ -1157,7 +1167,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       if (!kRoom<DP>) {
         fence_async_proxy();      // (the next load comes over what was written there)
         __syncwarp();
-        if (lane == 0) bar_arrive(free_own);
+        if (lane == 0) bar_arrive(free_v);
       }
     }
   }
