@@ -527,12 +527,13 @@ __device__ __forceinline__ bool fits(const char* end, const char* dynamic) {
 
 // ------------------------------------------------------------------ backward
 // Both kernels: warps 0-15 hold the tile's rows four times, each a quarter of the 128 columns (P and dS of a quarter go over the
-// first half of its scores' columns, so no thread writes where another reads); warp 16 loads, warp 17 issues the products,
-// warp 18 writes the zeros.  Shared memory: the CTA's own two tiles, three slots of the operand that is used by two products
-// and two of the other.  P is made in both (seven products for five): one kernel for all three gradients would add dq with
-// atomics, in an order that changes from run to run.  What bounds them is the chain of two products, exponentials and a third
-// product, and the ends of the pieces (4 x 2048 tokens, 16 heads of 128: dq 119 us, 0.87 PFLOP/s; dkv 135 us, 1.02 PFLOP/s; the
-// tensor pipe is busy 53 and 57 % of the time).
+// first half of its scores' columns, so no thread writes where another reads; with eight warps and halves
+// 8 x 1024 tokens, 16 heads of 64, take 166 us forward and backward for 161); warp 16 loads, warp 17 issues the products, warp 18
+// writes the zeros.  Shared memory: the CTA's own two tiles, three slots of the operand that is used by two products and two of
+// the other.  P is made in both (seven products for five): one kernel for all three gradients would add dq with atomics, in an
+// order that changes from run to run.  What bounds them is the chain of two products, exponentials and a third product, and the
+// ends of the pieces (16 heads of 128, 8192 tokens in sequences of 1024 to 8192: 1.2 us a tile and 39 us in dq, 1.8 us a tile and
+// 27 us in dkv; 4 x 2048: dq 110 us, 0.94 PFLOP/s; dkv 124 us, 1.11 PFLOP/s).
 constexpr int kRowWarps = 16, kRowThreads = kRowWarps * 32, kBwdThreads = kRowThreads + 96;
 
 // 32 scores of a row: P = exp2(scale S - lse)
