@@ -108,9 +108,10 @@ def check_operators(device=None):
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
-    """[T, H, D] whose heads are contiguous and start on 16-byte boundaries (copied if they do not)."""
+    """[T, H, D] whose heads are contiguous and start on 16-byte boundaries (copied if they do not, and where heads or tokens
+    are one in memory, as an expanded tensor's: a tensor map has no stride of zero)."""
     st, sh, one = t.stride()
-    if one == 1 and not ((st | sh) * t.element_size() | t.data_ptr()) & 15:
+    if one == 1 and st and sh and not ((st | sh) * t.element_size() | t.data_ptr()) & 15:
         return t
     return _aligned(t)
 

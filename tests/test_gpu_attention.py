@@ -172,6 +172,23 @@ def test_views_of_one_projection_and_odd_strides(cuda):
     assert torch.equal(dr, torch.cat([t.reshape(T, -1) for t in dx], 1))
 
 
+def test_expanded_inputs_and_gradients(cuda):
+    """Heads or tokens that are one in memory (strides of zero), among queries, keys, values and gradients."""
+    q, k, v, do = (t.detach() for t in make(300, 4, 4, 64, torch.bfloat16, seed=5))
+    for n in range(4):
+        for dim in (0, 1):
+            views = [q, k, v, do]
+            views[n] = views[n].narrow(dim, 0, 1).expand(300, 4, 64)
+            got = [run(*(whole(t) for t in views[:3]), views[3]) for whole in (
+                lambda t: t.detach().requires_grad_(), lambda t: t.contiguous().requires_grad_())]
+            assert all(torch.equal(a, b) for a, b in zip(*got))
+    shared = k[:, :1].clone().requires_grad_()                 # (its gradient: the sum over the heads that it was expanded to)
+    dk, = torch.autograd.grad(chb.causal_attention(q, shared.expand(300, 4, 64), v), shared, do)
+    whole = k[:, :1].expand(300, 4, 64).contiguous().requires_grad_()
+    dw, = torch.autograd.grad(chb.causal_attention(q, whole, v), whole, do)
+    assert torch.equal(dk, dw.sum(1, keepdim=True))
+
+
 def test_no_tokens_and_no_sequences(cuda):
     q, k, v, do = make(0, 4, 2, 64, torch.bfloat16)
     for t in run(q, k, v, do, on_device([0])) + run(q, k, v, do):
