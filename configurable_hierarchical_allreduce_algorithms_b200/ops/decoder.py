@@ -255,27 +255,28 @@ def _attention_forward(q, k, v, cu, scale):
     T, h, d = shape
     hk, seqs = k.shape[1], 0 if cu is None else cu.shape[0] - 1
     o = _new(q)
-    lse = torch.empty((h, T), dtype=torch.float32, device=dev)
-    plan = torch.empty(_plan_bytes(T, h // hk, seqs, cu is not None) if T else 0, dtype=torch.uint8, device=dev)
+    # for the backward pass: the list of work, and behind it the logarithms of the rows' sums, [h, T] fp32
+    side = torch.empty(_plan_bytes(T, h // hk, seqs, cu is not None) + 4 * h * T if T else 0, dtype=torch.uint8, device=dev)
     if T:
+        plan = side.data_ptr()
         q, k, v = _heads(q), _heads(k), _heads(v)
         (a, b, _), (c, e, _), (f, g, _) = q.stride(), k.stride(), v.stride()
         _call("chb_attention_forward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), _eight(a, b, c, e, f, g, 0, 0), T, h, hk, d,
-              None if cu is None else cu.data_ptr(), seqs, scale, o.data_ptr(), lse.data_ptr(), plan.data_ptr())
-    return o, lse, plan, -1 if cu is None else seqs
+              None if cu is None else cu.data_ptr(), seqs, scale, o.data_ptr(), plan + side.shape[0] - 4 * h * T, plan)
+    return o, side, -1 if cu is None else seqs
 
 
 class _CausalAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu, scale):
-        o, lse, plan, seqs = _attention_forward(q, k, v, cu, scale)
-        ctx.save_for_backward(q, k, v, o, lse, plan)      # (the bounds are in the plan)
+        o, side, seqs = _attention_forward(q, k, v, cu, scale)
+        ctx.save_for_backward(q, k, v, o, side)      # (the bounds are in the list of work)
         ctx.args = seqs, scale
         return o
 
     @_first_order
     def backward(ctx, grad):
-        q, k, v, o, lse, plan = ctx.saved_tensors
+        q, k, v, o, side = ctx.saved_tensors
         seqs, scale = ctx.args
         dev = q.device
         T, h, d = q.shape
@@ -287,7 +288,7 @@ class _CausalAttention(torch.autograd.Function):
             bounds, seqs = seqs >= 0, max(seqs, 0)
             work = torch.empty(_backward_bytes(dev, T, h, kv[1], d, bounds, seqs), dtype=torch.uint8, device=dev)
             _call("chb_attention_backward", dev, DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), grad.data_ptr(),
-                  _eight(a, b, c, e, f, g, m, n), lse.data_ptr(), plan.data_ptr(), T, h, kv[1], d, bounds, seqs, scale,
+                  _eight(a, b, c, e, f, g, m, n), side.data_ptr() + side.shape[0] - 4 * h * T, side.data_ptr(), T, h, kv[1], d, bounds, seqs, scale,
                   work.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
         return dq, dk, dv, None, None
 
