@@ -362,7 +362,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       if (w.nothing) continue;
       const Pair x(w, kvh, p.group);
       const int n0 = x.n(0), nu = x.n(u);
-      const uint32_t values = x.ragged() ? vready : vfull;
+      const bool ragged = x.ragged();
       if (nu) {
         if (!(ok = bar_wait_warp(qfull + 8 * u, qn++ & 1, &fault) && bar_wait_warp(kfull + 8 * (g & 1), (g >> 1) & 1, &fault))) break;
         scores(g & 1, nu == 1);
@@ -377,7 +377,9 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
           fence_after();
           scores(s ^ 1, i + 2 == nu);
         }
-        if (!(ok = bar_wait_warp(values + 8 * s, (g >> 1) & 1, &fault))) break;
+        // (the load first, even where the zeros count: the load comes behind the zeros' warp's last turn in this slot, so the phase
+        // of vready that is asked for cannot be taken for the one before the last)
+        if (!(ok = bar_wait_warp(vfull + 8 * s, (g >> 1) & 1, &fault) && (!ragged || bar_wait_warp(vready + 8 * s, (g >> 1) & 1, &fault)))) break;
         if (!(ok = bar_wait_warp(pfull + 8 * u, t & 1, &fault))) break;
         fence_after();
         if (one) {
@@ -662,8 +664,9 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
     // scores of the tile that comes as number i, over the dS of number i - 2
     const auto scores = [&](int i) {
       const int s3 = i % 3;
-      const uint32_t bar = ragged ? ready + 8 * (i & 1) : kfull + 8 * s3;
-      if (!bar_wait_warp(bar, ragged ? (i >> 1) & 1 : (i / 3) & 1, &fault)) return false;
+      // (as in the forward pass: the load of V comes behind the zeros' warp's last turn in the slot of `ready`; K's need not)
+      if (!(ragged ? bar_wait_warp(vfull + 8 * (i & 1), (i >> 1) & 1, &fault) && bar_wait_warp(ready + 8 * (i & 1), (i >> 1) & 1, &fault)
+                   : bar_wait_warp(kfull + 8 * s3, (i / 3) & 1, &fault))) return false;
       if (one) {
         product(tmem + (i & 1) * TILE, aq, k0 + (uint64_t)(s3 * (TB >> 4)));
         commit(sfull + 8 * (i & 1));
@@ -672,7 +675,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       return true;
     };
     const auto dprobs = [&](int i) {
-      if (!bar_wait_warp((ragged ? ready : vfull) + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (!bar_wait_warp(vfull + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;      // (its scores have waited for the zeros)
       if (one) {
         product(tdp, ado, v0 + (uint64_t)((i & 1) * (TB >> 4)));
         commit(dpfull);
@@ -973,8 +976,9 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     bool ragged = false;
     const auto scores = [&](int i) {
       const int s3 = i % 3;
-      const uint32_t bar = ragged ? ready + 8 * (i & 1) : qfull + 8 * s3;
-      if (!bar_wait_warp(bar, ragged ? (i >> 1) & 1 : (i / 3) & 1, &fault)) return false;
+      // (as in the forward pass: the load of dO comes behind the zeros' warp's last turn in the slot of `ready`; Q's need not)
+      if (!(ragged ? bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault) && bar_wait_warp(ready + 8 * (i & 1), (i >> 1) & 1, &fault)
+                   : bar_wait_warp(qfull + 8 * s3, (i / 3) & 1, &fault))) return false;
       if (one) {
         product(tmem, ak, q0 + (uint64_t)(s3 * (TB >> 4)));
         commit(sfull);
@@ -983,7 +987,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       return true;
     };
     const auto dprobs = [&](int i) {
-      if (!bar_wait_warp((ragged ? ready : gfull) + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;
+      if (!bar_wait_warp(gfull + 8 * (i & 1), (i >> 1) & 1, &fault)) return false;      // (its scores have waited for the zeros)
       if (one) {
         product(tdp, av, g0 + (uint64_t)((i & 1) * (TB >> 4)));
         commit(dpfull);
