@@ -182,7 +182,8 @@ int chb_adam_flat(const void* grad, void* master, void* m, void* v, void* param_
 
 /* --------------------------------------------------- operators of a decoder
  * Device pointers throughout; 16-bit operands CHB_BF16 or CHB_F16; strides in elements, multiples of 16 bytes.  All
- * launches go to `stream`; workspaces belong to the call, saved / plan buffers go from forward to backward. */
+ * launches go to `stream`; workspaces belong to the call, saved / plan buffers go from forward to backward.  Tensors, plan,
+ * saved and work lie on 16-byte boundaries (work of chb_linear_ce_backward: 32), the rest on its elements': else CHB_ERR_ARG. */
 /* causal attention: q [T, heads, D], k and v [T, kv_heads, D], D <= 128, a multiple of 8; cu: seqs + 1 bounds (device) or
  * null.  strides: token and head of q, k, v (and dout).  lse: heads * T floats */
 int chb_attention_plan_bytes(long long T, int group, int seqs, int bounds, long long* out);

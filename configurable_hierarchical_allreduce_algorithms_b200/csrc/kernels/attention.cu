@@ -1286,6 +1286,7 @@ int chb_attention_plan_bytes(long long T, int group, int seqs, int bounds, long 
 int chb_attention_forward(int dtype, const void* q, const void* k, const void* v, const long long* strides, long long T, int heads,
                           int kv_heads, int D, const int* cu, int seqs, float scale, void* o, float* lse, void* plan, cudaStream_t stream) {
   if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !strides || !o || !lse || !plan) return CHB_ERR_ARG;
+  if (!on_boundary(16, q, k, v, o, plan) || !on_boundary(8, strides) || !on_boundary(4, cu, lse)) return CHB_ERR_ARG;
   const int group = heads / kv_heads, sms = sm_count();
   const long long pairs = most_units(T, seqs, cu != nullptr, group), tiles = most_units(T, seqs, cu != nullptr, 0);
   if (tiles * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;      // (pieces of work)
@@ -1320,6 +1321,7 @@ int chb_attention_backward(int dtype, const void* q, const void* k, const void* 
                            const float* lse, const void* plan, long long T, int heads, int kv_heads, int D, int bounds, int seqs, float scale,
                            void* work, void* dq, void* dk, void* dv, cudaStream_t stream) {
   if (!args_ok(dtype, T, heads, kv_heads, D, seqs, scale) || !q || !k || !v || !o || !dout || !strides || !lse || !plan || !work || !dq || !dk || !dv) return CHB_ERR_ARG;
+  if (!on_boundary(16, q, k, v, o, dout, plan, work, dq, dk, dv) || !on_boundary(8, strides) || !on_boundary(4, lse)) return CHB_ERR_ARG;
   const int sms = sm_count();
   const long long pairs = most_units(T, seqs, bounds != 0, heads / kv_heads), tiles = most_units(T, seqs, bounds != 0, 0);
   if (tiles * heads > 0x7fffffffll) return CHB_ERR_UNSUPPORTED;

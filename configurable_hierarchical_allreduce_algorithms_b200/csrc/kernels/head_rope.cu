@@ -407,6 +407,8 @@ int chb_head_rope(int dtype, const void* const* x, const void* const* dy, void* 
     low |= (uintptr_t)((d.xt | d.xh | (dy ? d.dt | d.dh : 0)) * size);
   }
   if (low & 15u) return CHB_ERR_ARG;
+  if (!tc::on_boundary(pos64 ? 8 : 4, static_cast<const char*>(pos)) || !tc::on_boundary(4, part)) return CHB_ERR_ARG;
+  if (dw && !tc::on_boundary(w_dtype == CHB_F32 ? 4 : 2, static_cast<const char*>(dw[0]), static_cast<const char*>(dw[1]))) return CHB_ERR_ARG;
   a.w_f32 = half && w && w_dtype == CHB_F32;
   a.pos = pos;
   a.pos64 = pos64;

@@ -804,7 +804,7 @@ int chb_linear_ce_bytes(long long N, int D, int V, long long* saved, long long* 
 int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w, const long long* targets, long long N, int D,
                           int V, long long ignore_index, int reduction, float* loss, void* saved, void* work, cudaStream_t stream) {
   if (!sizes_ok(dtype, N, D, V, reduction) || !x || !w || !targets || !loss || !saved || !work || ldx % 8) return CHB_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15u) return CHB_ERR_ARG;
+  if (!on_boundary(16, x, w, saved, work) || !on_boundary(8, targets) || !on_boundary(4, loss)) return CHB_ERR_ARG;
   Saved sv;
   Fwd f;
   const long long pad = up(N, BM);
@@ -840,8 +840,9 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
 
 int chb_linear_ce_backward(int dtype, const void* w, const float* grad, long long N, int D, int V, int reduction, const void* saved,
                            void* work, void* dx, void* dw, cudaStream_t stream) {
-  if (!sizes_ok(dtype, N, D, V, reduction) || !w || !grad || !saved || !work || (reinterpret_cast<uintptr_t>(w) & 15u)) return CHB_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(dw)) & 15u) return CHB_ERR_ARG;
+  if (!sizes_ok(dtype, N, D, V, reduction) || !w || !grad || !saved || !work) return CHB_ERR_ARG;
+  // (G is stored in words of 32 bytes, at a multiple of 256 in `work`)
+  if (!on_boundary(32, work) || !on_boundary(16, w, saved, dx, dw) || !on_boundary(4, grad)) return CHB_ERR_ARG;
   if (!dx && !dw) return CHB_SUCCESS;
   const int sms = sm_count();
   if (!sms) return CHB_ERR_CUDA;

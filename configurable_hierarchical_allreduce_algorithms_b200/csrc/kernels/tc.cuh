@@ -279,6 +279,13 @@ inline cudaError_t launch_big(K kernel, int smem, unsigned ctas, int threads, cu
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Whether all of these (null included) lie on boundaries of so many bytes: what a kernel reads or writes in words of that size is
+// checked before it is launched, as a misaligned word ends the context.
+template <typename... P>
+inline bool on_boundary(unsigned bytes, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (bytes - 1)) == 0;
+}
+
 // Tiled view of a 16-bit tensor: `dims` extents from the innermost out, strides in elements (of dims 1..), one box of
 // 64 elements x `rows`.  False: the layout cannot be loaded this way.
 bool make_map(CUtensorMap* m, int dtype, const void* base, int ndims, const unsigned long long* dims,
