@@ -569,8 +569,9 @@ ce_join(const float2* part, const float* tlogit, int nt, int rows_pad, int reduc
   if (lane == 0) *loss = (float)(reduction == 1 ? d / count : d);
 }
 
-// Before the backward products: every row's weight relative to the largest, that largest, and zeros in dx where a row has
-// no label.  Every CTA finds the largest for itself (the gradients of the rows are few bytes and in L2).
+// Before the backward products: every row's weight relative to the largest finite one, that largest, and zeros in dx where a row
+// has no label.  Every CTA finds the largest for itself (the gradients of the rows are few bytes and in L2).  A row whose gradient
+// is infinite or NaN keeps that as its weight, so it reaches its own dx (and dW, which sums over all rows) and no other row's.
 __global__ void __launch_bounds__(256)
 ce_weights(const float* grad, int reduction, int N, int D, Saved sv, float* gs, float* coef, char* dx) {
   __shared__ float mx[8];
@@ -582,17 +583,15 @@ ce_weights(const float* grad, int reduction, int N, int D, Saved sv, float* gs, 
     float m = 0.f;
     for (int i = threadIdx.x; i < count; i += 256) {
       const float a = fabsf(grad[sv.idx[i]]);
-      m = a > m || !(a == a) ? a : m;
+      m = a > m && a < INFINITY ? a : m;
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float a = __shfl_xor_sync(0xffffffffu, m, o);
-      m = a > m || !(a == a) ? a : m;
-    }
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) mx[warp] = m;
     __syncthreads();
     top = mx[0];
-    for (int w = 1; w < 8; ++w) top = mx[w] > top || !(mx[w] == mx[w]) ? mx[w] : top;
+    for (int w = 1; w < 8; ++w) top = fmaxf(top, mx[w]);
+    if (top == 0.f) top = 1.f;      // (zeros, infinities and NaN only: they stay what they are)
   } else {
     top = fabsf(*grad) / (reduction == 1 ? (float)count : 1.f);
   }
