@@ -34,7 +34,8 @@ struct Saved {
   int* idx;        // row of x of every gathered row
   int* pos;        // gathered row of every row of x, -1: none
   int* tgt;        // label of every gathered row, -1: not in the vocabulary
-  float* lse2;     // log2 of the sum of exponentials
+  float2* norm;    // largest logit, and log2 of the sum of the exponentials relative to it (one number for both would round by the
+                   // size of the logits: a factor of 2^(1/16) at 2^20, infinity from 2^32 on)
   char* xc;        // gathered rows
 };
 
@@ -50,7 +51,7 @@ struct GemmArgs {
   const int* tgt;
   int rows_pad;
   // GRAD
-  const float* lse2;
+  const float2* norm;
   const float* gs;
   char* g;
   long long ldg;
@@ -244,8 +245,9 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
         const int tg = in ? p.tgt[row] - p.v0 - n0 : -1;
         const int cols = min(bn, p.V - p.v0 - n0);
         float m = -INFINITY, sum = 0.f;
-        float lse = 0.f, gs = 0.f;
-        if (MODE == GRAD && in) { lse = p.lse2[row]; gs = p.gs[row] * GScale<T>::up; }
+        float2 norm = make_float2(0.f, 0.f);
+        float gs = 0.f;
+        if (MODE == GRAD && in) { norm = p.norm[row]; gs = p.gs[row] * GScale<T>::up; }
 #pragma unroll 1
         for (int c = 0; c < bn; c += 32) {
           uint32_t r[32];
@@ -261,11 +263,12 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
             float cm = m;
 #pragma unroll
             for (int j = 0; j < 32; ++j) cm = fmaxf(cm, __uint_as_float(r[j]));
-            const float ref = cm == -INFINITY ? 0.f : cm * kLog2e;
+            // (subtracted ahead of the factor: exact where it matters, whatever the logits' size)
+            const float ref = cm == -INFINITY ? 0.f : cm;
             float add = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) add += ex2(fmaf(__uint_as_float(r[j]), kLog2e, -ref));
-            sum = fmaf(sum, ex2(fmaf(m, kLog2e, -ref)), add);
+            for (int j = 0; j < 32; ++j) add += ex2((__uint_as_float(r[j]) - ref) * kLog2e);
+            sum = fmaf(sum, ex2((m - ref) * kLog2e), add);
             m = cm;
             if ((unsigned)(tg - c) < 32u) {
               float x = 0.f;
@@ -277,7 +280,7 @@ ce_gemm(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensor
             uint32_t o[16];
             float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(__uint_as_float(r[j]), kLog2e, -lse));
+            for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(__uint_as_float(r[j]) - norm.x, kLog2e, -norm.y));
             if ((unsigned)(tg - c) < 32u) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] -= tg - c == j ? 1.f : 0.f;
@@ -543,7 +546,7 @@ ce_join(const float2* part, const float* tlogit, int nt, int rows_pad, int reduc
       for (int w = 0; w < kJoinWarps; ++w) S += ss[w][lane] * ex2((sm[w][lane] - ref) * kLog2e);
       const bool known = label >= 0;
       loss_r = known ? logf(S) + (M - target) : __int_as_float(0x7fffffff);      // (no such label: NaN)
-      sv.lse2[row] = known ? fmaf(M, kLog2e, log2f(S)) : __int_as_float(0x7fffffff);
+      sv.norm[row] = make_float2(known ? M : __int_as_float(0x7fffffff), log2f(S));
       if (reduction == 0) loss[sv.idx[row]] = loss_r;
     }
     if (reduction != 0) {
@@ -632,7 +635,7 @@ long long saved_layout(char* base, long long N, int D, Saved* sv) {
   sv->idx = c.take<int>(pad * 4);
   sv->pos = c.take<int>(pad * 4);
   sv->tgt = c.take<int>(pad * 4);
-  sv->lse2 = c.take<float>(pad * 4);
+  sv->norm = c.take<float2>(pad * 8);
   sv->xc = c.take<char>(pad * D * 2);
   return c.at;
 }
@@ -755,7 +758,7 @@ int backward(int dtype, const char* w, int N, int D, int V, const Saved& sv, con
   GemmArgs p{};
   p.count = sv.head;
   p.V = V; p.D = D;
-  p.tgt = sv.tgt; p.lse2 = sv.lse2; p.gs = b.gs; p.g = b.g; p.ldg = q.width;
+  p.tgt = sv.tgt; p.norm = sv.norm; p.gs = b.gs; p.g = b.g; p.ldg = q.width;
   p.slab_x = b.slab_x; p.slab_w = b.slab_w; p.split_x = q.split_x; p.split_w = q.split_w;
   p.rows_pad = (int)pad;
   p.a_rows = rows_loaded(N);
