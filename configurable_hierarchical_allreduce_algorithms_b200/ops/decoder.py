@@ -5,7 +5,8 @@ grouped heads (``csrc/kernels/attention.cu``), and softmax cross entropy of a li
 
 They take CUDA tensors, run on the current stream of the tensors' device, and get their workspaces from torch's allocator,
 so they can be captured into CUDA graphs (a backward pass, as of every torch operation, only while no eager graph of the
-same leaves is alive).  Results and gradients do not depend on the order in which CTAs run: repeated calls agree bit for bit.  The reference stops at the collectives
+same leaves is alive).  Gradients are first-order and reverse-mode; other derivatives are refused.  Results and gradients do
+not depend on the order in which CTAs run: repeated calls agree bit for bit.  The reference stops at the collectives
 (testing/custom_implementations/work_dir/all_reduce/all_reduce_radix_batch.cpp:202); these are the operators of the
 models whose gradients this package's data-parallel paths move."""
 from __future__ import annotations
@@ -15,6 +16,7 @@ import struct
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _native as N
@@ -92,6 +94,8 @@ def _first_order(backward):
     slow = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            raise NotImplementedError("forward-mode derivatives of a decoder operator's gradients are not implemented")
         return slow(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return staticmethod(run)
@@ -184,6 +188,9 @@ def _rope_rows(device: torch.device, heads_q: int, heads_k: int) -> int:
 
 
 def _wants_grad(*tensors) -> bool:
+    # (inside a level of forward-mode differentiation too: torch refuses a tangent there, which a plain call would drop)
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
