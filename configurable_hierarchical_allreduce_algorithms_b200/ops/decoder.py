@@ -75,6 +75,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    """The same with the strides of its shape (a dimension of one element keeps any stride otherwise)."""
+    return _aligned(t).view(-1).view(t.shape)
+
+
 def _new(t: torch.Tensor) -> torch.Tensor:
     """Uninitialised and contiguous, otherwise like ``t`` (half the time of torch.empty with a shape, type and device)."""
     return _empty_like(t, memory_format=_contiguous)
@@ -85,7 +90,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     row, one = t.stride()
     if one == 1 and row % 8 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
-    return _aligned(t)
+    return _plain(t)
 
 
 def _first_order(backward):
@@ -117,7 +122,7 @@ def _heads(t: torch.Tensor) -> torch.Tensor:
     st, sh, one = t.stride()
     if one == 1 and st and sh and not ((st | sh) * t.element_size() | t.data_ptr()) & 15:
         return t
-    return _aligned(t)
+    return _plain(t)
 
 
 _two = struct.Struct("2Q").pack        # (device pointers as a C array: packed bytes take a tenth of the time of a ctypes array)
