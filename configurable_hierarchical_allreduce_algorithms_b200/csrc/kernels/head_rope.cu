@@ -13,9 +13,7 @@
 // so far positions are as exact as near ones; only the angle within the turn is rounded to fp32.
 #include <math.h>
 
-#include <memory>
 #include <mutex>
-#include <vector>
 
 #include "../api/chb.h"
 #include "common.cuh"
@@ -345,21 +343,26 @@ cudaError_t launch(const RopeArgs& a, const Turns& t, bool interleaved, bool bac
   return interleaved ? launch_order<T, V, true>(a, t, back, sms, s) : launch_order<T, V, false>(a, t, back, sms, s);
 }
 
-// The fractions of a turn for one base and D, kept from call to call (as a program keeps its tables): the last few.
-const Turns& turns_of(double base, int D) {
+// The fractions of a turn for one base and D, kept from call to call (as a program keeps its tables): the last eight that were
+// made, as a base may change with every call.  A copy, as the entry may be overwritten by the next call.
+Turns turns_of(double base, int D) {
+  constexpr unsigned kKept = 8;
   struct Entry { double base; int D; Turns t; };
   static std::mutex mu;
-  static std::vector<std::unique_ptr<Entry>> known;      // (entries stay where they are once made)
+  static Entry known[kKept];
+  static unsigned made = 0;
   std::lock_guard<std::mutex> g(mu);
-  for (const auto& e : known)
-    if (e->base == base && e->D == D) return e->t;
-  std::unique_ptr<Entry> e(new Entry{base, D, {}});
+  for (unsigned i = 0; i < kKept && i < made; ++i)
+    if (known[i].base == base && known[i].D == D) return known[i].t;
+  Entry& e = known[made % kKept];
+  made = made + 1 < 2 * kKept ? made + 1 : kKept;      // (a number of the same remainder: it never wraps)
+  e.base = base;
+  e.D = D;
   for (int i = 0; i < D / 2; ++i) {
     const long double f = powl((long double)base, -2.0L * i / D) / 6.283185307179586476925286766559L;
-    e->t.f[i] = (unsigned long long)ldexpl(f - floorl(f), 64);
+    e.t.f[i] = (unsigned long long)ldexpl(f - floorl(f), 64);
   }
-  known.push_back(std::move(e));
-  return known.back()->t;
+  return e.t;
 }
 
 }  // namespace
@@ -425,7 +428,7 @@ int chb_head_rope(int dtype, const void* const* x, const void* const* dy, void* 
   share_out(&a, sms);
   const int shares = a.side[0].slices + a.side[1].slices;
   if (shares > 65535) return CHB_ERR_UNSUPPORTED;
-  const Turns& t = turns_of(base, D);
+  const Turns t = turns_of(base, D);
   const cudaError_t e = dtype == CHB_F32 ? launch<float, 4>(a, t, in, back, sms, stream)
                         : dtype == CHB_BF16 ? (V == 8 ? launch<__nv_bfloat16, 8>(a, t, in, back, sms, stream) : launch<__nv_bfloat16, 4>(a, t, in, back, sms, stream))
                                             : (V == 8 ? launch<__half, 8>(a, t, in, back, sms, stream) : launch<__half, 4>(a, t, in, back, sms, stream));
@@ -437,7 +440,7 @@ int chb_head_rope(int dtype, const void* const* x, const void* const* dy, void* 
   }
   return CHB_SUCCESS;
 } catch (...) {
-  return CHB_ERR_NO_MEM;      // (the table of angles)
+  return CHB_ERR_OTHER;      // (the lock of the table of angles)
 }
 
 }  // extern "C"
