@@ -94,7 +94,7 @@ class Block(nn.Module):
         llama = self.cfg.style == "llama"
         qkv = self.qkv(self.ln1(x))
         if self.cfg.native:
-            q, k, v = (t.view(B * T, -1, hd) for t in qkv.view(B * T, -1).split([d, kv * hd, kv * hd], dim=1))
+            q, k, v = (t.unflatten(1, (-1, hd)) for t in qkv.view(B * T, d + 2 * kv * hd).split([d, kv * hd, kv * hd], dim=1))
             if llama:
                 norms = (None, None) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
                 q, k = decoder.head_norm_rope(q, k, *norms, pos, eps=self.q_norm.eps if self.q_norm is not None else 1e-5)
@@ -156,10 +156,10 @@ class GPT(nn.Module):
                 mask = (seq[:, None] == seq[None]) & (rows[:, None] >= rows[None])
         elif native:
             pos = rows % T
-            cu = torch.arange(0, B * T + 1, T, device=idx.device, dtype=torch.int32)
+            cu = torch.arange(B + 1, device=idx.device, dtype=torch.int32) * T
         x = self.wte(idx)
         if self.wpe is not None:
-            x = x + (self.wpe(torch.arange(T, device=idx.device)) if cu_seqlens is None else self.wpe(pos.clamp(0, self.cfg.seq_len - 1)).view(B, T, -1))
+            x = x + (self.wpe(torch.arange(T, device=idx.device)) if cu_seqlens is None else self.wpe(pos.clamp(0, self.cfg.seq_len - 1)).view(B, T, self.cfg.d_model))
         for blk in self.blocks:
             x = blk(x, pos, cu, mask)
         x = self.ln_f(x)

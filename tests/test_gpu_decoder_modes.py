@@ -1,4 +1,5 @@
-"""The decoder operators and what torch can do around a call: forward-mode derivatives, a first call inside a capture."""
+"""The decoder operators and what torch can do around a call: forward-mode derivatives, a first call inside a capture,
+batches without tokens."""
 import subprocess
 import sys
 
@@ -7,6 +8,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 import configurable_hierarchical_allreduce_algorithms_b200 as chb
+from configurable_hierarchical_allreduce_algorithms_b200.models.gpt import GPT, GPTConfig
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +68,18 @@ print("captured")
 def test_first_calls_inside_a_capture(cuda):
     r = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("shape", [(2, 0), (0, 8), (0, 0)])
+@pytest.mark.parametrize("style", ["gpt2", "llama"])
+def test_batches_without_tokens(cuda, style, shape):
+    cfg = GPTConfig.tiny(style)
+    cfg.native = True
+    model = GPT(cfg).cuda().bfloat16()
+    idx = torch.zeros(shape, dtype=torch.long, device="cuda")
+    assert model(idx).shape == (*shape, cfg.vocab)
+    loss = model(idx, idx)
+    loss.backward()
+    assert loss.isnan()
+    cu = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert model(idx, cu_seqlens=cu).shape == (*shape, cfg.vocab)
