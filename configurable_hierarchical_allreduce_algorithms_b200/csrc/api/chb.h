@@ -205,8 +205,10 @@ int chb_linear_ce_forward(int dtype, const void* x, long long ldx, const void* w
                           long long ignore_index, int reduction, float* loss, void* saved, void* work, chb_stream_t stream);
 int chb_linear_ce_backward(int dtype, const void* w, const float* grad, long long N, int D, int V, int reduction, const void* saved,
                            void* work, void* dx, void* dw, chb_stream_t stream);
-/* synchronises the stream; 0, or 1 after a bounded wait inside one of these kernels ran out; cleared by the call */
+/* synchronises the stream; 1 if a bounded wait inside one of these kernels ran out since the last call, else 0 */
 int chb_matrix_status(unsigned* out, chb_stream_t stream);
+/* as if a wait had run out, for tests of what a program does then */
+int chb_matrix_status_raise(chb_stream_t stream);
 
 int chb_dtype_size(int dtype);
 const char* chb_version(void);

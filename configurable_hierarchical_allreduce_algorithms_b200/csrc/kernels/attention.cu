@@ -867,7 +867,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
     if (lane == 31) {
       fault.raised = !fits(smem_p + 7 * TB + (kRoom<DP> ? kRowWarps * 2048 : 0), smem_raw);
       fault.status = p.status;
-      if (fault.raised) atomicExch(p.status, 1u);
+      if (fault.raised) atomicAdd(p.status, 1u);
     }
     // (a lane a barrier: dO arrives with lse and D; slots are freed by the products and by the zeros' warp)
     const int count = lane >= 4 && lane < 11 ? 2 : lane == 13 || lane == 14 ? kRowThreads : lane == 20 && !kRoom<DP> ? kRowWarps : 1;

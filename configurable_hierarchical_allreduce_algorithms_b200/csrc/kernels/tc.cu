@@ -1,4 +1,4 @@
-// Host side of the matrix kernels: tensor maps, and the status word that an expired wait leaves.
+// Host side of the matrix kernels: tensor maps, and the status word in which expired waits are counted.
 #include "tc.cuh"
 
 #include <mutex>
@@ -10,6 +10,11 @@ namespace tc {
 
 namespace {
 __device__ unsigned int g_status = 0;
+__global__ void count_a_fault() { atomicAdd(&g_status, 1u); }
+
+constexpr int kDevices = 64;
+std::mutex status_mu;
+unsigned status_seen[kDevices];      // what the host was told of
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -53,7 +58,6 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int ndims, const unsi
 }
 
 unsigned* status_word() {
-  constexpr int kDevices = 64;
   static std::mutex mu;
   static unsigned* known[kDevices] = {};
   int dev = 0;
@@ -68,7 +72,6 @@ unsigned* status_word() {
 }
 
 int sm_count() {
-  constexpr int kDevices = 64;
   static std::atomic<int> known[kDevices];
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
@@ -90,12 +93,26 @@ bool allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& 
 }  // namespace tc
 }  // namespace chb
 
-// Status of the matrix kernels on the current device (synchronises the stream): 0, or 1 after a wait ran out; cleared.
-extern "C" int chb_matrix_status(unsigned* out, cudaStream_t stream) {
-  unsigned* p = chb::tc::status_word();
-  if (!p || !out) return CHB_ERR_ARG;
-  if (cudaMemcpyAsync(out, p, sizeof(unsigned), cudaMemcpyDeviceToHost, stream) != cudaSuccess ||
-      cudaMemsetAsync(p, 0, sizeof(unsigned), stream) != cudaSuccess || cudaStreamSynchronize(stream) != cudaSuccess)
+// Status of the matrix kernels on the current device (synchronises the stream): 1 if a wait ran out since the last call, else 0.
+// The device only counts, and the host remembers how far it has read: a wait that runs out on another stream meanwhile is either
+// in what this call reads or left for the next one.
+extern "C" int chb_matrix_status(unsigned* out, cudaStream_t stream) try {
+  using namespace chb::tc;
+  unsigned* p = status_word();
+  int dev = 0;
+  if (!p || !out || cudaGetDevice(&dev) != cudaSuccess) return CHB_ERR_ARG;
+  std::lock_guard<std::mutex> g(status_mu);
+  unsigned now = 0;
+  if (cudaMemcpyAsync(&now, p, sizeof(unsigned), cudaMemcpyDeviceToHost, stream) != cudaSuccess || cudaStreamSynchronize(stream) != cudaSuccess)
     return CHB_ERR_CUDA;
+  *out = now != status_seen[dev];
+  status_seen[dev] = now;
   return CHB_SUCCESS;
+} catch (...) {
+  return CHB_ERR_OTHER;
+}
+
+extern "C" int chb_matrix_status_raise(cudaStream_t stream) {
+  chb::tc::count_a_fault<<<1, 1, 0, stream>>>();
+  return cudaGetLastError() == cudaSuccess ? CHB_SUCCESS : CHB_ERR_CUDA;
 }

@@ -7,7 +7,7 @@
 // along the summed axis: 16 of them are 2048 bytes, and the next 64 elements of the other axis lie one tile further.
 //
 // Waits.  Every wait ends: after kWaitLimitNs the waiting thread raises the CTA's fault, which ends all other waits of the
-// CTA, and records it in the device's status word, which the host can read.
+// CTA, and counts it in the device's status word, which the host can read.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -25,7 +25,7 @@ constexpr unsigned long long kWaitLimitNs = 4000000000ull;
 // In shared memory: raised once a wait of the CTA ran out, and where the host finds out.
 struct Fault {
   volatile unsigned raised;
-  unsigned* status;      // the device's status word: 0, or 1 after a wait of a matrix kernel ran out
+  unsigned* status;      // the device's status word: waits of matrix kernels that ran out, since the library was loaded
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -68,7 +68,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, unsigned parity, Fault* f
     }
   }
   fault->raised = 1;
-  atomicExch(fault->status, 1u);
+  atomicAdd(fault->status, 1u);
   return false;
 }
 // The same by a whole warp, with one answer for all its lanes (what follows is often a warp-wide instruction).

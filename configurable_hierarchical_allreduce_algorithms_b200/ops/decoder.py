@@ -24,6 +24,7 @@ from ..parallel.comm import DTYPES
 
 vp, i32, i64, f32 = C.c_void_p, C.c_int, C.c_longlong, C.c_float
 N.optional("chb_matrix_status", i32, [C.POINTER(C.c_uint), vp])
+N.optional("chb_matrix_status_raise", i32, [vp])
 N.optional("chb_linear_ce_bytes", i32, [i64, i32, i32, C.POINTER(i64), C.POINTER(i64), C.POINTER(i64)])
 N.optional("chb_linear_ce_forward", i32, [i32, vp, i64, vp, vp, i64, i32, i32, i64, i32, vp, vp, vp, vp])
 N.optional("chb_linear_ce_backward", i32, [i32, vp, vp, i64, i32, i32, i32, vp, vp, vp, vp, vp])
@@ -107,9 +108,13 @@ def _first_order(backward):
 
 
 def check_operators(device=None):
-    """Synchronise the current stream and raise :class:`OperatorError` if a bounded wait inside a matrix kernel of this
-    module ran out since the last call (its outputs are not to be used then)."""
-    device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
+    """Synchronise the current stream of ``device`` (None, or "cuda" without a number: the current device) and raise
+    :class:`OperatorError` if a bounded wait inside a matrix kernel of this module ran out there since the last call (what was
+    computed since then is not to be used)."""
+    device = torch.device("cuda" if device is None else device)
+    _need(device.type == "cuda", "check_operators: a CUDA device expected")
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     word = C.c_uint(0)
     _call("chb_matrix_status", device, C.byref(word))
     if word.value:
