@@ -23,6 +23,7 @@ import torch
 import torch.distributed as dist
 
 from ..models.gpt import GPT, GPTConfig
+from ..ops.decoder import check_operators
 from ..parallel.comm import Communicator
 from ..parallel.ddp import DataParallel, FusedMasterAdamW, MasterAdamW
 from ..parallel.zero import ShardedAdamW
@@ -131,6 +132,8 @@ def main(argv=None):
     ms = float(t.item()) / args.steps
     if comm:
         comm.check()
+    if args.native:
+        check_operators()       # (a wait that ran out: neither the loss nor the weights are to be used)
     out = None
     if rank == 0:
         out = {

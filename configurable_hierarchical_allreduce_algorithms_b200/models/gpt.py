@@ -4,7 +4,9 @@ Llama style block (RMSNorm, SwiGLU, rotary positions).  GEMMs go to the vendor
 libraries through PyTorch; this library's kernels are the collectives and the
 fused optimizer / gradient steps around them and, with ``native=True`` (bf16 or
 fp16 parameters on a GPU), causal attention, the head norm with the rotation, and
-the loss of the output layer (``ops/decoder.py``)."""
+the loss of the output layer (``ops/decoder.py``).  A program that runs these
+asks ``check_operators()`` before it uses a result or writes a checkpoint, as it
+asks the communicator: both synchronise."""
 from __future__ import annotations
 
 from dataclasses import dataclass
