@@ -422,7 +422,9 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
       }
       const int nu = x.n(u);
       if (!nu) continue;
-      float ref = 0.f;                       // the maximum that the sums are relative to, times scale log2 e
+      // The maximum that the sums are relative to, times scale log2 e.  Rows behind the sequence's end hold the next one's queries:
+      // at infinity they never ask for the tile's maxima to be moved (which would change this sequence's rounding).
+      float ref = (nu - 1) * TILE + r0 < x.len ? 0.f : INFINITY;
       uint64_t sum2[2] = {0ull, 0ull};       // (two zeros each)
       // The warps of a tile meet at barriers that cannot give up, so none of them leaves the loops: once a wait ran out all
       // waits end at once, and the turns that are left go over whatever the scores hold.
@@ -458,7 +460,7 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
           const float both = fmaxf(top, joint[(half ^ 1) * TILE + r0]);
           sync_tile(u);
           if (left == nu) {
-            ref = both == -INFINITY ? 0.f : both;
+            if (ref == 0.f) ref = both == -INFINITY ? 0.f : both;
           } else {
             // (the output rests: the products of the tile before are done, as the scores' commit came behind them or odone says so)
             fence_after();

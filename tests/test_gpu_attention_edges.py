@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_attention import make, run
+from test_gpu_attention import bounds, make, on_device, run
 
 pytestmark = pytest.mark.gpu
 
@@ -19,3 +19,20 @@ def test_one_token_of_odd_strides(cuda):
         odd.append(rows.as_strided(t.shape, (t.numel() + 3, 64, 1)))
     odd[:3] = [t.detach().requires_grad_() for t in odd[:3]]
     assert all(torch.equal(a, b) for a, b in zip(run(*odd), want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_neighbours_change_no_rounding(cuda, dtype, d):
+    """The next sequence's queries lie in this one's last tile; what they are changes no bit of this one's results."""
+    lens = [300, 200]
+    q, k, v, do = make(500, 4, 2, d, dtype, seed=6)
+    with torch.no_grad():
+        k[:300] *= torch.linspace(0.5, 2, 300, device="cuda")[:, None, None]      # (maxima that grow by less than 2^8)
+    cu = on_device(bounds(lens))
+    want = run(q, k, v, do, cu)
+    with torch.no_grad():
+        for t in (q, k, v, do):
+            t[300:] *= 100
+    for a, b in zip(run(q, k, v, do, cu), want):
+        assert torch.equal(a[:300], b[:300])
