@@ -460,7 +460,8 @@ attn_forward(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUt
           const float both = fmaxf(top, joint[(half ^ 1) * TILE + r0]);
           sync_tile(u);
           if (left == nu) {
-            if (ref == 0.f) ref = both == -INFINITY ? 0.f : both;
+            // (no key with a weight yet: so low that any score moves it, and finite, as infinities have no difference)
+            if (ref == 0.f) ref = both == -INFINITY ? -1.7e38f : both;
           } else {
             // (the output rests: the products of the tile before are done, as the scores' commit came behind them or odone says so)
             fence_after();

@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from test_gpu_attention import bounds, make, on_device, run
+import configurable_hierarchical_allreduce_algorithms_b200 as chb
+from test_gpu_attention import bounds, formula, make, on_device, run
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +37,17 @@ def test_large_neighbours_change_no_rounding(cuda, dtype, d):
             t[300:] *= 100
     for a, b in zip(run(q, k, v, do, cu), want):
         assert torch.equal(a[:300], b[:300])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_ruled_out_by_infinities(cuda, dtype, d):
+    """A document whose first keys are padding, ruled out by minus infinity in one place: whole tiles without a weight."""
+    q, k, v, _ = make(400, 2, 1, d, dtype, seed=7)
+    q, k, v = q.detach(), k.detach(), v.detach()
+    q[..., 0], q[..., 1] = 1, 30
+    k[:150, :, 0], k[150:, :, 0], k[150:, :, 1] = -float("inf"), 0, -30
+    got = chb.causal_attention(q, k, v)
+    want, tol = formula(q[150:], k[150:], v[150:], torch.zeros_like(q[150:]), [0, 250], d ** -0.5)
+    assert ((got[150:].double() - want[0]).abs() <= tol[0]).all()
+    assert got[:150].isnan().all()                               # (no key at all)
