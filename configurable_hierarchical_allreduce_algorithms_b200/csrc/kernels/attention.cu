@@ -24,7 +24,9 @@
 // Rows outside all sequences get zeros.  A tile that reaches past its sequence holds the next one's rows: those are overwritten with zeros
 // where they would be summed over (a product 0 * infinity would carry them across).
 //
-// P and dS are rounded to the operands' type (as the tensor cores need them); maxima, sums, lse and D are fp32.
+// P and dS are rounded to the operands' type (as the tensor cores need them); maxima, sums, lse and D are fp32.  An fp16 dS is kept
+// 2^k times larger, with k from the sizes of the dO and V that go into it (Range below): dO may be near either end of fp16's range
+// (scaled losses, gradients of a mean over many tokens), where dS would be infinite or zero and dQ and dK, which sum it, are not.
 #include "../api/chb.h"
 #include "common.cuh"
 #include "tc.cuh"
@@ -45,6 +47,9 @@ struct AttnArgs {
   char* o;                // [T, heads, D] (written by forward, read by dq)
   float* lse;             // [heads, T], in units of log2
   float* delta;           // [heads, T]
+  float2* sizes;          // fp16: [kv_heads, T], at the first row of every tile the largest |dO_i| (of the group) and |V_j| there
+  const char* v;          // for the sizes
+  long long v_t, v_h;
   const char* dout;       // strides in elements
   long long dout_t, dout_h;
   char *dq, *dk, *dv;     // contiguous
@@ -551,6 +556,91 @@ __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_
   }
 }
 
+// The range of dS.  |P (dP - D)| is at most 2 max|dO_i| max|V_j| (lengths of rows; D is a mean of dP), over the rows that a piece
+// multiplies; 2^k brings that bound to 2^14 to 2^15.  A bound by rows' lengths is about sqrt(D) above what dP reaches, which leaves
+// 13 bits of normal numbers below a dS of 1/2048 of the largest dP.  Sequences have ranges of their own.  Exact: the power is
+// taken out again from fp32 sums.  Only fp16 has it (bf16 has the exponents of fp32).
+template <typename T> constexpr bool kRanged = false;
+template <> constexpr bool kRanged<__half> = true;
+
+struct Range {
+  float o = 0.f, v = 0.f;
+  // sizes of tile `u` of the sequence at `at`
+  __device__ __forceinline__ void take(const float2* at, int u, bool queries, bool keys) {
+    const float2 s = __ldcg(at + (long long)u * TILE);
+    if (queries) o = fmaxf(o, s.x);
+    if (keys) v = fmaxf(v, s.y);
+  }
+  // k, from all lanes' tiles
+  __device__ __forceinline__ int power() const {
+    const float a = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(o)));
+    const float b = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+    const float most = 2.f * a * b;
+    return most > 0.f ? 14 + 127 - (int)(__float_as_uint(most) >> 23) : 0;
+  }
+};
+__device__ __forceinline__ float power_of_two(int k) { return __uint_as_float((unsigned)(127 + k) << 23); }      // |k| < 127
+// dP - D, of the range; nd: -D, of the range already
+template <typename T>
+__device__ __forceinline__ uint64_t less(uint64_t dp, uint64_t nd, float power) {
+  return kRanged<T> ? fma2(dp, pair(power, power), nd) : add2(dp, nd);
+}
+
+// The sizes: CTA = a listed tile and a key head, 8 or 16 lanes a row, rows of V behind those of the group's dO.  Rows that hold
+// infinities or NaN have no size: what they make of their own dS needs no range.  Reads dO and V once: 8191 tokens, 16 / 4 heads
+// of 128, 42 MB; the pass costs that case 18 us of 286 on the device (as much with eight loads in flight, or 1024 threads).
+constexpr int kSizesThreads = 512, kSizesLoads = 4;
+__global__ void __launch_bounds__(kSizesThreads) attn_sizes(const AttnArgs p) {
+  __shared__ float most[2][kSizesThreads / 32];
+  dependent_launch();
+  if ((int)blockIdx.x >= *(volatile const int*)p.listed * p.kv_heads) return;
+  const int4 e = p.list[blockIdx.x / p.kv_heads];
+  const int kvh = blockIdx.x % p.kv_heads, first = e.x + e.z * TILE, rows = min(TILE, e.y - e.z * TILE), each = p.group + 1;
+  if (e.w) return;
+  const int lanes = p.D <= 64 ? 8 : 16, sub = threadIdx.x / lanes, per = kSizesThreads / lanes, col = threadIdx.x % lanes * 8;
+  float o = 0.f, v = 0.f;
+  for (int i0 = sub; i0 - sub < rows * each; i0 += per * kSizesLoads) {
+    uint4 x[kSizesLoads];
+#pragma unroll
+    for (int j = 0; j < kSizesLoads; ++j) {
+      const int i = i0 + j * per, row = i / each, head = i - row * each;
+      x[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows && col < p.D) {
+        const long long at = head < p.group ? (first + row) * p.dout_t + (kvh * p.group + head) * p.dout_h : (first + row) * p.v_t + kvh * p.v_h;
+        x[j] = __ldcg(reinterpret_cast<const uint4*>((head < p.group ? p.dout : p.v) + (at + col) * 2));
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kSizesLoads; ++j) {
+      const uint32_t r[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2<__half>(r[k]);
+        s = fmaf(f.x, f.x, fmaf(f.y, f.y, s));
+      }
+      for (int d = lanes / 2; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+      if (s < INFINITY) {
+        if ((i0 + j * per) % each < p.group) o = fmaxf(o, s);
+        else v = fmaxf(v, s);
+      }
+    }
+  }
+  o = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(o)));
+  v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+  if (threadIdx.x % 32 == 0) {
+    most[0][threadIdx.x / 32] = o;
+    most[1][threadIdx.x / 32] = v;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < kSizesThreads / 32; ++i) {
+    o = fmaxf(o, most[0][i]);
+    v = fmaxf(v, most[1][i]);
+  }
+  p.sizes[(long long)kvh * p.T + first] = make_float2(sqrtf(o), sqrtf(v));
+}
+
 // At DP = 64 there is room for the outputs' way out beside the tiles; else it leads through the second own tile (dO or V), whose
 // next load waits; the first one's (Q or K) does not.
 template <int DP> constexpr bool kRoom = DP == 64;
@@ -733,6 +823,9 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       }
       const bool in = row < w.len;
       const long long at = (long long)head * p.T + w.start + row;
+      Range range;
+      const float2* const sizes = p.sizes + (long long)(head / p.group) * p.T + w.start;
+      if (kRanged<T> && lane <= tile) range.take(sizes, lane, lane == tile, true);
       // D.  A piece with one tile of keys has all of P and dP at once and sums them (below): with few keys the rounding of O
       // would weigh (sequences of two tokens, bf16: dQ off by 0.0036 of its norm, 0.0026 like this).  Else D = dO . O, eight rows
       // a warp, a row to kLanes lanes, so that a load takes whole rows.
@@ -772,6 +865,11 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
         meet();      // (for the next use)
         if (in && quarter == 0) p.delta[at] = delta;
       }
+      float power = 1.f;
+      if (kRanged<T>) {
+        for (int u = lane + 32; u <= tile; u += 32) range.take(sizes, u, u == tile, true);
+        power = power_of_two(range.power());
+      }
       const uint64_t nlse2 = pair(-lse, -lse);
 #pragma unroll 1
       for (int i = 0; i < n; ++i, ++g) {
@@ -804,10 +902,10 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
           meet();
           if (in && quarter == 0) p.delta[at] = delta;
         }
-        const uint64_t ndelta2 = pair(-delta, -delta);
+        const uint64_t ndelta2 = kRanged<T> ? pair(-delta * power, -delta * power) : pair(-delta, -delta);
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
-          const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), add2(pair(v[2 * c], v[2 * c + 1]), ndelta2)));
+          const float2 t = unpair(mul2(pair(r[2 * c], r[2 * c + 1]), less<T>(pair(v[2 * c], v[2 * c + 1]), ndelta2, power)));
           v[2 * c] = __float_as_uint(t.x);
           v[2 * c + 1] = __float_as_uint(t.y);
         }
@@ -830,7 +928,7 @@ attn_dq(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensor
       fence_after();
       const int first = tile * TILE + (warp & 3) * 32;
       if (quarter * 32 < DP)
-        store_rows<T>(FromTmem{tdq + quarter * 32 + lanes}, 32, p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
+        store_rows<T>(FromTmem{tdq + quarter * 32 + lanes}, 32, kRanged<T> ? p.scale / power : p.scale, stage, p.dq + ((long long)(w.start + first) * p.heads + head) * p.D * 2,
                       (long long)p.heads * p.D * 2, w.len - first, quarter * 32, p.D);
       fence_before();
       if (!kRoom<DP>) {
@@ -856,7 +954,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[21];
-  __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D
+  __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D (times the range's power)
+  __shared__ float power_[2];                                         // that power
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   __shared__ int last_share;
@@ -909,6 +1008,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       const Work w = it.work(p, shares);
       const int share = it.head(shares), kvh = share / p.split, nt = tiles_in(w), n = (nt - w.unit) * each;
       if (w.nothing) continue;
+      float power = 1.f;
       for (int i = 0, head = share * each, q = w.unit; i < n; ++i, ++g) {
         const int s3 = g % 3, s2 = g & 1, q0 = q * TILE;
         if (!(ok = bar_wait_warp(qempty + 8 * s3, ((g / 3) & 1) ^ 1, &fault))) break;
@@ -919,14 +1019,20 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           if (!(ok = bar_wait_warp(free_own, (pieces & 1) ^ 1, &fault))) break;
           load_tile(sk, &mk, w.start + w.unit * TILE, kvh, own);
         }
+        if (kRanged<T> && i == 0) {
+          Range range;
+          for (int u = lane; u < nt; u += 32) range.take(p.sizes + (long long)kvh * p.T + w.start, u, u >= w.unit, true);
+          power = power_of_two(range.power());
+        }
         // behind the sequence's end P becomes 0
+        if (kRanged<T> && one) power_[s2] = power;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = lane + 32 * j;
           const long long at = (long long)head * p.T + w.start + q0 + r;
           const bool in = q0 + r < w.len;
           nlse[s2][r] = in ? -__ldcg(p.lse + at) : -INFINITY;
-          ndelta[s2][r] = in ? -__ldcg(p.delta + at) : 0.f;
+          ndelta[s2][r] = in ? -__ldcg(p.delta + at) * power : 0.f;
         }
         __syncwarp();
         if (one) bar_arrive(gfull + 8 * s2);
@@ -1055,6 +1161,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         zero_out(p.dv, w.start + tile * TILE, rows_here, p.kv_heads, kvh, p.D, kRowThreads);
         continue;
       }
+      float power = 1.f;
 #pragma unroll 1
       for (int i = 0, q = tile; i < n; ++i, ++g) {
         const float4* l4 = reinterpret_cast<const float4*>(nlse[g & 1] + quarter * 32);
@@ -1062,6 +1169,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         const bool diagonal = q == tile;
         if (++q == nt) q = tile;
         bar_wait_warp(gfull + 8 * (g & 1), (g >> 1) & 1, &fault);
+        if (kRanged<T>) power = power_[g & 1];
         bar_wait_warp(sfull, g & 1, &fault);
         fence_after();
         uint32_t r[32];
@@ -1097,8 +1205,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const float4 l = d4[c];
-          const float2 a = unpair(mul2(pair(r[4 * c], r[4 * c + 1]), add2(pair(v[4 * c], v[4 * c + 1]), pair(l.x, l.y))));
-          const float2 b = unpair(mul2(pair(r[4 * c + 2], r[4 * c + 3]), add2(pair(v[4 * c + 2], v[4 * c + 3]), pair(l.z, l.w))));
+          const float2 a = unpair(mul2(pair(r[4 * c], r[4 * c + 1]), less<T>(pair(v[4 * c], v[4 * c + 1]), pair(l.x, l.y), power)));
+          const float2 b = unpair(mul2(pair(r[4 * c + 2], r[4 * c + 3]), less<T>(pair(v[4 * c + 2], v[4 * c + 3]), pair(l.z, l.w), power)));
           v[4 * c] = __float_as_uint(a.x);
           v[4 * c + 1] = __float_as_uint(a.y);
           v[4 * c + 2] = __float_as_uint(b.x);
@@ -1119,6 +1227,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       }
       bar_wait_warp(done, pieces++ & 1, &fault);
       fence_after();
+      const float scale = kRanged<T> ? p.scale / power : p.scale;      // (exact: a power of two)
       const int first_row = tile * TILE + (warp & 3) * 32;
       const long long at = ((long long)(w.start + first_row) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
       // 32 columns of dV and of dK a warp, at DP = 64 of one of them
@@ -1129,7 +1238,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
         for (int k = 0; k < kOutputs; ++k) {
           const bool of_k = tensor(k);
-          store_rows<T>(FromTmem{(of_k ? tdk : tdv) + col + lanes}, 32, of_k ? p.scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
+          store_rows<T>(FromTmem{(of_k ? tdk : tdv) + col + lanes}, 32, of_k ? scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
         }
       } else {
         const int piece = (int)(it.at() / p.split);
@@ -1166,7 +1275,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
               for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(f[c]);
             };
-            store_rows<T>(summed, 32, of_k ? p.scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
+            store_rows<T>(summed, 32, of_k ? scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
           }
         }
         meet();      // (last_share is read)
@@ -1239,7 +1348,7 @@ int head_shares(long long tiles, int kv_heads, int group, int sms) {
   return n;
 }
 
-struct BackwardWork { float* delta; int* arrived; float* sums; };
+struct BackwardWork { float* delta; float2* sizes; int* arrived; float* sums; };
 long long backward_layout(char* base, long long T, int heads, int kv_heads, int D, long long tiles, int split, BackwardWork* w) {
   long long at = 0;
   const auto take = [&](long long bytes) {
@@ -1248,6 +1357,7 @@ long long backward_layout(char* base, long long T, int heads, int kv_heads, int 
     return r;
   };
   w->delta = reinterpret_cast<float*>(take(4 * heads * T));
+  w->sizes = reinterpret_cast<float2*>(take(8 * kv_heads * T));      // (few bytes, so bf16 has them too)
   w->arrived = reinterpret_cast<int*>(take(split > 1 ? 4 * tiles * kv_heads : 0));
   w->sums = reinterpret_cast<float*>(take(split > 1 ? tiles * kv_heads * split * 2 * (D <= 64 ? 64 : 128) * TILE * 4 : 0));
   return at;
@@ -1264,6 +1374,7 @@ int run_backward(const CUtensorMap* m, const AttnArgs& p, long long tiles, int s
     own.store((int)f.sharedSizeBytes, std::memory_order_relaxed);
   }
   const int left = kMost - own.load(std::memory_order_relaxed);
+  if (kRanged<T> && launch_overlapped(attn_sizes, dim3((unsigned)(tiles * p.kv_heads)), dim3(kSizesThreads), s, p) != cudaSuccess) return CHB_ERR_CUDA;
   if (launch_big(attn_dq<T, DP>, kNeed, ctas(tiles * p.heads, sms), kBwdThreads, s, done_q, m[0], m[1], m[2], m[3], p) != cudaSuccess ||
       launch_big(attn_dkv<T, DP>, kNeed < left ? kNeed : left, ctas(tiles * p.kv_heads * p.split, sms), kBwdThreads, s, done_kv, m[0], m[1], m[2], m[3], p) != cudaSuccess)
     return CHB_ERR_CUDA;
@@ -1338,6 +1449,10 @@ int chb_attention_backward(int dtype, const void* q, const void* k, const void* 
   p.split = head_shares(tiles, kv_heads, heads / kv_heads, sms);
   backward_layout(static_cast<char*>(work), T, heads, kv_heads, D, tiles, p.split, &bw);
   p.delta = bw.delta;
+  p.sizes = bw.sizes;
+  p.v = static_cast<const char*>(v);
+  p.v_t = strides[4];
+  p.v_h = strides[5];
   p.arrived = bw.arrived;
   p.sums = bw.sums;
   p.pieces = (int)(tiles * kv_heads);

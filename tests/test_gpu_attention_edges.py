@@ -4,9 +4,14 @@ import pytest
 import torch
 
 import configurable_hierarchical_allreduce_algorithms_b200 as chb
-from test_gpu_attention import bounds, formula, make, on_device, run
+from test_gpu_attention import bounds, check, formula, make, on_device, run
 
 pytestmark = pytest.mark.gpu
+
+
+def in_eighths(t):
+    """Multiples of 1/8, at most 2: any power of two times them is exact from 2^-21 on."""
+    return (t.detach().float().clamp(-2, 2) * 8).round().div(8)
 
 
 def test_one_token_of_odd_strides(cuda):
@@ -51,3 +56,48 @@ def test_keys_ruled_out_by_infinities(cuda, dtype, d):
     want, tol = formula(q[150:], k[150:], v[150:], torch.zeros_like(q[150:]), [0, 250], d ** -0.5)
     assert ((got[150:].double() - want[0]).abs() <= tol[0]).all()
     assert got[:150].isnan().all()                               # (no key at all)
+
+
+@pytest.mark.parametrize("h,hk,d,lens", [(2, 1, 128, [300, 2, 257]), (2, 2, 64, [640]), (3, 1, 40, [127, 0, 1, 128])])
+def test_fp16_gradients_of_any_size(cuda, h, hk, d, lens):
+    """Gradients are linear in dO, and a power of two rounds nothing: what 2^13 dO (whose dS is past fp16's largest value, while
+    the results are not) and 2^-14 dO (whose dS is below its smallest one) give is that of dO times the power, but for the
+    result's own rounding: half a step of both, or of 2^-24 below the normal range."""
+    q, k, v, do = make(sum(lens), h, hk, d, torch.float16, seed=3)
+    with torch.no_grad():
+        q.mul_(0.25), k.mul_(0.25), v.mul_(4)
+    do = in_eighths(do)
+    cu = bounds(lens)
+    want = check(q, k, v, do.half(), cu)
+    for e in (13, -14):
+        got = run(q, k, v, (do * 2.0 ** e).half(), on_device(cu))
+        assert torch.equal(got[0], want[0])
+        for a, b in zip(got[1:], want[1:]):
+            # (a is off by 2^-11 |a| or 2^-25, the larger of them; b was, before its power: 2^-11 |b| or 2^-25 2^e)
+            b = b.double() * 2.0 ** e
+            assert ((a.double() - b).abs() <= 2.0 ** -10 * b.abs() + 2.0 ** -25 * (1 + 2.0 ** e)).all(), e
+
+
+def test_fp16_gradients_of_sequences_of_different_size(cuda):
+    """A sequence whose dO is 2^20 times another's changes nothing of the other's gradients, nor do rows that hold no number."""
+    lens = [200, 300, 150]
+    q, k, v, do = make(sum(lens), 4, 2, 64, torch.float16, seed=4)
+    do = in_eighths(do)
+    do[200:500] *= 2.0 ** 10
+    do[:200] *= 2.0 ** -10
+    do = do.half()
+    cu = bounds(lens)
+    got = run(q, k, v, do, on_device(cu))
+    for s, e in zip(cu[:-1], cu[1:]):
+        alone = run(*(t[s:e].detach().requires_grad_() for t in (q, k, v)), do[s:e])
+        assert all(torch.equal(a[s:e], b) for a, b in zip(got[:2], alone))      # (dk and dv: heads may be shared out otherwise)
+        want, tol = formula(*(t[s:e].detach() for t in (q, k, v)), do[s:e], [0, e - s], 0.125)
+        size = do[s:e].abs().max().double() / 2                  # (the formula's tolerance is for dO of about 1)
+        for a, b, t in zip(got, want, tol):
+            assert ((a[s:e].double() - b).abs() <= t * max(size, 1.0) if s == 200 else (a[s:e].double() - b).abs() <= t).all()
+    bad = do.clone()
+    bad[250, 1, 3], bad[260, 0, 0] = float("nan"), float("inf")
+    dq = run(q, k, v, bad, on_device(cu))[1]
+    keep = torch.ones_like(dq, dtype=torch.bool)
+    keep[250, 1] = keep[260, 0] = False
+    assert torch.equal(dq[keep], got[1][keep]) and not dq[250, 1].isfinite().any()
