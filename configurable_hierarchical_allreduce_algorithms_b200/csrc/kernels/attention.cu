@@ -562,6 +562,9 @@ __device__ __forceinline__ void probabilities(uint32_t* r, uint64_t sl2, uint64_
 // taken out again from fp32 sums.  Only fp16 has it (bf16 has the exponents of fp32).
 template <typename T> constexpr bool kRanged = false;
 template <> constexpr bool kRanged<__half> = true;
+// dkv's own P, the left operand of dV, is kept 2^14 times larger there: a key that many queries give less than 2^-14 each would
+// lose bits of its dV (the sums run over up to T such weights).
+template <typename T> constexpr int kUp = kRanged<T> ? 14 : 0;
 
 struct Range {
   float o = 0.f, v = 0.f;
@@ -954,8 +957,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
   constexpr int ATOMS = DP / 64, TB = ATOMS * kAtom;
   extern __shared__ char smem_raw[];
   __shared__ __align__(8) unsigned long long bars[21];
-  __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: -lse, -D (times the range's power)
-  __shared__ float power_[2];                                         // that power
+  __shared__ __align__(16) float nlse[2][TILE], ndelta[2][TILE];      // of the walked queries: kUp - lse, -D times the next
+  __shared__ float power_[2];                                         // the range's power, less kUp
   __shared__ uint32_t tmem_;
   __shared__ Fault fault;
   __shared__ int last_share;
@@ -1022,7 +1025,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
         if (kRanged<T> && i == 0) {
           Range range;
           for (int u = lane; u < nt; u += 32) range.take(p.sizes + (long long)kvh * p.T + w.start, u, u >= w.unit, true);
-          power = power_of_two(range.power());
+          power = power_of_two(range.power() - kUp<T>);      // (P has the rest)
         }
         // behind the sequence's end P becomes 0
         if (kRanged<T> && one) power_[s2] = power;
@@ -1031,7 +1034,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
           const int r = lane + 32 * j;
           const long long at = (long long)head * p.T + w.start + q0 + r;
           const bool in = q0 + r < w.len;
-          nlse[s2][r] = in ? -__ldcg(p.lse + at) : -INFINITY;
+          nlse[s2][r] = in ? (float)kUp<T> - __ldcg(p.lse + at) : -INFINITY;
           ndelta[s2][r] = in ? -__ldcg(p.delta + at) * power : 0.f;
         }
         __syncwarp();
@@ -1227,7 +1230,8 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
       }
       bar_wait_warp(done, pieces++ & 1, &fault);
       fence_after();
-      const float scale = kRanged<T> ? p.scale / power : p.scale;      // (exact: a power of two)
+      // (exact: powers of two)
+      const float scale_v = 1.f / (float)(1 << kUp<T>), scale_k = kRanged<T> ? p.scale * scale_v / power : p.scale;
       const int first_row = tile * TILE + (warp & 3) * 32;
       const long long at = ((long long)(w.start + first_row) * p.kv_heads + kvh) * p.D * 2, pitch = (long long)p.kv_heads * p.D * 2;
       // 32 columns of dV and of dK a warp, at DP = 64 of one of them
@@ -1238,7 +1242,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
         for (int k = 0; k < kOutputs; ++k) {
           const bool of_k = tensor(k);
-          store_rows<T>(FromTmem{(of_k ? tdk : tdv) + col + lanes}, 32, of_k ? scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
+          store_rows<T>(FromTmem{(of_k ? tdk : tdv) + col + lanes}, 32, of_k ? scale_k : scale_v, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
         }
       } else {
         const int piece = (int)(it.at() / p.split);
@@ -1275,7 +1279,7 @@ attn_dkv(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtenso
 #pragma unroll
               for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(f[c]);
             };
-            store_rows<T>(summed, 32, of_k ? scale : 1.f, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
+            store_rows<T>(summed, 32, of_k ? scale_k : scale_v, stage, (of_k ? p.dk : p.dv) + at, pitch, w.len - first_row, col, p.D);
           }
         }
         meet();      // (last_share is read)

@@ -101,3 +101,23 @@ def test_fp16_gradients_of_sequences_of_different_size(cuda):
     keep = torch.ones_like(dq, dtype=torch.bool)
     keep[250, 1] = keep[260, 0] = False
     assert torch.equal(dq[keep], got[1][keep]) and not dq[250, 1].isfinite().any()
+
+
+def test_fp16_gradient_of_values_with_small_weights(cuda):
+    """A key that every query behind it gives less than 2^-12: its dV is as exact, relative to its size, as any other's."""
+    n, d = 1500, 64
+    q, k, v, do = make(n, 1, 1, d, torch.float16, seed=5)
+    with torch.no_grad():
+        q[:, 0, 0], k[:, 0, 0], k[7, 0, 0] = 8, 0, -8            # (8 * -8 / 8 = -8: 2^-11.5 beside 2^-8 to 2^-11)
+    dv = run(q, k, v, do, on_device([0, n]))[3]
+    Q, K, G = (t.detach().double()[:, 0] for t in (q, k, do))
+    keep = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+    S = (Q @ K.t() / 8).masked_fill(~keep, -float("inf"))
+    P = torch.softmax(S, -1)[100:, 7]                            # (of queries that see more than a hundred keys)
+    full = torch.softmax(S, -1)[:, 7]
+    assert P.max() < 2.0 ** -12
+    E = 2.0 ** -24
+    delta = 2 * d * E / 8 * (Q.abs() @ K.abs().t()).max() + 32 * E * (1 + S[keep].abs().max())
+    size, want = full @ G.abs(), full @ G
+    u = 2.0 ** -11
+    assert ((dv[7, 0].double() - want).abs() <= (u + delta + (n + 16) * E) * size + u * want.abs() + 2.0 ** -25).all()
