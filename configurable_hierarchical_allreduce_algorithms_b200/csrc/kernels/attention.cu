@@ -225,8 +225,9 @@ __device__ __forceinline__ void zero_out(char* base, long long first, int rows, 
 // What bounds the kernel is the chain scores -> softmax -> product of one tile (per tile of 128 x 128: 1024 clocks of products
 // at D = 128, 1024 of the special function unit, and latencies between them), so each tile has a warp of its own for its
 // products, and four warps a scheduler hide the latencies in a softmax (16384 tokens, 16 / 4 heads of 128: 858 us; with two
-// warps a scheduler 1066 us, or 917 us with tile 1 held back by half a turn).  That case runs at 1.28 PFLOP/s.  Short
-// sequences pay for the ends of their pieces: 4 x 2048 tokens, 16 heads of 128, 85 us, 0.81 PFLOP/s; 8 x 1024, 16 of 64, 47 us.
+// warps a scheduler 1066 us, or 917 us with tile 1 held back by half a turn).  That is 1.28 PFLOP/s, the best of replayed passes;
+// calls in a row, under the power limit, run at 1.1 (1000 us).  Short sequences pay for the ends of their pieces: 4 x 2048 tokens,
+// 16 heads of 128, 85 us, 0.81 PFLOP/s; 8 x 1024, 16 of 64, 47 us.
 constexpr int kFwdThreads = 640;
 
 // Whether any of a tile's 256 threads wants it; barrier 1 + tile

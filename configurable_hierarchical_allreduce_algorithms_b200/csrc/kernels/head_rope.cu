@@ -9,8 +9,9 @@
 // 8192 tokens, 16 + 16 heads of 128, bf16: forward 33 us (134 MB, 4.1 TB/s), backward with dw 47 us (201 MB, 4.3 TB/s); latency
 // and the registers that the loads ahead take are what is between that and a copy's 6.5 TB/s.
 // A CTA has queries or keys only, so that a thread sums one weight's gradient.
-// Angles: base^(-2i/D) / 2 pi is a 64-bit fraction of a turn, and position times fraction wraps modulo one turn exactly,
-// so far positions are as exact as near ones; only the angle within the turn is rounded to fp32.
+// Angles: base^(-2i/D) / 2 pi is a 64-bit fraction of a turn, and position times fraction wraps modulo one turn exactly; only the
+// angle within the turn is rounded to fp32.  The fraction is cut at 2^-64, so positions up to about 2^38 are as exact as near ones;
+// each doubling beyond costs a bit.
 #include <math.h>
 
 #include <mutex>

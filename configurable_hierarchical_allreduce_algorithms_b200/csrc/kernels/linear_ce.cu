@@ -612,7 +612,8 @@ ce_weights(const float* grad, int reduction, int N, int D, Saved sv, float* gs, 
 }
 
 // ------------------------------------------------------------------ host side
-// Bytes of G at most.  A launch costs about ten microseconds of its own, so fewer pieces are faster though less of G is in L2
+// Bytes of G at most, as long as that leaves a piece 256 columns: above 393216 rows a piece has 256, and G 512 bytes a row.
+// A launch costs about ten microseconds of its own, so fewer pieces are faster though less of G is in L2
 // when it is read (8192 x 1024 x 50257: 48 MiB 3209 us, 96 MiB 2770, 192 MiB 2612, 384 MiB 2598).
 constexpr long long kPieceBytes = 192ll << 20;
 

@@ -216,8 +216,9 @@ def head_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | No
 
     bf16, fp16 or fp32; D a multiple of 8, at most 256; any strides (views of one projection's output are read in place
     where their heads start on 16-byte boundaries).  ``q_weight``, ``k_weight`` [D]: fp32 or the type of ``q``, both or
-    neither (no norm then).  ``positions``: int32 or int64, any value; None: 0, 1, 2, ...  ``interleaved``: pair i is
-    elements 2i and 2i + 1, else i and i + D / 2.  Returns contiguous tensors of the types of ``q`` and ``k``."""
+    neither (no norm then).  ``positions``: int32 or int64; None: 0, 1, 2, ...  Angles are exact to fp32's rounding within the
+    turn up to positions of about 2^38 of either sign; each doubling beyond costs a bit.  ``interleaved``: pair i is elements
+    2i and 2i + 1, else i and i + D / 2.  Returns contiguous tensors of the types of ``q`` and ``k``."""
     qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
     if len(qs) != 3 or len(ks) != 3 or qs[0] != ks[0] or qs[2] != ks[2] or qs[1] == 0 or ks[1] == 0:
         raise ValueError("head_norm_rope: q [T, H, D] and k [T, Hk, D] expected")
@@ -318,7 +319,9 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (views of one projection's output are read in place where their heads start on 16-byte boundaries).  ``cu_seqlens``
     [B + 1], int32 on the same device: sequence s is the rows cu_seqlens[s] to cu_seqlens[s + 1], ascending from 0 to T at
     most (not checked; bounds are clamped to 0 and T); lengths of zero are fine, rows outside all sequences get zeros and no
-    gradient, and no sequence is reached by what another holds, infinities and NaN included.  None: one sequence.
+    gradient, and no bit of a sequence's result depends on what another holds, infinities and NaN included.  (Within a sequence
+    a weight of zero times an infinity or NaN is NaN: such a value or gradient of a later token reaches the rows of its tile of
+    128.)  None: one sequence.
     ``scale`` (default D ** -0.5) has to be positive.  Returns [T, H, D], contiguous."""
     qs, ks, dtype, dev = q.shape, k.shape, q.dtype, q.device
     if len(qs) != 3 or len(ks) != 3 or v.shape != ks or qs[0] != ks[0] or qs[2] != ks[2]:
