@@ -121,3 +121,67 @@ def test_fp16_gradient_of_values_with_small_weights(cuda):
     size, want = full @ G.abs(), full @ G
     u = 2.0 ** -11
     assert ((dv[7, 0].double() - want).abs() <= (u + delta + (n + 16) * E) * size + u * want.abs() + 2.0 ** -25).all()
+
+
+def test_fp16_captured_and_replayed_on_gradients_of_another_size(cuda):
+    """The range is found on the device: a replay takes that of its own inputs."""
+    q, k, v, do = make(400, 4, 2, 64, torch.float16, seed=9)
+    do = in_eighths(do).half()
+    cu = on_device([0, 150, 150, 390])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(chb.causal_attention(q, k, v, cu), (q, k, v), do)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:                                          # (two graphs of the same call share no workspace)
+        with torch.cuda.graph(graph):
+            outs.append(torch.autograd.grad(chb.causal_attention(q, k, v, cu), (q, k, v), do))
+    for e in (2.0 ** 12, 2.0 ** -22):
+        do *= e
+        cu.copy_(on_device([0, 3, 300, 400]))
+        for graph in graphs:
+            graph.replay()
+        want = run(q, k, v, do, cu)[1:]
+        assert all(t.isfinite().all() and t.any() for t in want)
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_fp16_streams_at_once(cuda):
+    inputs = [make(900, 4, 2, 64, torch.float16, seed=i) for i in range(2)]
+    inputs[1][3].mul_(1000)
+    cus = [on_device([0, 100, 900]), on_device([0, 33, 700, 890])]
+    alone = [run(*inputs[i], cus[i]) for i in range(2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                o = chb.causal_attention(*inputs[i][:3], cus[i])
+                got[i].append((o.detach(), *torch.autograd.grad(o, inputs[i][:3], inputs[i][3])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, alone[i]))
+    chb.check_operators()
+
+
+def test_fp16_offsets_beyond_32_bits(cuda):
+    T, h, d, n = (1 << 18) + 512, 64, 128, 512                # 2.15e9 elements of q and of dO
+    g = torch.Generator(device="cuda").manual_seed(4)
+    last = [torch.randn(n, x, d, generator=g, device="cuda").half() for x in (h, 1, 1, h)]
+    last[3] *= 1000                                           # (the size of the last rows is theirs)
+    big = [torch.zeros(T, x, d, dtype=torch.float16, device="cuda") for x in (h, 1, 1, h)]
+    for b, t in zip(big, last):
+        b[-n:] = t
+    for t in big[:3] + last[:3]:
+        t.requires_grad_()
+    got = run(*big, on_device(list(range(0, T + 1, n))))
+    alone = run(*last)
+    assert all(torch.equal(a[-n:], b) for a, b in zip(got[:2], alone))
+    # (dk and dv sum the heads in another order, as more CTAs share them: the formula's tolerance, n 2^-24 of the sum of sizes
+    # among it, and not the other result's bits)
+    want, tol = formula(*last, [0, n], d ** -0.5)
+    for a, b, t in zip(got, want, tol):
+        assert ((a[-n:].double() - b).abs() <= t).all() and not a[:-n].any()
