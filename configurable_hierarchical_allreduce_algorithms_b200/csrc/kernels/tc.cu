@@ -58,17 +58,15 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, int ndims, const unsi
 }
 
 unsigned* status_word() {
-  static std::mutex mu;
-  static unsigned* known[kDevices] = {};
+  // (no lock: it could throw through the C entries; two threads that both ask get the same answer)
+  static std::atomic<unsigned*> known[kDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return nullptr;
-  std::lock_guard<std::mutex> g(mu);
-  if (!known[dev]) {
-    void* p = nullptr;
-    if (cudaGetSymbolAddress(&p, g_status) != cudaSuccess) return nullptr;
-    known[dev] = static_cast<unsigned*>(p);
-  }
-  return known[dev];
+  if (unsigned* p = known[dev].load(std::memory_order_relaxed)) return p;
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_status) != cudaSuccess) return nullptr;
+  known[dev].store(static_cast<unsigned*>(p), std::memory_order_relaxed);
+  return static_cast<unsigned*>(p);
 }
 
 int sm_count() {
